@@ -5,6 +5,8 @@
 // reference binding (agent_workdir/kernels/axpby_binding.cpp:1-5).
 #pragma once
 
+#include <string>
+
 #include <torch/types.h>
 #include <torch/csrc/utils/pybind.h>
 #include <cuda_runtime.h>
@@ -33,6 +35,10 @@ inline void check_status(int status, const char* op) {
 }
 
 inline cudaStream_t current_stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+
+// Numbers go into error messages as text: a module that was linked with its own copy of the C++ runtime must not
+// format them through a stream.
+inline std::string text(long long v) { return std::to_string(v); }
 
 template <typename T>
 inline T* ptr(const torch::Tensor& t) {

@@ -49,7 +49,8 @@ torch::Tensor mla_sparse_decode_forward(torch::Tensor q, torch::Tensor kv, torch
                                                 bytes ? scratch.data_ptr() : nullptr, ptr<int>(status), config,
                                                 current_stream()),
                "mla_sparse_decode_forward");
-  if (check) TORCH_CHECK(status.item<int>() == 0, "mla_sparse_decode: a bounded wait gave up (code ", status.item<int>(), ")");
+  if (check) TORCH_CHECK(status.item<int>() == 0, "mla_sparse_decode: a bounded wait gave up (code ",
+                         cab_binding::text(status.item<int>()), ")");
   return out;
 }
 

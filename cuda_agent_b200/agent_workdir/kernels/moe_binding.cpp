@@ -181,10 +181,10 @@ torch::Tensor moe_forward(torch::Tensor x, torch::Tensor router_w, torch::Tensor
   if (check) {
     auto st = tables.slice(0, tables.numel() - 2).cpu();
     TORCH_CHECK(st[0].item<int>() == 0 && st[1].item<int>() == 0, "moe_forward: a GEMM kernel gave up a bounded wait (codes ",
-                st[0].item<int>(), ", ", st[1].item<int>(), ")");
+                cab_binding::text(st[0].item<int>()), ", ", cab_binding::text(st[1].item<int>()), ")");
     auto flag = scratch.cpu();
     const int permute_flag = reinterpret_cast<const int*>(flag.data_ptr<uint8_t>())[flag.numel() / 4 - 1];
-    TORCH_CHECK(permute_flag == 0, "moe_forward: permutation flagged code ", permute_flag);
+    TORCH_CHECK(permute_flag == 0, "moe_forward: permutation flagged code ", cab_binding::text(permute_flag));
     if (has_shared) {
       auto ss = shared_status.cpu();
       TORCH_CHECK(ss[0].item<int>() == 0 && ss[1].item<int>() == 0, "moe_forward: shared-expert GEMM gave up a wait");

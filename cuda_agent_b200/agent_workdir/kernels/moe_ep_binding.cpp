@@ -45,7 +45,7 @@ int64_t g_next = 1;
 
 Handle& lookup(int64_t h) {
   auto it = g_handles.find(h);
-  TORCH_CHECK(it != g_handles.end(), "moe_ep: unknown handle ", h);
+  TORCH_CHECK(it != g_handles.end(), "moe_ep: unknown handle ", cab_binding::text(h));
   return it->second;
 }
 
@@ -149,7 +149,7 @@ torch::Tensor moe_ep_forward(int64_t h, torch::Tensor x, torch::Tensor router_w,
     int st[8];
     check_status(moe_ep_peer_read_status(hd.ctx, &hd.args, hd.workspace.data_ptr(), st), "moe_ep_peer_read_status");
     for (int i = 0; i < 8; ++i)
-      TORCH_CHECK(st[i] == 0, "moe_ep_forward: status word ", i, " = ", st[i],
+      TORCH_CHECK(st[i] == 0, "moe_ep_forward: status word ", cab_binding::text(i), " = ", cab_binding::text(st[i]),
                   " (0-3 GEMM waits, 4 permutation, 5 wait for dispatches, 6 wait for returns)");
   }
   return out;
