@@ -7,6 +7,8 @@
 // validate, allocate output and scratch with torch::empty, current stream, launcher.
 #include "binding_common.h"
 
+void register_mla_paged(pybind11::module& m);   // mla_paged_binding.cpp
+
 namespace {
 using cab_binding::check_cuda_contig;
 using cab_binding::check_status;
@@ -71,6 +73,7 @@ void register_mla(pybind11::module& m) {
         py::arg("idx"), py::arg("softmax_scale"), py::arg("nsplit") = 0, py::arg("check") = false,
         py::arg("config") = 0);
   m.def("mla_gather_rows", &mla_gather_rows, py::arg("kv"), py::arg("seq_len"), py::arg("idx"));
+  register_mla_paged(m);
 }
 }  // namespace
 

@@ -1,0 +1,781 @@
+// Dense latent attention of each sequence's new tokens over its rows of a paged cache:
+//   s_j = scale * q . c_j (576 columns),  out = sum_j softmax(s)_j c_j[:512],  lse = log sum_j exp(s_j)
+// over the rows that the token may see (causal, window, length). All heads read the same rows, so the (token,
+// head) pairs of a sequence are the rows of one matrix, and 128 of them make a tile whatever the head count:
+// one token with 128 heads, eight tokens with 16, or a decode step's 16 rows in a tile that is mostly empty.
+//
+// A tile of 128 rows times 512 value columns of fp32 would take all of tensor memory, so two CTAs share a tile:
+// each accumulates 256 of the value columns and computes the scores for itself (832 column steps instead of
+// 544; the alternative, exchanging partial scores between the CTAs, costs more than the second Q.K^T here).
+// Tensor memory: O 256 columns, S two buffers of 64, 256 columns of Q as the A operand in 128. P (16 bit)
+// overwrites the S it came from and is the A operand of P.V. Shared memory: the other 320 columns of Q (80 KB)
+// and two rings for blocks of 64 cache rows: 64-column tiles that only Q.K^T reads (six of 8 KB), and this
+// CTA's 256 value columns, which P.V reads as well (three blocks of 32 KB). A tile slot is released as soon as
+// its last reader is done, so every load has about a block's time to land.
+//   warps 0-3  one (token, head) row per thread: Q, softmax, result. The reference maximum of a row moves only
+//              when it would grow by more than 2^8, so O is hardly ever rescaled
+//   warp 4     issues Q.K^T of block j+1 before P.V of block j: the tensor core works while the softmax does
+//   warp 5     TMA: one box per run of rows that lie in one page
+// The work of a call (tiles x blocks of 64 rows) is cut into equal runs, one for each pair of CTAs, wherever
+// that cuts a tile; each CTA finds its run itself from q_start and kv_len. Tiles cut by a boundary leave
+// unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
+// Every wait is bounded.
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "cab_common.cuh"
+#include "sm100_primitives.cuh"
+
+namespace {
+
+constexpr int kD = 576, kDv = 512, kHalf = 256;
+constexpr int kRows = 128;                     // (token, head) rows per tile
+constexpr int kKeys = 64;                      // cache rows per block
+constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 128-byte swizzle
+constexpr int kNTiles = 5, kVTiles = 4;        // tiles of a block: the other value half and the rotary columns / own half
+constexpr int kNSlots = 6, kVSlots = 3;
+constexpr int kQChunk = kRows * 128;
+constexpr int kThreads = 6 * 32;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384, kTmemCols = 512;
+constexpr float kRescale = 8.f;
+constexpr int kMaxBatch = 16384;
+enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitDrain };
+
+struct __align__(16) Control {
+  uint64_t n_full[kNSlots], n_empty[kNSlots], v_full[kVSlots], v_empty[kVSlots], s_full[2], p_full[2], pv_done[2], q_ready;
+  long long scan[kThreads / 32], total;
+  long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
+  int seq, tile;                               // its first tile
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr int kRingBytes = kNSlots * kTile + kVSlots * kVTiles * kTile;
+constexpr int kSmemBytes = kNTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
+static_assert(kSmemBytes <= 232448 && (kMaxBatch + 2) * 4 <= kRingBytes, "shared memory");
+
+// What the merge kernel has to know of the tile that a pair ends: its first (token, head) row, its rows, the pair
+// that holds its first part, and the work of the whole call (which says what runs are empty).
+struct Meta { long long row0, total; int rows, first; };
+
+struct Params {
+  const void* q;
+  void* out;
+  float* lse;
+  const int *page_table, *q_start, *kv_len;
+  int T, H, batch, max_pages, num_pages, page_size, box;
+  int tail;                                    // write the tokens behind the last sequence as such that see nothing
+  int causal, window, rows_cap, pairs;
+  float scale_log2;
+  float* part_o;                               // [pair][2][rows_cap][512]
+  float* part_ml;                              // [pair][2][half][rows_cap][2]
+  Meta* meta;                                  // [pair]
+  int* status;
+};
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t lbo) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fff) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
+// A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
+struct Seq { int tok, n, len, pos; };
+__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
+  Seq s;
+  const int a = min(max(__ldg(p.q_start + b), 0), p.T);
+  const int e = min(max(__ldg(p.q_start + b + 1), a), p.T);
+  s.tok = a;
+  s.n = e - a;
+  s.len = (int)min((long long)max(__ldg(p.kv_len + b), 0), (long long)p.max_pages * p.page_size);
+  s.pos = s.len - s.n;
+  return s;
+}
+__device__ __forceinline__ int tiles_of(const Params& p, int n) {
+  return (int)(((long long)n * p.H + kRows - 1) / kRows);
+}
+// Blocks [first, first + count) of 64 cache rows that some row of tile i sees; `units` = max(count, 1) is what
+// the tile counts as when the work is divided, so that a tile that sees nothing is still written.
+struct Item { long long row0; int rows, first, count, units; };
+__device__ __forceinline__ Item item_of(const Params& p, const Seq& s, int i) {
+  Item t;
+  const long long r0 = (long long)i * kRows, r1 = min(r0 + kRows, (long long)s.n * p.H);
+  t.row0 = (long long)s.tok * p.H + r0;
+  t.rows = (int)(r1 - r0);
+  const int t0 = (int)(r0 / p.H), t1 = (int)((r1 - 1) / p.H);
+  const int hi = p.causal ? min(s.len, s.pos + t1 + 1) : s.len;
+  const int lo = p.window > 0 ? (int)max(0LL, (long long)s.pos + t0 + 1 - p.window) : 0;
+  t.first = lo / kKeys;
+  t.count = hi > lo ? (hi + kKeys - 1) / kKeys - t.first : 0;
+  t.units = max(t.count, 1);
+  return t;
+}
+
+// The run of a pair as a sequence of tiles, walked in the same way by every role.
+struct Walk {
+  int b, i;
+  long long x, x1, item_x;
+  Seq s;
+  Item t;
+  int u0, u1;                                  // units of the tile that belong to this run
+  __device__ __forceinline__ Walk(const Params& p, const Control& c)
+      : b(c.seq), i(c.tile), x(c.x0), x1(c.x1), item_x(c.item_x) {
+    if (x < x1) load(p);
+  }
+  __device__ __forceinline__ void load(const Params& p) {
+    s = seq_of(p, b);
+    t = item_of(p, s, i);
+    u0 = (int)(x - item_x);
+    u1 = (int)min((long long)t.units, x1 - item_x);
+  }
+  __device__ __forceinline__ bool live() const { return x < x1; }
+  __device__ __forceinline__ void next(const Params& p) {
+    x = item_x + u1;
+    if (x >= x1) return;
+    item_x += t.units;
+    ++i;
+    while (b < p.batch && i >= tiles_of(p, s.n)) {
+      i = 0;
+      if (++b < p.batch) s = seq_of(p, b);
+    }
+    if (b >= p.batch) { x = x1; return; }
+    load(p);
+  }
+  // blocks of this segment, as block numbers of the sequence
+  __device__ __forceinline__ int begin() const { return t.first + u0; }
+  __device__ __forceinline__ int blocks() const { return t.count == 0 ? 0 : u1 - u0; }
+  __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == t.units; }
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
+  const bool ok = sm100::mbar_wait(bar, parity, abort_flag, status, where);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// Exclusive scan over the CTA's threads; the sum of all goes to ctl.total.
+__device__ __forceinline__ long long block_scan(Control& ctl, long long v) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) ctl.scan[warp] = x;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += ctl.scan[w];
+    all += ctl.scan[w];
+  }
+  if (threadIdx.x == 0) ctl.total = all;
+  __syncthreads();
+  return before + x - v;
+}
+
+// Where pair `pair` begins: thread-parallel over the sequences, then over the tiles. `pre`: batch + 1 ints of
+// shared memory that nothing else uses yet.
+__device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
+  const int tid = threadIdx.x;
+  {
+    const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+    long long sum = 0;
+    for (int b = b0; b < b1; ++b) sum += tiles_of(p, seq_of(p, b).n);
+    long long at = block_scan(ctl, sum);
+    for (int b = b0; b < b1; ++b) {
+      pre[b] = (int)min(at, (long long)0x7fffffff);
+      at += tiles_of(p, seq_of(p, b).n);
+    }
+  }
+  const int tiles = (int)min(ctl.total, (long long)0x7fffffff);
+  if (tid == 0) pre[p.batch] = tiles;
+  if (tid == 0) { ctl.x0 = ctl.x1 = ctl.item_x = 0; ctl.seq = ctl.tile = 0; }
+  __syncthreads();
+  const int per = (tiles + kThreads - 1) / kThreads;
+  const int i0 = (int)min((long long)tid * per, (long long)tiles), i1 = min(i0 + per, tiles);
+  int b = 0;
+  if (i0 < i1) {                               // last b with pre[b] <= i0
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= i0) lo = mid; else hi = mid;
+    }
+    b = lo;
+  }
+  long long sum = 0;
+  if (i0 < i1) {
+    int bb = b;
+    Seq s = seq_of(p, bb);
+    for (int i = i0; i < i1; ++i) {
+      while (pre[bb + 1] <= i) s = seq_of(p, ++bb);
+      sum += item_of(p, s, i - pre[bb]).units;
+    }
+  }
+  long long at = block_scan(ctl, sum);
+  const long long W = ctl.total, x0 = W * pair / p.pairs, x1 = W * (pair + 1) / p.pairs;
+  if (x0 < x1 && at <= x0 && x0 < at + sum) {
+    Seq s = seq_of(p, b);
+    for (int i = i0; i < i1; ++i) {
+      while (pre[b + 1] <= i) s = seq_of(p, ++b);
+      const Item t = item_of(p, s, i - pre[b]);
+      if (x0 < at + t.units) {
+        ctl.x0 = x0; ctl.x1 = x1; ctl.item_x = at; ctl.seq = b; ctl.tile = i - pre[b];
+        // the pair that ends a cut tile says so to the merge kernel
+        Meta m{t.row0, W, 0, 0};
+        if (x0 > at && at + t.units <= x1) {
+          m.rows = t.rows;
+          int f = pair - 1;
+          while (f > 0 && W * f / p.pairs > at) --f;
+          m.first = f;
+        }
+        if ((blockIdx.x & 1) == 0) p.meta[pair] = m;
+        break;
+      }
+      at += t.units;
+    }
+  }
+  if (x0 >= x1 && tid == 0 && (blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0, 0};
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_smem = base;
+  uint8_t* n_ring = base + kNTiles * kQChunk;
+  uint8_t* v_ring = n_ring + kNSlots * kTile;
+  Control& ctl = *reinterpret_cast<Control*>(v_ring + kVSlots * kVTiles * kTile);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kNSlots; ++s) { sm100::mbar_init(&ctl.n_full[s], 1); sm100::mbar_init(&ctl.n_empty[s], 1); }
+    for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_full[s], 1); sm100::mbar_init(&ctl.v_empty[s], 1); }
+    // by block parity. pv_done too: a softmax thread may wait for P.V of block j while that of j - 1 is not done
+    for (int s = 0; s < 2; ++s) {
+      sm100::mbar_init(&ctl.s_full[s], 1);
+      sm100::mbar_init(&ctl.p_full[s], 4);
+      sm100::mbar_init(&ctl.pv_done[s], 1);
+    }
+    sm100::mbar_init(&ctl.q_ready, 4);
+    ctl.abort_flag = 0;
+    sm100::mbar_fence_init();
+  }
+  if (warp == 4) {
+    sm100::tmem_alloc(&ctl.tmem_base, kTmemCols);
+    sm100::tmem_relinquish();
+  }
+  if (warp == 5 && lane == 0) sm100::prefetch_tensormap(&map);
+  find_run(p, ctl, reinterpret_cast<int*>(n_ring), pair);
+  sm100::fence_proxy_async();                  // the rings were used as scratch
+  sm100::tc_fence_before_sync();
+  __syncthreads();
+  sm100::tc_fence_after_sync();
+  const uint32_t tmem = ctl.tmem_base;
+  volatile int* abort_flag = &ctl.abort_flag;
+  constexpr uint32_t kFmt = std::is_same_v<T, __half> ? 0 : 1;
+
+  if (warp == 5) {
+    // ---------------------------------------------------------------- loads
+    uint32_t n_at = 0, v_at = 0;               // tiles / blocks loaded so far
+    bool ok = true;
+    const int other = half ? 0 : 4;            // first of the four column tiles of the other value half
+    for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
+      const int* table = p.page_table + (size_t)w.b * p.max_pages;
+      const int nb = w.blocks();
+      // page and row in the page of this lane's boxes (two when a box is a single row), one block ahead
+      int page[2], row[2];
+      auto look = [&](int j) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const long long key = (long long)j * kKeys + (lane + 32 * k) * p.box;
+          page[k] = p.num_pages;               // outside the pool: TMA fills with zeros
+          row[k] = 0;
+          if ((lane + 32 * k) * p.box < kKeys && key < w.s.len) {
+            const int at = (int)(key / p.page_size);
+            row[k] = (int)(key - (long long)at * p.page_size);
+            page[k] = __ldg(table + at);
+          }
+        }
+      };
+      if (nb > 0) look(w.begin());
+      for (int k = 0; k < nb && ok; ++k) {
+        const int j = w.begin() + k;
+        const int boxes = (min(kKeys, w.s.len - j * kKeys) + p.box - 1) / p.box;
+        int pg[2], rw[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          pg[e] = page[e];
+          rw[e] = row[e];
+          if (lane + 32 * e < boxes && ((unsigned)pg[e] >= (unsigned)p.num_pages)) {
+            if (p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
+            pg[e] = p.num_pages;
+            rw[e] = 0;
+          }
+        }
+        if (k + 1 < nb) look(j + 1);
+        auto issue = [&](uint8_t* dst, uint64_t* bar, int col) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (lane + 32 * e < boxes)
+              tma_load_3d(sm100::smem_u32(dst) + (lane + 32 * e) * p.box * 128, &map, bar, col, rw[e], pg[e]);
+        };
+        for (int c = 0; c < kNTiles; ++c, ++n_at) {
+          const uint32_t s = n_at % kNSlots, use = n_at / kNSlots;
+          if (use > 0 && !warp_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree)) { ok = false; break; }
+          if (lane == 0) sm100::mbar_arrive_expect_tx(&ctl.n_full[s], boxes * p.box * 128);
+          __syncwarp();
+          issue(n_ring + s * kTile, &ctl.n_full[s], 64 * (c < 4 ? other + c : 8));
+        }
+        if (!ok) break;
+        const uint32_t s = v_at % kVSlots, use = v_at / kVSlots;
+        if (use > 0 && !warp_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree)) { ok = false; break; }
+        if (lane == 0) sm100::mbar_arrive_expect_tx(&ctl.v_full[s], kVTiles * boxes * p.box * 128);
+        __syncwarp();
+        for (int c = 0; c < kVTiles; ++c) issue(v_ring + (s * kVTiles + c) * kTile, &ctl.v_full[s], 64 * (4 - other + c));
+        ++v_at;
+      }
+    }
+    if (!ok) {                                 // giving up: copies in flight land before the CTA may end
+      int never = 0;
+      for (uint32_t i = n_at > kNSlots ? n_at - kNSlots : 0; i < n_at; ++i)
+        sm100::mbar_wait_limited(&ctl.n_full[i % kNSlots], (i / kNSlots) & 1, &never, nullptr, kWaitDrain, 200000000LL);
+      for (uint32_t i = v_at > kVSlots ? v_at - kVSlots : 0; i < v_at; ++i)
+        sm100::mbar_wait_limited(&ctl.v_full[i % kVSlots], (i / kVSlots) & 1, &never, nullptr, kWaitDrain, 200000000LL);
+    }
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- tensor core
+    constexpr uint32_t idesc_qk = sm100::umma_idesc(kFmt, kRows, kKeys);
+    constexpr uint32_t idesc_pv = sm100::umma_idesc(kFmt, kRows, kHalf) | (1u << 16);   // V: keys down, columns along
+    const uint32_t q_addr = sm100::smem_u32(q_smem), n_addr = sm100::smem_u32(n_ring), v_addr = sm100::smem_u32(v_ring);
+    uint32_t n_at = 0, g_qk = 0, g_pv = 0, seg = 0;
+    bool ok = true;
+    for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
+      const int nb = w.blocks();
+      if (nb == 0) continue;
+      if (!warp_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ)) { ok = false; break; }
+      ++seg;
+      sm100::tc_fence_after_sync();
+      for (int k = 0; k <= nb && ok; ++k) {
+        if (k < nb) {                          // S = Q . K^T of block k
+          const uint32_t d = tmem + kColS + (g_qk & 1) * kKeys;
+          for (int c = 0; c < kNTiles; ++c, ++n_at) {
+            const uint32_t s = n_at % kNSlots;
+            if (!warp_wait(&ctl.n_full[s], (n_at / kNSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
+            if (lane == 0) {
+              const uint64_t a = desc_sw128(q_addr + c * kQChunk, 16), b = desc_sw128(n_addr + s * kTile, 16);
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) sm100::umma_f16(d, a + 2 * k4, b + 2 * k4, idesc_qk, (c > 0 || k4 > 0) ? 1u : 0u);
+              sm100::umma_commit(&ctl.n_empty[s]);
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          const uint32_t s = g_qk % kVSlots;
+          if (!warp_wait(&ctl.v_full[s], (g_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
+          const int valid = w.s.len - (w.begin() + k) * kKeys;
+          if (valid < kKeys) {
+            // rows behind the sequence's end may hold anything, also NaN, which a weight of zero would keep
+            uint8_t* v = v_ring + s * kVTiles * kTile;
+            for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)
+#pragma unroll
+              for (int c = 0; c < kVTiles; ++c) *reinterpret_cast<uint4*>(v + c * kTile + e * 16) = make_uint4(0, 0, 0, 0);
+            sm100::fence_proxy_async();
+            __syncwarp();
+          }
+          if (lane == 0) {
+#pragma unroll
+            for (int c = 0; c < kVTiles; ++c) {
+              const uint64_t b = desc_sw128(v_addr + (s * kVTiles + c) * kTile, 16);
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) umma_ts(d, tmem + kColQ + c * 32 + k4 * 8, b + 2 * k4, idesc_qk, 1u);
+            }
+            sm100::umma_commit(&ctl.s_full[g_qk & 1]);
+          }
+          __syncwarp();
+          ++g_qk;
+        }
+        if (k > 0) {                           // O += P . V of block k - 1
+          const uint32_t sb = g_pv & 1, s = g_pv % kVSlots;
+          if (!warp_wait(&ctl.p_full[sb], (g_pv >> 1) & 1, abort_flag, p.status, kWaitP)) { ok = false; break; }
+          sm100::tc_fence_after_sync();
+          if (lane == 0) {
+            const uint64_t b = desc_sw128(v_addr + s * kVTiles * kTile, kTile);
+#pragma unroll
+            for (int k4 = 0; k4 < kKeys / 16; ++k4)
+              umma_ts(tmem + kColO, tmem + kColS + sb * kKeys + k4 * 8, b + (uint64_t)k4 * (2048 >> 4), idesc_pv,
+                      (k > 1 || k4 > 0) ? 1u : 0u);
+            sm100::umma_commit(&ctl.v_empty[s]);
+            sm100::umma_commit(&ctl.pv_done[sb]);
+          }
+          __syncwarp();
+          ++g_pv;
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax, one row per thread
+    const int row = threadIdx.x;
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const T* q = static_cast<const T*>(p.q);
+    uint32_t g = 0;
+    bool ok = true;
+    const int own = half * kHalf, oth = kHalf - own;
+    auto load_q = [&](const Walk& w) {
+      const T* rows = q + w.t.row0 * kD;
+      const uint32_t dst = sm100::smem_u32(q_smem);
+      // the other half and the rotary columns (32 + 8 pieces of 16 bytes a row) as five swizzled tiles; a warp
+      // copies its own 32 rows
+#pragma unroll 8
+      for (int e = lane; e < 32 * 40; e += 32) {
+        const int r = warp * 32 + e / 40, c = e % 40, chunk = c >> 3;
+        cp_async_16(dst + chunk * kQChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                    rows + (r < w.t.rows ? (size_t)r * kD : 0) + (c < 32 ? oth + c * 8 : kDv + (c - 32) * 8), r < w.t.rows);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      const uint4* src = reinterpret_cast<const uint4*>(rows + (size_t)min(row, w.t.rows - 1) * kD + own);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t u[32];
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          uint4 x = __ldg(src + c * 8 + v);
+          if (row >= w.t.rows) x = make_uint4(0, 0, 0, 0);
+          u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
+        }
+        tmem_st_32x32(lanes + kColQ + c * 32, u);
+      }
+      tmem_st_wait();
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      sm100::fence_proxy_async();
+      sm100::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&ctl.q_ready);
+    };
+
+    Walk w(p, ctl);
+    if (w.live() && w.blocks() > 0) load_q(w);
+    while (w.live() && ok) {
+      const int nb = w.blocks();
+      // what this row sees: cache rows [lo, hi)
+      const int tok = (int)((w.t.row0 + row) / p.H) - w.s.tok;
+      const bool live = row < w.t.rows;
+      int hi = p.causal ? min(w.s.len, w.s.pos + tok + 1) : w.s.len;
+      const int lo = p.window > 0 ? (int)max(0LL, (long long)w.s.pos + tok + 1 - p.window) : 0;
+      if (!live) hi = 0;
+      const bool warp_live = warp * 32 < w.t.rows;
+      float m_ref = -INFINITY, l_sum = 0.f;
+      for (int k = 0; k < nb; ++k, ++g) {
+        const uint32_t sb = g & 1;
+        if (!warp_wait(&ctl.s_full[sb], (g >> 1) & 1, abort_flag, p.status, kWaitS)) { ok = false; break; }
+        sm100::tc_fence_after_sync();
+        if (warp_live) {
+          uint32_t u0[32], u1[32];
+          sm100::tmem_ld_32x32(lanes + kColS + sb * kKeys, u0);
+          sm100::tmem_ld_32x32(lanes + kColS + sb * kKeys + 32, u1);
+          sm100::tmem_ld_wait();
+          const int key0 = (w.begin() + k) * kKeys;
+          if (!__all_sync(0xffffffffu, lo <= key0 && key0 + kKeys <= hi)) {
+            const unsigned a = (unsigned)(key0 - lo), span = hi > lo ? (unsigned)(hi - lo) : 0u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (a + i >= span) u0[i] = 0xff800000u;
+              if (a + 32 + i >= span) u1[i] = 0xff800000u;
+            }
+          }
+          float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            m0 = fmaxf(m0, __uint_as_float(u0[i]));
+            m1 = fmaxf(m1, __uint_as_float(u1[i]));
+          }
+          const float m_blk = fmaxf(m0, m1) * p.scale_log2;      // scale > 0: the maximum commutes with it
+          float factor = 1.f;
+          if (m_blk > -INFINITY) {
+            if (m_ref == -INFINITY) {
+              m_ref = m_blk;                   // O is zero or not begun: nothing to rescale
+            } else if (m_blk > m_ref + kRescale) {
+              factor = exp2_approx(m_ref - m_blk);
+              m_ref = m_blk;
+            }
+          }
+          const float neg = m_ref == -INFINITY ? 0.f : -m_ref;   // masked scores: exp2(-inf) = 0
+          uint32_t pk[32];
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float a = exp2_approx(fmaf(__uint_as_float(u0[i]), p.scale_log2, neg));
+            const float b = exp2_approx(fmaf(__uint_as_float(u0[i + 1]), p.scale_log2, neg));
+            const float c = exp2_approx(fmaf(__uint_as_float(u1[i]), p.scale_log2, neg));
+            const float d = exp2_approx(fmaf(__uint_as_float(u1[i + 1]), p.scale_log2, neg));
+            s0 += a + b;
+            s1 += c + d;
+            // P is rounded to the cache's 16-bit type, the only form the tensor core takes beside it: half a
+            // step of 2^-8 (bf16) or 2^-11 (fp16) per weight, as much as the rounding of the result itself
+            pk[i >> 1] = pack2<T>(a, b);
+            pk[16 + (i >> 1)] = pack2<T>(c, d);
+          }
+          l_sum = l_sum * factor + (s0 + s1);
+          if (__any_sync(0xffffffffu, factor != 1.f)) {
+            // only from the second block of a segment on: O holds the blocks up to k - 1
+            if (!warp_wait(&ctl.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
+            sm100::tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < kHalf; c += 32) {
+              uint32_t o[32];
+              sm100::tmem_ld_32x32(lanes + kColO + c, o);
+              sm100::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+              tmem_st_32x32(lanes + kColO + c, o);
+            }
+          }
+          tmem_st_32x32(lanes + kColS + sb * kKeys, pk);
+          tmem_st_wait();
+        }
+        sm100::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&ctl.p_full[sb]);
+      }
+      if (!ok) break;
+      // Q of the next tile may go in as soon as the last scores are out
+      Walk nx = w;
+      nx.next(p);
+      if (nx.live() && nx.blocks() > 0) load_q(nx);
+      if (nb > 0) {
+        if (!warp_wait(&ctl.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
+        sm100::tc_fence_after_sync();
+      }
+      if (warp_live) {
+        const bool any = nb > 0;
+        if (w.whole()) {
+          const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;    // NaN stays NaN
+          const bool zero = l_sum == 0.f;
+          T* dst = static_cast<T*>(p.out) + (w.t.row0 + row) * kDv + own;
+#pragma unroll 1
+          for (int c = 0; c < kHalf; c += 32) {
+            uint32_t o[32];
+            if (any) { sm100::tmem_ld_32x32(lanes + kColO + c, o); sm100::tmem_ld_wait(); }
+            if (live) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint32_t x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  x[k] = zero ? 0u : pack2<T>(__uint_as_float(o[8 * v + 2 * k]) * inv, __uint_as_float(o[8 * v + 2 * k + 1]) * inv);
+                *reinterpret_cast<uint4*>(dst + c + 8 * v) = make_uint4(x[0], x[1], x[2], x[3]);
+              }
+            }
+          }
+          if (live && half == 0 && p.lse)
+            p.lse[w.t.row0 + row] = zero ? -INFINITY : m_ref * 0.6931471805599453f + logf(l_sum);
+        } else {
+          const size_t slot = (size_t)pair * 2 + (w.u0 == 0 ? 1 : 0);
+          float* dst = p.part_o + (slot * p.rows_cap + row) * kDv + own;
+#pragma unroll 1
+          for (int c = 0; c < kHalf; c += 32) {
+            uint32_t o[32];
+            sm100::tmem_ld_32x32(lanes + kColO + c, o);          // a cut tile has at least one block in each part
+            sm100::tmem_ld_wait();
+            if (live) {
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<uint4*>(dst + c + 4 * v) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            }
+          }
+          if (live)
+            *reinterpret_cast<float2*>(p.part_ml + ((slot * 2 + half) * p.rows_cap + row) * 2) = make_float2(m_ref, l_sum);
+        }
+      }
+      sm100::tc_fence_before_sync();           // O was read: the next tile's first P.V comes after these threads' next p_full
+      w = nx;
+    }
+    if (p.tail && ok) {                        // a warp per row; outside the division of work, so that padding does not move its cuts
+      const long long end = (long long)p.T * p.H;
+      for (long long r = (long long)min(max(__ldg(p.q_start + p.batch), 0), p.T) * p.H + blockIdx.x * 4 + warp; r < end;
+           r += gridDim.x * 4) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * kDv);
+        dst[lane] = dst[lane + 32] = make_uint4(0, 0, 0, 0);
+        if (lane == 0 && p.lse) p.lse[r] = -INFINITY;
+      }
+    }
+  }
+
+  sm100::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 4) {
+    sm100::tc_fence_after_sync();
+    sm100::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own maximum m_k.
+// One CTA per row, four columns per thread; parts in the order of the pairs.
+template <typename T>
+__global__ void __launch_bounds__(128) mla_paged_merge_kernel(const Params p) {
+  const int pair = blockIdx.x, row = blockIdx.y;
+  const Meta m = p.meta[pair];
+  if (row >= m.rows) return;
+  const int col = threadIdx.x * 4, half = col >= kHalf;
+  auto slot_of = [&](int k) { return (size_t)k * 2 + (k == m.first ? 1 : 0); };
+  auto empty = [&](int k) { return m.total * k / p.pairs == m.total * (k + 1) / p.pairs; };
+  float top = -INFINITY;
+  for (int k = m.first; k <= pair; ++k) {
+    if (empty(k)) continue;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot_of(k) * 2 + half) * p.rows_cap + row) * 2);
+    if (ml.y != 0.f) top = fmaxf(top, ml.x);
+  }
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int k = m.first; k <= pair; ++k) {
+    if (empty(k)) continue;
+    const size_t slot = slot_of(k);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot * 2 + half) * p.rows_cap + row) * 2);
+    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (slot * p.rows_cap + row) * kDv + col);
+    const float f = ml.y != 0.f ? exp2_approx(ml.x - top) : 0.f;
+    if (f != 0.f) {                            // also true for NaN
+      acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+      l += f * ml.y;
+    }
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const bool zero = l == 0.f;
+  uint2 r;
+  r.x = zero ? 0u : pack2<T>(acc.x * inv, acc.y * inv);
+  r.y = zero ? 0u : pack2<T>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (m.row0 + row) * kDv + col) = r;
+  if (threadIdx.x == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
+}
+
+constexpr int kPairs = cab::kNumSMs / 2;       // the workspace is sized for this many, a smaller device runs fewer
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+int rows_cap_of(int T, int H) { return (int)((long long)T * H < kRows ? (long long)T * H : kRows); }
+
+template <typename T>
+int launch(Params& p, const CUtensorMap& map, cudaStream_t stream) {
+  if (!cab::ensure_dynamic_smem<&mla_paged_attention_kernel<T>>(kSmemBytes)) return CAB_ERR_LAUNCH;
+  mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, map);
+  const int rc = cab::launch_status();
+  if (rc != CAB_OK || p.pairs == 1) return rc;
+  mla_paged_merge_kernel<T><<<dim3(p.pairs, p.rows_cap), 128, 0, stream>>>(p);
+  return cab::launch_status();
+}
+
+}  // namespace
+
+extern "C" size_t mla_paged_attention_workspace_bytes(int T, int H) {
+  if (T <= 0 || H <= 0) return 0;
+  const size_t rows = (size_t)kPairs * 2 * rows_cap_of(T, H);
+  return align256(rows * kDv * 4) + align256(rows * 2 * 2 * 4) + align256(kPairs * sizeof(Meta));
+}
+
+extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q, const cab_mla_paged_batch* batch, int T,
+                                            int H, float softmax_scale, int causal, int window, void* workspace,
+                                            size_t workspace_bytes, int* status, int config, cudaStream_t stream) {
+  if (T < 0 || H <= 0 || !batch || batch->batch < 0) return CAB_ERR_BAD_ARGUMENT;
+  const bool tail = (config & 256) != 0;
+  if (T == 0 || (batch->batch == 0 && !tail)) {
+    if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
+    return CAB_OK;
+  }
+  if (!out || !q || !workspace || !batch->rows || !batch->q_start ||
+      (batch->batch > 0 && (!batch->page_table || !batch->kv_len)))
+    return CAB_ERR_BAD_ARGUMENT;
+  if (batch->num_pages <= 0 || batch->page_size <= 0 || batch->max_pages <= 0 || window < 0 || !(softmax_scale > 0.f) ||
+      !(softmax_scale < 3.0e38f) || (batch->dtype != CAB_BF16 && batch->dtype != CAB_F16))
+    return CAB_ERR_BAD_ARGUMENT;
+  if (batch->page_stride % 8 || batch->token_stride % 8 || batch->token_stride < kD || batch->page_stride < kD)
+    return CAB_ERR_BAD_ARGUMENT;
+  if ((long long)T * H > 0x7fffffffLL || batch->batch > kMaxBatch) return CAB_ERR_TOO_LARGE;
+  if ((long long)batch->max_pages * batch->page_size > 0x7fffff00LL) return CAB_ERR_TOO_LARGE;
+  if (!cab::aligned_to(out, 16) || !cab::aligned_to(q, 16) || !cab::aligned_to(batch->rows, 16) ||
+      !cab::aligned_to(workspace, 16))
+    return CAB_ERR_MISALIGNED;
+  if (workspace_bytes < mla_paged_attention_workspace_bytes(T, H)) return CAB_ERR_BAD_ARGUMENT;
+
+  Params p;
+  p.q = q; p.out = out; p.lse = lse;
+  p.page_table = batch->page_table; p.q_start = batch->q_start; p.kv_len = batch->kv_len;
+  p.T = T; p.H = H; p.batch = batch->batch; p.tail = tail;
+  p.max_pages = batch->max_pages; p.num_pages = batch->num_pages; p.page_size = batch->page_size;
+  int box = 1;                                 // rows that are sure to lie in one page: a box of the tensor map
+  while (box < kKeys && batch->page_size % (2 * box) == 0) box *= 2;
+  p.box = box;
+  p.causal = causal != 0;
+  p.window = window < (long long)batch->max_pages * batch->page_size ? window : 0;   // wider than any history: none
+  p.rows_cap = rows_cap_of(T, H);
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2)
+    return CAB_ERR_LAUNCH;
+  p.pairs = sms / 2 < kPairs ? sms / 2 : kPairs;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const size_t rows = (size_t)kPairs * 2 * p.rows_cap;
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + align256(rows * kDv * 4));
+  p.meta = reinterpret_cast<Meta*>(ws + align256(rows * kDv * 4) + align256(rows * 2 * 2 * 4));
+  p.status = status;
+
+  CUtensorMap map;
+  sm100::EncodeTiledFn encode = sm100::encode_tiled_fn();
+  if (!encode) return CAB_ERR_LAUNCH;
+  const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)batch->page_size, (cuuint64_t)batch->num_pages};
+  const cuuint64_t strides[2] = {(cuuint64_t)batch->token_stride * 2, (cuuint64_t)batch->page_stride * 2};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
+  if (encode(&map, batch->dtype == CAB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+             batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return CAB_ERR_BAD_ARGUMENT;
+  if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
+  return batch->dtype == CAB_F16 ? launch<__half>(p, map, stream) : launch<__nv_bfloat16>(p, map, stream);
+}

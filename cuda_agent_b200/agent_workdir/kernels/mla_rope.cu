@@ -1,0 +1,324 @@
+// Rotary positions on a part of a head, and the same fused with the write of a batch's new rows into the paged
+// latent cache.
+//   (x0, x1) -> mscale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a),  a = position * freq[i]
+// Memory bound: each column is read and written once. The angles depend on the token alone, so a CTA makes the
+// sines and cosines of its tokens once, in shared memory, and uses them for all the heads it handles. The angle
+// is formed and reduced to a fraction of a turn in 64 bits (at position 10^6 a 32-bit product is off by 0.03
+// radian); sine and cosine of the fraction are 32-bit, as is the rotation; one rounding at the end.
+// Columns move in 16-byte pieces where pointers, strides and R allow it, else pair by pair.
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "cab_common.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxR = 2048;
+constexpr int kAngles = 1024;                  // sine / cosine pairs of a CTA
+
+template <typename T> __device__ __forceinline__ float to_f(T v) { return static_cast<float>(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float2 turn_of(int position, double freq, float mscale, bool inverse) {
+  const double t = (double)position * (freq * 0.15915494309189533577);   // turns
+  float s, c;
+  sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+  return make_float2(c * mscale, (inverse ? -s : s) * mscale);
+}
+__device__ __forceinline__ void rotate(float& a, float& b, float2 cs) {
+  const float x = a * cs.x - b * cs.y, y = b * cs.x + a * cs.y;
+  a = x;
+  b = y;
+}
+
+// N elements that are one memory access.
+template <typename T, int N>
+struct __align__(sizeof(T) * N) Vec { T v[N]; };
+
+// One unit of a head: with `interleaved` N consecutive columns (N / 2 pairs), else N columns of either half.
+template <typename T, int N, bool kInterleaved>
+struct Unit {
+  static constexpr int kVecs = kInterleaved ? 1 : 2;
+  Vec<T, N> d[kVecs];
+  __device__ __forceinline__ void load(const T* x, int unit, int half) {
+    d[0] = *reinterpret_cast<const Vec<T, N>*>(x + unit * N);
+    if constexpr (!kInterleaved) d[1] = *reinterpret_cast<const Vec<T, N>*>(x + half + unit * N);
+  }
+  __device__ __forceinline__ void turn(const float2* cs, int unit) {
+    if constexpr (kInterleaved) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        float a = to_f(d[0].v[2 * i]), b = to_f(d[0].v[2 * i + 1]);
+        rotate(a, b, cs[unit * (N / 2) + i]);
+        d[0].v[2 * i] = from_f<T>(a);
+        d[0].v[2 * i + 1] = from_f<T>(b);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float a = to_f(d[0].v[i]), b = to_f(d[kVecs - 1].v[i]);
+        rotate(a, b, cs[unit * N + i]);
+        d[0].v[i] = from_f<T>(a);
+        d[kVecs - 1].v[i] = from_f<T>(b);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* x, int unit, int half) const {
+    *reinterpret_cast<Vec<T, N>*>(x + unit * N) = d[0];
+    if constexpr (!kInterleaved) *reinterpret_cast<Vec<T, N>*>(x + half + unit * N) = d[1];
+  }
+};
+
+struct RopeParams {
+  void* out;
+  const void* x;
+  const int* positions;
+  const double* freq;
+  int T, H, R, tokens;                         // tokens per CTA
+  int heads;                                   // heads per CTA
+  long long xt, xh, ot, oh;
+  float mscale;
+  int inverse;
+};
+
+// The units of `tokens` tokens x heads [h0, h1), four in flight per thread.
+template <typename T, int N, bool kInterleaved>
+__device__ __forceinline__ void rotate_heads(T* out, const T* x, const float2* cs, int tokens, int h0, int h1, int R,
+                                             long long xt, long long xh, long long ot, long long oh) {
+  const int half = R / 2, units = (kInterleaved ? R : half) / N, heads = h1 - h0;
+  const int total = tokens * heads * units;
+  for (int e0 = threadIdx.x; e0 < total; e0 += 4 * kThreads) {
+    Unit<T, N, kInterleaved> u[4];
+    int tok[4], head[4], unit[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = e0 + k * kThreads;
+      if (e >= total) break;
+      unit[k] = e % units;
+      const int th = e / units;
+      tok[k] = th / heads;
+      head[k] = h0 + th % heads;
+      u[k].load(x + tok[k] * xt + head[k] * xh, unit[k], half);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (e0 + k * kThreads >= total) break;
+      u[k].turn(cs + tok[k] * half, unit[k]);
+      u[k].store(out + tok[k] * ot + head[k] * oh, unit[k], half);
+    }
+  }
+}
+
+template <typename T, int N, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads) mla_rope_kernel(const RopeParams p) {
+  __shared__ float2 cs[kAngles];
+  const int t0 = blockIdx.x * p.tokens, tokens = min(p.tokens, p.T - t0), half = p.R / 2;
+  for (int e = threadIdx.x; e < tokens * half; e += kThreads)
+    cs[e] = turn_of(__ldg(p.positions + t0 + e / half), __ldg(p.freq + e % half), p.mscale, p.inverse != 0);
+  __syncthreads();
+  const int h0 = blockIdx.y * p.heads, h1 = min(p.H, h0 + p.heads);
+  rotate_heads<T, N, kInterleaved>(static_cast<T*>(p.out) + t0 * p.ot, static_cast<const T*>(p.x) + t0 * p.xt, cs, tokens,
+                                   h0, h1, p.R, p.xt, p.xh, p.ot, p.oh);
+}
+
+constexpr int kLatent = 512, kRot = 64;
+
+struct AppendParams {
+  RopeParams r;                                // q: R = 64
+  const void *c_kv, *k_pe;
+  long long ct, kt;                            // token strides
+  void* rows;
+  long long page_stride, token_stride;
+  int num_pages, page_size, batch, max_pages;
+  const int *page_table, *q_start, *kv_len;
+  int* status;
+};
+
+// kVec: every row and stride allows 16-byte accesses. Head group 0 of a token also writes the token's cache row.
+template <typename T, bool kInterleaved, bool kVec>
+__global__ void __launch_bounds__(kThreads) mla_rope_append_kernel(const AppendParams p) {
+  constexpr int N = kVec ? 8 : (kInterleaved ? 2 : 1);
+  constexpr int half = kRot / 2;
+  __shared__ float2 cs[kAngles];
+  __shared__ int s_pos[kAngles / half];
+  __shared__ long long s_row[kAngles / half];  // where the cache row begins, -1: nowhere
+  const int t0 = blockIdx.x * p.r.tokens;
+  const int end = min(max(__ldg(p.q_start + p.batch), 0), p.r.T);     // tokens behind the last sequence stay as they are
+  const int tokens = min(p.r.tokens, end - t0);
+  if (tokens <= 0) return;
+  if (threadIdx.x < tokens) {
+    const int t = t0 + threadIdx.x;
+    int lo = 0, hi = p.batch;                  // last b with q_start[b] <= t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(p.q_start + mid) <= t) lo = mid; else hi = mid;
+    }
+    const int pos = __ldg(p.kv_len + lo) - __ldg(p.q_start + lo + 1) + t;
+    const int at = pos / p.page_size;
+    const int page = pos >= 0 && at < p.max_pages ? __ldg(p.page_table + (long long)lo * p.max_pages + at) : -1;
+    const bool ok = (unsigned)page < (unsigned)p.num_pages;
+    s_pos[threadIdx.x] = pos;
+    s_row[threadIdx.x] = ok ? page * p.page_stride + (pos - at * p.page_size) * p.token_stride : -1;
+    if (!ok && blockIdx.y == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < tokens * half; e += kThreads)
+    cs[e] = turn_of(s_pos[e / half], __ldg(p.r.freq + e % half), p.r.mscale, false);
+  if (blockIdx.y == 0) {                       // the latent part of the rows: a copy
+    constexpr int C = kVec ? 8 : 1;
+    T* rows = static_cast<T*>(p.rows);
+    const T* c = static_cast<const T*>(p.c_kv) + t0 * p.ct;
+    for (int e = threadIdx.x; e < tokens * (kLatent / C); e += kThreads) {
+      const int t = e / (kLatent / C), col = e % (kLatent / C) * C;
+      if (s_row[t] >= 0)
+        *reinterpret_cast<Vec<T, C>*>(rows + s_row[t] + col) = *reinterpret_cast<const Vec<T, C>*>(c + t * p.ct + col);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.y == 0) {
+    constexpr int units = (kInterleaved ? kRot : half) / N;
+    const T* k = static_cast<const T*>(p.k_pe) + t0 * p.kt;
+    for (int e = threadIdx.x; e < tokens * units; e += kThreads) {
+      const int t = e / units, unit = e % units;
+      if (s_row[t] < 0) continue;
+      Unit<T, N, kInterleaved> u;
+      u.load(k + t * p.kt, unit, half);
+      u.turn(cs + t * half, unit);
+      u.store(static_cast<T*>(p.rows) + s_row[t] + kLatent, unit, half);
+    }
+  }
+  const int h0 = blockIdx.y * p.r.heads, h1 = min(p.r.H, h0 + p.r.heads);
+  if (h0 < h1)
+    rotate_heads<T, N, kInterleaved>(static_cast<T*>(p.r.out) + t0 * p.r.ot, static_cast<const T*>(p.r.x) + t0 * p.r.xt, cs,
+                                     tokens, h0, h1, kRot, p.r.xt, p.r.xh, p.r.ot, p.r.oh);
+}
+
+// Tokens and heads per CTA: about 2048 units (8 a thread), fewer where the call is too small to fill the device.
+void split(RopeParams& p, int units_per_head, dim3& grid) {
+  const int half = p.R / 2;
+  const long long per_token = (long long)(p.H > 0 ? p.H : 1) * units_per_head;
+  long long tokens = 2048 / per_token;
+  const long long most = kAngles / half < 1 ? 1 : kAngles / half;
+  if (tokens > most) tokens = most;
+  const long long fill = ((long long)p.T + 4 * cab::kNumSMs - 1) / (4 * cab::kNumSMs);
+  if (tokens > fill) tokens = fill;
+  if (tokens < 1) tokens = 1;
+  p.tokens = (int)tokens;
+  // a token alone is split over its heads when it is large, or when there are few tokens
+  long long heads = p.H > 0 ? p.H : 1;
+  if (tokens == 1) {
+    const long long groups_wanted = p.T < 2 * cab::kNumSMs ? (2 * cab::kNumSMs + p.T - 1) / p.T : 1;
+    long long smallest = 256 / units_per_head;                        // a thread has something to do
+    if (smallest < 1) smallest = 1;
+    heads = (heads + groups_wanted - 1) / groups_wanted;
+    if (heads < smallest) heads = smallest;
+    long long largest = 4096 / units_per_head;
+    if (largest < 1) largest = 1;
+    if (heads > largest) heads = largest;
+  }
+  p.heads = (int)heads;
+  grid = dim3((unsigned)((p.T + tokens - 1) / tokens), (unsigned)(((p.H > 0 ? p.H : 1) + heads - 1) / heads));
+}
+
+template <typename T, int N, bool kInterleaved>
+int launch_rope(RopeParams& p, cudaStream_t stream) {
+  dim3 grid;
+  split(p, (kInterleaved ? p.R : p.R / 2) / N, grid);
+  if (grid.y > 65535) return CAB_ERR_TOO_LARGE;
+  mla_rope_kernel<T, N, kInterleaved><<<grid, kThreads, 0, stream>>>(p);
+  return cab::launch_status();
+}
+
+template <typename T>
+int run_rope(RopeParams& p, bool interleaved, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = cab::aligned_to(p.x, 16) && cab::aligned_to(p.out, 16) && p.xt % V == 0 && p.xh % V == 0 &&
+                   p.ot % V == 0 && p.oh % V == 0 && (interleaved ? p.R : p.R / 2) % V == 0;
+  if (interleaved) return vec ? launch_rope<T, V, true>(p, stream) : launch_rope<T, 2, true>(p, stream);
+  return vec ? launch_rope<T, V, false>(p, stream) : launch_rope<T, 1, false>(p, stream);
+}
+
+template <typename T>
+int run_append(AppendParams& p, bool interleaved, cudaStream_t stream) {
+  auto vec16 = [](const void* q, long long a, long long b) { return cab::aligned_to(q, 16) && a % 8 == 0 && b % 8 == 0; };
+  const bool vec = vec16(p.c_kv, p.ct, 0) && vec16(p.k_pe, p.kt, 0) &&
+                   (p.r.H == 0 || (vec16(p.r.x, p.r.xt, p.r.xh) && vec16(p.r.out, p.r.ot, p.r.oh)));
+  const int n = vec ? 8 : (interleaved ? 2 : 1);
+  dim3 grid;
+  split(p.r, (interleaved ? kRot : kRot / 2) / n, grid);
+  if (grid.y > 65535) return CAB_ERR_TOO_LARGE;
+  if (interleaved) {
+    if (vec) mla_rope_append_kernel<T, true, true><<<grid, kThreads, 0, stream>>>(p);
+    else mla_rope_append_kernel<T, true, false><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    if (vec) mla_rope_append_kernel<T, false, true><<<grid, kThreads, 0, stream>>>(p);
+    else mla_rope_append_kernel<T, false, false><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return cab::launch_status();
+}
+
+}  // namespace
+
+extern "C" int mla_rope_launcher(void* out, const void* x, const int* positions, const double* freq, int T, int H, int R,
+                                 long long x_stride_t, long long x_stride_h, long long out_stride_t,
+                                 long long out_stride_h, int dtype, int interleaved, int inverse, float mscale, int config,
+                                 cudaStream_t stream) {
+  (void)config;
+  if (T < 0 || H < 0 || R <= 0 || R % 2) return CAB_ERR_BAD_ARGUMENT;
+  if (T == 0 || H == 0) return CAB_OK;
+  if (!out || !x || !positions || !freq) return CAB_ERR_BAD_ARGUMENT;
+  if (R > kMaxR) return CAB_ERR_TOO_LARGE;
+  const size_t element = dtype == CAB_F32 ? 4 : 2;
+  // the pair by pair form takes the two columns of an interleaved pair as one access
+  const size_t unit = interleaved ? 2 * element : element;
+  if (!cab::aligned_to(x, unit) || !cab::aligned_to(out, unit) ||
+      (interleaved && (x_stride_t % 2 || x_stride_h % 2 || out_stride_t % 2 || out_stride_h % 2)))
+    return CAB_ERR_MISALIGNED;
+  RopeParams p{out, x, positions, freq, T, H, R, 0, 0, x_stride_t, x_stride_h, out_stride_t, out_stride_h, mscale, inverse};
+  switch (dtype) {
+    case CAB_BF16: return run_rope<__nv_bfloat16>(p, interleaved != 0, stream);
+    case CAB_F16: return run_rope<__half>(p, interleaved != 0, stream);
+    case CAB_F32: return run_rope<float>(p, interleaved != 0, stream);
+    default: return CAB_ERR_BAD_ARGUMENT;
+  }
+}
+
+extern "C" int mla_rope_append_launcher(void* q_out, const void* q_pe, const void* c_kv, const void* k_pe,
+                                        const cab_mla_paged_batch* batch, const double* freq, int T, int H,
+                                        long long q_out_stride_t, long long q_out_stride_h, long long q_stride_t,
+                                        long long q_stride_h, long long c_stride_t, long long k_stride_t, int interleaved,
+                                        float mscale, int* status, int config, cudaStream_t stream) {
+  (void)config;
+  if (T < 0 || H < 0 || !batch || batch->batch < 0) return CAB_ERR_BAD_ARGUMENT;
+  if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
+  if (T == 0 || batch->batch == 0) return CAB_OK;
+  if (!c_kv || !k_pe || !freq || !batch->rows || !batch->page_table || !batch->q_start || !batch->kv_len ||
+      (H > 0 && (!q_out || !q_pe)))
+    return CAB_ERR_BAD_ARGUMENT;
+  if (batch->num_pages <= 0 || batch->page_size <= 0 || batch->max_pages <= 0 || batch->page_stride % 8 ||
+      batch->token_stride % 8 || batch->token_stride < kLatent + kRot)
+    return CAB_ERR_BAD_ARGUMENT;
+  if (!cab::aligned_to(batch->rows, 16)) return CAB_ERR_MISALIGNED;
+  if (interleaved && (!cab::aligned_to(k_pe, 4) || k_stride_t % 2 ||
+                      (H > 0 && (!cab::aligned_to(q_pe, 4) || !cab::aligned_to(q_out, 4) || q_stride_t % 2 ||
+                                 q_stride_h % 2 || q_out_stride_t % 2 || q_out_stride_h % 2))))
+    return CAB_ERR_MISALIGNED;
+  AppendParams p;
+  p.r = RopeParams{q_out, q_pe, nullptr, freq, T, H, kRot, 0, 0, q_stride_t, q_stride_h, q_out_stride_t, q_out_stride_h,
+                   mscale, 0};
+  p.c_kv = c_kv; p.k_pe = k_pe; p.ct = c_stride_t; p.kt = k_stride_t;
+  p.rows = batch->rows; p.page_stride = batch->page_stride; p.token_stride = batch->token_stride;
+  p.num_pages = batch->num_pages; p.page_size = batch->page_size; p.batch = batch->batch; p.max_pages = batch->max_pages;
+  p.page_table = batch->page_table; p.q_start = batch->q_start; p.kv_len = batch->kv_len;
+  p.status = status;
+  switch (batch->dtype) {
+    case CAB_BF16: return run_append<__nv_bfloat16>(p, interleaved != 0, stream);
+    case CAB_F16: return run_append<__half>(p, interleaved != 0, stream);
+    default: return CAB_ERR_BAD_ARGUMENT;
+  }
+}

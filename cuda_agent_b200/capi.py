@@ -8,7 +8,7 @@ reach the kernels without going through pybind.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libcuda_agent_b200.so"
@@ -37,6 +37,22 @@ SIGNATURES = {
     "mla_sparse_decode_multi_launcher": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_float, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     "mla_sparse_decode_noalloc_launcher": (c_int, [c_void_p] * 5 + [c_int] * 4 + [c_float, c_int, c_void_p, c_int, c_void_p]),
     "mla_gather_rows_launcher": (c_int, [c_void_p] * 4 + [c_int] * 4 + [c_void_p]),
+    "mla_rope_launcher": (c_int, [c_void_p] * 4 + [c_int] * 3 + [c_longlong] * 4 + [c_int] * 3 + [c_float, c_int, c_void_p]),
+    "mla_rope_append_launcher": (c_int, [c_void_p] * 6 + [c_int] * 2 + [c_longlong] * 6
+                                 + [c_int, c_float, c_void_p, c_int, c_void_p]),
+    "mla_paged_attention_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "mla_paged_attention_launcher": (c_int, [c_void_p] * 4 + [c_int] * 2 + [c_float, c_int, c_int, c_void_p, c_size_t, c_void_p,
+                                                                           c_int, c_void_p]),
+    "mla_pages_scratch_bytes": (c_size_t, [c_int, c_int]),
+    "mla_pages_copy_launcher": (c_int, [c_void_p, c_longlong, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_void_p,
+                                        c_void_p, c_int, c_void_p]),
+    "mla_pages_extend_launcher": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p] * 2 + [c_int] + [c_void_p] * 2
+                                  + [c_int, c_void_p]),
+    "mla_pages_fork_launcher": (c_int, [c_void_p, c_longlong, c_int, c_longlong] + [c_void_p] * 3 + [c_int] * 4
+                                + [c_void_p] * 2 + [c_int] + [c_void_p] * 2 + [c_int, c_void_p]),
+    "mla_pages_free_launcher": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    "mla_pages_compact_launcher": (c_int, [c_void_p, c_longlong, c_int, c_longlong] + [c_void_p] * 3 + [c_int] * 4
+                                   + [c_void_p] * 2 + [c_int, c_void_p]),
     "moe_grouped_gemm_fp8_launcher": (c_int, [c_int] + [c_void_p] * 8 + [c_int] * 6 + [c_void_p, c_int, c_void_p]),
     "moe_ep_peer_buffer_bytes": (c_size_t, [c_int] * 4),
     "moe_ep_peer_create": (c_int, [c_void_p] + [c_int] * 6),
@@ -62,6 +78,13 @@ class MoeEpLayerArgs(ctypes.Structure):
                                         "shared_w13_s", "shared_w2_q", "shared_w2_s")] + \
                [("E", c_int), ("I", c_int), ("routing", c_int), ("n_group", c_int), ("topk_group", c_int),
                 ("scaling", c_float), ("entry_cap", c_int), ("gemm_ctas", c_int)]
+
+
+class MlaPagedBatch(ctypes.Structure):
+    """`cab_mla_paged_batch` of the header, field for field."""
+    _fields_ = [("rows", c_void_p), ("page_stride", c_longlong), ("token_stride", c_longlong), ("num_pages", c_int),
+                ("page_size", c_int), ("page_table", c_void_p), ("q_start", c_void_p), ("kv_len", c_void_p),
+                ("batch", c_int), ("max_pages", c_int), ("dtype", c_int)]
 
 
 class CabError(RuntimeError):
@@ -263,6 +286,55 @@ def mla_sparse_decode_noalloc(out, q, kv, seq_len, idx, softmax_scale: float, ns
     _check("mla_sparse_decode_noalloc_launcher",
            lib().mla_sparse_decode_noalloc_launcher(_p(out), _p(q), _p(kv), _p(seq_len), _p(idx), B, Hh, S, topk,
                                                     softmax_scale, nsplit, _opt(status), config, _stream()))
+
+
+# ----------------------------------------------------------------------------- paged latent cache
+def _dtype_code(t) -> int:
+    import torch
+    return {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[t.dtype]
+
+
+def mla_paged_batch(cache, page_table, q_start, kv_len) -> MlaPagedBatch:
+    """cache [pages, page_size, 576] (rows and pages may be strided), page_table [batch, max_pages], q_start [batch + 1],
+    kv_len [batch]; the tensors have to outlive the calls that take the result."""
+    if not cache.is_cuda:
+        raise ValueError("the C ABI takes device pointers; got a CPU tensor")
+    return MlaPagedBatch(cache.data_ptr(), cache.stride(0), cache.stride(1), cache.shape[0], cache.shape[1], _p(page_table),
+                         _p(q_start), _p(kv_len), page_table.shape[0], page_table.shape[1], _dtype_code(cache))
+
+
+def mla_rope(out, x, positions, freq, interleaved: bool = False, mscale: float = 1.0, inverse: bool = False,
+             config: int = 0) -> None:
+    """Rotary positions on x [T, H, R] (any strides but the last); out may be x."""
+    T, H, R = x.shape
+    _check("mla_rope_launcher",
+           lib().mla_rope_launcher(out.data_ptr(), x.data_ptr(), _p(positions), _p(freq), T, H, R, x.stride(0), x.stride(1),
+                                   out.stride(0), out.stride(1), _dtype_code(x), int(interleaved), int(inverse), mscale,
+                                   config, _stream()))
+
+
+def mla_rope_append(q_out, q_pe, c_kv, k_pe, batch: MlaPagedBatch, freq, interleaved: bool = False, mscale: float = 1.0,
+                    status=None, config: int = 0) -> None:
+    T, H, _ = q_pe.shape
+    _check("mla_rope_append_launcher",
+           lib().mla_rope_append_launcher(q_out.data_ptr(), q_pe.data_ptr(), c_kv.data_ptr(), k_pe.data_ptr(),
+                                          ctypes.byref(batch), _p(freq), T, H, q_out.stride(0), q_out.stride(1),
+                                          q_pe.stride(0), q_pe.stride(1), c_kv.stride(0), k_pe.stride(0), int(interleaved),
+                                          mscale, _opt(status), config, _stream()))
+
+
+def mla_paged_workspace_bytes(T: int, H: int) -> int:
+    return lib().mla_paged_attention_workspace_bytes(T, H)
+
+
+def mla_paged_attention(out, lse, q, batch: MlaPagedBatch, softmax_scale: float, causal: bool = True, window: int = 0,
+                        workspace=None, status=None, config: int = 0) -> None:
+    T, H, _ = q.shape
+    _check("mla_paged_attention_launcher",
+           lib().mla_paged_attention_launcher(_p(out), _opt(lse), _p(q), ctypes.byref(batch), T, H, softmax_scale,
+                                              int(causal), window, _opt(workspace),
+                                              0 if workspace is None else workspace.numel(), _opt(status), config,
+                                              _stream()))
 
 
 # ----------------------------------------------------------------------------- expert-parallel row movement
