@@ -12,10 +12,14 @@
 // and two rings for blocks of 64 cache rows: 64-column tiles that only Q.K^T reads (six of 8 KB), and this
 // CTA's 256 value columns, which P.V reads as well (three blocks of 32 KB). A tile slot is released as soon as
 // its last reader is done, so every load has about a block's time to land.
-//   warps 0-3  one (token, head) row per thread: Q, softmax, result. The reference maximum of a row moves only
+//   warps 0-3  one (token, head) row per thread: softmax, result. The reference maximum of a row moves only
 //              when it would grow by more than 2^8, so O is hardly ever rescaled
 //   warp 4     issues Q.K^T of block j+1 before P.V of block j: the tensor core works while the softmax does
-//   warp 5     TMA: one box per run of rows that lie in one page
+//   warps 5, 7 TMA, each for one of the rings: one box per run of rows that lie in one page. Q comes the same way,
+//              its tensor-memory half through two slots of the value ring
+//   warp 6     clears the rows behind a sequence's end in its last block of V
+// Whoever issues tensor or TMA instructions does so in one elected thread, waits included: the operands then sit
+// in uniform registers, and a wait polled by 32 lanes costs some 300 clk more than one polled by a single lane.
 // The work of a call (tiles x blocks of 64 rows) is cut into equal runs, one for each pair of CTAs, wherever
 // that cuts a tile; each CTA finds its run itself from q_start and kv_len. Tiles cut by a boundary leave
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
@@ -36,17 +40,19 @@ constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 12
 constexpr int kNTiles = 5, kVTiles = 4;        // tiles of a block: the other value half and the rotary columns / own half
 constexpr int kNSlots = 6, kVSlots = 3;
 constexpr int kQChunk = kRows * 128;
-constexpr int kThreads = 6 * 32;
+constexpr int kThreads = 8 * 32;
+constexpr int kQBox = 16;                      // rows of the small box for Q
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384, kTmemCols = 512;
 constexpr float kRescale = 8.f;
 constexpr int kMaxBatch = 16384;
 enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitDrain };
 
 struct __align__(16) Control {
-  uint64_t n_full[kNSlots], n_empty[kNSlots], v_full[kVSlots], v_empty[kVSlots], s_full[2], p_full[2], pv_done[2], q_ready;
+  uint64_t n_full[kNSlots], n_empty[kNSlots], v_full[kVSlots], v_empty[kVSlots], v_land[kVSlots], s_full[2], p_full[2], pv_done[2], q_ready, q_full, q_free;
   long long scan[kThreads / 32], total;
   long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
   int seq, tile;                               // its first tile
+  int pages[2][2][kKeys];                      // [ring][block parity]: the pages of a block's boxes
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -54,9 +60,9 @@ constexpr int kRingBytes = kNSlots * kTile + kVSlots * kVTiles * kTile;
 constexpr int kSmemBytes = kNTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
 static_assert(kSmemBytes <= 232448 && (kMaxBatch + 2) * 4 <= kRingBytes, "shared memory");
 
-// What the merge kernel has to know of the tile that a pair ends: its first (token, head) row, its rows, the pair
-// that holds its first part, and the work of the whole call (which says what runs are empty).
-struct Meta { long long row0, total; int rows, first; };
+// What the merge kernel has to know of the tile that a pair ends: its first (token, head) row, its rows, and the pair
+// that holds its first part.
+struct Meta { int row0, rows, first; };
 
 struct Params {
   const void* q;
@@ -73,8 +79,17 @@ struct Params {
   int* status;
 };
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+// Issued where it stands, so that the load is under way while other work is done.
+__device__ __forceinline__ int load_now(const int* p) {
+  int v;
+  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
   asm volatile(
@@ -112,6 +127,16 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same_v<T, __half>) {
@@ -136,17 +161,17 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   return s;
 }
 __device__ __forceinline__ int tiles_of(const Params& p, int n) {
-  return (int)(((long long)n * p.H + kRows - 1) / kRows);
+  return (int)(((unsigned)n * (unsigned)p.H + kRows - 1) / kRows);    // T * H < 2^31
 }
 // Blocks [first, first + count) of 64 cache rows that some row of tile i sees; `units` = max(count, 1) is what
 // the tile counts as when the work is divided, so that a tile that sees nothing is still written.
-struct Item { long long row0; int rows, first, count, units; };
+struct Item { int row0, rows, first, count, units; };
 __device__ __forceinline__ Item item_of(const Params& p, const Seq& s, int i) {
   Item t;
-  const long long r0 = (long long)i * kRows, r1 = min(r0 + kRows, (long long)s.n * p.H);
-  t.row0 = (long long)s.tok * p.H + r0;
-  t.rows = (int)(r1 - r0);
-  const int t0 = (int)(r0 / p.H), t1 = (int)((r1 - 1) / p.H);
+  const int r0 = i * kRows, left = s.n * p.H - r0;
+  t.row0 = s.tok * p.H + r0;
+  t.rows = min(kRows, left);
+  const int t0 = (unsigned)r0 / (unsigned)p.H, t1 = (unsigned)(r0 + t.rows - 1) / (unsigned)p.H;
   const int hi = p.causal ? min(s.len, s.pos + t1 + 1) : s.len;
   const int lo = p.window > 0 ? (int)max(0LL, (long long)s.pos + t0 + 1 - p.window) : 0;
   t.first = lo / kKeys;
@@ -192,8 +217,12 @@ struct Walk {
 };
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int where) {
-  const bool ok = sm100::mbar_wait(bar, parity, abort_flag, status, where);
-  return __all_sync(0xffffffffu, ok);
+  // one lane polls: a try_wait by 32 lanes costs some 300 clk more, which is the time of seven tensor instructions
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = sm100::mbar_wait(bar, parity, abort_flag, status, where);
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
 }
 
 // Exclusive scan over the CTA's threads; the sum of all goes to ctl.total.
@@ -257,7 +286,9 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
     }
   }
   long long at = block_scan(ctl, sum);
-  const long long W = ctl.total, x0 = W * pair / p.pairs, x1 = W * (pair + 1) / p.pairs;
+  const long long W = ctl.total;
+  const int pairs = (int)min((long long)p.pairs, W);           // no run is empty but those of the pairs behind
+  const long long x0 = pair < pairs ? W * pair / pairs : W, x1 = pair < pairs ? W * (pair + 1) / pairs : W;
   if (x0 < x1 && at <= x0 && x0 < at + sum) {
     Seq s = seq_of(p, b);
     for (int i = i0; i < i1; ++i) {
@@ -266,12 +297,10 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
       if (x0 < at + t.units) {
         ctl.x0 = x0; ctl.x1 = x1; ctl.item_x = at; ctl.seq = b; ctl.tile = i - pre[b];
         // the pair that ends a cut tile says so to the merge kernel
-        Meta m{t.row0, W, 0, 0};
+        Meta m{t.row0, 0, 0};
         if (x0 > at && at + t.units <= x1) {
           m.rows = t.rows;
-          int f = pair - 1;
-          while (f > 0 && W * f / p.pairs > at) --f;
-          m.first = f;
+          m.first = (int)(((at + 1) * pairs - 1) / W);         // the last pair that begins at or before `at`
         }
         if ((blockIdx.x & 1) == 0) p.meta[pair] = m;
         break;
@@ -279,25 +308,27 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
       at += t.units;
     }
   }
-  if (x0 >= x1 && tid == 0 && (blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0, 0};
+  if (x0 >= x1 && tid == 0 && (blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0};
   __syncthreads();
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
-mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap map) {
+mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap map,
+                           const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q16) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = base;
   uint8_t* n_ring = base + kNTiles * kQChunk;
   uint8_t* v_ring = n_ring + kNSlots * kTile;
   Control& ctl = *reinterpret_cast<Control*>(v_ring + kVSlots * kVTiles * kTile);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be: the tensor instructions take their operands from uniform registers
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNSlots; ++s) { sm100::mbar_init(&ctl.n_full[s], 1); sm100::mbar_init(&ctl.n_empty[s], 1); }
-    for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_full[s], 1); sm100::mbar_init(&ctl.v_empty[s], 1); }
+    for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_full[s], 1); sm100::mbar_init(&ctl.v_empty[s], 1); sm100::mbar_init(&ctl.v_land[s], 1); }
     // by block parity. pv_done too: a softmax thread may wait for P.V of block j while that of j - 1 is not done
     for (int s = 0; s < 2; ++s) {
       sm100::mbar_init(&ctl.s_full[s], 1);
@@ -305,6 +336,8 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
       sm100::mbar_init(&ctl.pv_done[s], 1);
     }
     sm100::mbar_init(&ctl.q_ready, 4);
+    sm100::mbar_init(&ctl.q_full, 1);
+    sm100::mbar_init(&ctl.q_free, 1);
     ctl.abort_flag = 0;
     sm100::mbar_fence_init();
   }
@@ -312,200 +345,262 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
     sm100::tmem_alloc(&ctl.tmem_base, kTmemCols);
     sm100::tmem_relinquish();
   }
-  if (warp == 5 && lane == 0) sm100::prefetch_tensormap(&map);
+  if (warp == 5 && lane == 0) {
+    sm100::prefetch_tensormap(&map);
+    sm100::prefetch_tensormap(&map_q);
+  }
   find_run(p, ctl, reinterpret_cast<int*>(n_ring), pair);
   sm100::fence_proxy_async();                  // the rings were used as scratch
   sm100::tc_fence_before_sync();
   __syncthreads();
   sm100::tc_fence_after_sync();
-  const uint32_t tmem = ctl.tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);
   volatile int* abort_flag = &ctl.abort_flag;
   constexpr uint32_t kFmt = std::is_same_v<T, __half> ? 0 : 1;
 
-  if (warp == 5) {
+  if (warp == 5 || warp == 7) {
     // ---------------------------------------------------------------- loads
-    uint32_t n_at = 0, v_at = 0;               // tiles / blocks loaded so far
-    bool ok = true;
+    const int ring = warp == 7;                // 0: the tiles that only Q.K^T reads, 1: V
     const int other = half ? 0 : 4;            // first of the four column tiles of the other value half
-    for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
-      const int* table = p.page_table + (size_t)w.b * p.max_pages;
-      const int nb = w.blocks();
-      // page and row in the page of this lane's boxes (two when a box is a single row), one block ahead
-      int page[2], row[2];
-      auto look = [&](int j) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const long long key = (long long)j * kKeys + (lane + 32 * k) * p.box;
-          page[k] = p.num_pages;               // outside the pool: TMA fills with zeros
-          row[k] = 0;
-          if ((lane + 32 * k) * p.box < kKeys && key < w.s.len) {
-            const int at = (int)(key / p.page_size);
-            row[k] = (int)(key - (long long)at * p.page_size);
-            page[k] = __ldg(table + at);
-          }
-        }
-      };
-      if (nb > 0) look(w.begin());
-      for (int k = 0; k < nb && ok; ++k) {
-        const int j = w.begin() + k;
-        const int boxes = (min(kKeys, w.s.len - j * kKeys) + p.box - 1) / p.box;
-        int pg[2], rw[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          pg[e] = page[e];
-          rw[e] = row[e];
-          if (lane + 32 * e < boxes && ((unsigned)pg[e] >= (unsigned)p.num_pages)) {
-            if (p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
-            pg[e] = p.num_pages;
-            rw[e] = 0;
-          }
-        }
-        if (k + 1 < nb) look(j + 1);
-        auto issue = [&](uint8_t* dst, uint64_t* bar, int col) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (lane + 32 * e < boxes)
-              tma_load_3d(sm100::smem_u32(dst) + (lane + 32 * e) * p.box * 128, &map, bar, col, rw[e], pg[e]);
-        };
-        for (int c = 0; c < kNTiles; ++c, ++n_at) {
-          const uint32_t s = n_at % kNSlots, use = n_at / kNSlots;
-          if (use > 0 && !warp_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree)) { ok = false; break; }
-          if (lane == 0) sm100::mbar_arrive_expect_tx(&ctl.n_full[s], boxes * p.box * 128);
-          __syncwarp();
-          issue(n_ring + s * kTile, &ctl.n_full[s], 64 * (c < 4 ? other + c : 8));
-        }
-        if (!ok) break;
-        const uint32_t s = v_at % kVSlots, use = v_at / kVSlots;
-        if (use > 0 && !warp_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree)) { ok = false; break; }
-        if (lane == 0) sm100::mbar_arrive_expect_tx(&ctl.v_full[s], kVTiles * boxes * p.box * 128);
-        __syncwarp();
-        for (int c = 0; c < kVTiles; ++c) issue(v_ring + (s * kVTiles + c) * kTile, &ctl.v_full[s], 64 * (4 - other + c));
-        ++v_at;
-      }
-    }
-    if (!ok) {                                 // giving up: copies in flight land before the CTA may end
-      int never = 0;
-      for (uint32_t i = n_at > kNSlots ? n_at - kNSlots : 0; i < n_at; ++i)
-        sm100::mbar_wait_limited(&ctl.n_full[i % kNSlots], (i / kNSlots) & 1, &never, nullptr, kWaitDrain, 200000000LL);
-      for (uint32_t i = v_at > kVSlots ? v_at - kVSlots : 0; i < v_at; ++i)
-        sm100::mbar_wait_limited(&ctl.v_full[i % kVSlots], (i / kVSlots) & 1, &never, nullptr, kWaitDrain, 200000000LL);
-    }
-  } else if (warp == 4) {
-    // ---------------------------------------------------------------- tensor core
-    constexpr uint32_t idesc_qk = sm100::umma_idesc(kFmt, kRows, kKeys);
-    constexpr uint32_t idesc_pv = sm100::umma_idesc(kFmt, kRows, kHalf) | (1u << 16);   // V: keys down, columns along
-    const uint32_t q_addr = sm100::smem_u32(q_smem), n_addr = sm100::smem_u32(n_ring), v_addr = sm100::smem_u32(v_ring);
-    uint32_t n_at = 0, g_qk = 0, g_pv = 0, seg = 0;
+    uint32_t at = 0, g = 0, seg = 0;           // slots filled, blocks, segments so far
+    uint32_t landed[kVSlots] = {};
     bool ok = true;
+    // pages of this lane's boxes (two when a box is a single row) in block j
+    int page[2];
+    auto look = [&](const Walk& w, int j) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int key = j * kKeys + (lane + 32 * k) * p.box;       // lengths end below 2^31 - 256
+        const bool in = (lane + 32 * k) * p.box < kKeys && key < w.s.len;
+        page[k] = in ? load_now(p.page_table + (size_t)w.b * p.max_pages + (unsigned)key / (unsigned)p.page_size) : 0;
+      }
+    };
+    auto keep = [&](int parity) {              // one outside the pool: TMA fills with zeros
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const bool bad = (unsigned)page[k] >= (unsigned)p.num_pages;
+        if (bad && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
+        ctl.pages[ring][parity][lane + 32 * k] = bad ? p.num_pages : page[k];
+      }
+      __syncwarp();
+    };
     for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
       const int nb = w.blocks();
       if (nb == 0) continue;
-      if (!warp_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ)) { ok = false; break; }
+      look(w, w.begin());
+      if (elect_one()) {                       // Q of this tile
+        const int boxes = w.t.rows > 4 * kQBox ? 1 : (w.t.rows + kQBox - 1) / kQBox, rows = w.t.rows > 4 * kQBox ? kRows : kQBox;
+        const CUtensorMap* m = w.t.rows > 4 * kQBox ? &map_q : &map_q16;
+        auto chunk = [&](uint8_t* dst, uint64_t* bar, int col) {
+          for (int e = 0; e < boxes; ++e)
+            tma_load_2d(sm100::smem_u32(dst) + e * rows * 128, m, bar, col, w.t.row0 + e * rows);
+        };
+        if (ring == 0) {
+          ok = seg == 0 || sm100::mbar_wait(&ctl.q_free, (seg - 1) & 1, abort_flag, p.status, kWaitQ);
+          if (ok) {
+            sm100::mbar_arrive_expect_tx(&ctl.q_full, kNTiles * boxes * rows * 128);
+            for (int c = 0; c < kNTiles; ++c) chunk(q_smem + c * kQChunk, &ctl.q_full, 64 * (c < 4 ? other + c : 8));
+          }
+        } else {
+          for (int h = 0; h < 2 && ok; ++h) {
+            const uint32_t s = (at + h) % kVSlots, use = (at + h) / kVSlots;
+            ok = use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
+            if (!ok) break;
+            sm100::mbar_arrive_expect_tx(&ctl.v_full[s], 2 * boxes * rows * 128);
+            for (int c = 0; c < 2; ++c)
+              chunk(v_ring + s * kVTiles * kTile + c * kQChunk, &ctl.v_full[s], 64 * (4 - other + 2 * h + c));
+          }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       ++seg;
-      sm100::tc_fence_after_sync();
-      for (int k = 0; k <= nb && ok; ++k) {
-        if (k < nb) {                          // S = Q . K^T of block k
-          const uint32_t d = tmem + kColS + (g_qk & 1) * kKeys;
-          for (int c = 0; c < kNTiles; ++c, ++n_at) {
-            const uint32_t s = n_at % kNSlots;
-            if (!warp_wait(&ctl.n_full[s], (n_at / kNSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
-            if (lane == 0) {
-              const uint64_t a = desc_sw128(q_addr + c * kQChunk, 16), b = desc_sw128(n_addr + s * kTile, 16);
+      if (ring == 1) at += 2;
+      keep(g & 1);
+      for (int k = 0; k < nb; ++k, ++g) {
+        const int j = w.begin() + k;
+        if (k + 1 < nb) look(w, j + 1);
+        if (elect_one()) {
+          const int boxes = (min(kKeys, w.s.len - j * kKeys) + p.box - 1) / p.box, bytes = boxes * p.box * 128;
+          const int row0 = (unsigned)(j * kKeys) % (unsigned)p.page_size;
+          const int* list = ctl.pages[ring][g & 1];
+          auto tile = [&](uint8_t* dst, uint64_t* bar, int col) {
+            int row = row0;
+            for (int e = 0; e < boxes; ++e) {
+              tma_load_3d(sm100::smem_u32(dst) + e * p.box * 128, &map, bar, col, row, list[e]);
+              row += p.box;
+              if (row == p.page_size) row = 0;
+            }
+          };
+          if (ring == 0) {
+            for (int c = 0; c < kNTiles; ++c) {
+              const uint32_t s = (at + c) % kNSlots, use = (at + c) / kNSlots;
+              ok = use == 0 || sm100::mbar_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
+              if (!ok) break;
+              sm100::mbar_arrive_expect_tx(&ctl.n_full[s], bytes);
+              tile(n_ring + s * kTile, &ctl.n_full[s], 64 * (c < 4 ? other + c : 8));
+            }
+          } else {
+            const uint32_t s = at % kVSlots, use = at / kVSlots;
+            ok = use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
+            if (ok) {
+              // a last block that the sequence does not fill goes to the clearing warp first
+              const bool last = w.s.len - j * kKeys < kKeys;
+              uint64_t* land = last ? &ctl.v_land[s] : &ctl.v_full[s];
+#pragma unroll
+              for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
+              sm100::mbar_arrive_expect_tx(land, kVTiles * bytes);
+              for (int c = 0; c < kVTiles; ++c) tile(v_ring + (s * kVTiles + c) * kTile, land, 64 * (4 - other + c));
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        at += ring == 0 ? kNTiles : 1;
+        if (k + 1 < nb) keep((g + 1) & 1);
+      }
+    }
+    // Giving up: nothing that is on its way may land after the CTA has ended. What was asked for in the last
+    // round of the slots is waited for (a slot of which nothing is missing answers at once, or the limit ends it).
+    if (__any_sync(0xffffffffu, !ok) && elect_one()) {
+      int never = 0;
+      const long long limit = 20000000LL;
+      const uint32_t slots = ring == 0 ? kNSlots : kVSlots, end = at + (ring == 0 ? kNTiles : 2);
+      for (uint32_t i = end > slots ? end - slots : 0; i < end; ++i) {
+        uint64_t* bar = ring == 0 ? &ctl.n_full[i % slots] : &ctl.v_full[i % slots];
+        sm100::mbar_wait_limited(bar, (i / slots) & 1, &never, nullptr, kWaitDrain, limit);
+      }
+#pragma unroll
+      for (int e = 0; e < kVSlots; ++e)
+        if (landed[e]) sm100::mbar_wait_limited(&ctl.v_land[e], (landed[e] - 1) & 1, &never, nullptr, kWaitDrain, limit);
+      if (ring == 0 && seg > 0) sm100::mbar_wait_limited(&ctl.q_full, (seg - 1) & 1, &never, nullptr, kWaitDrain, limit);
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    // ---------------------------------------------------------------- rows behind a sequence's end
+    // They may hold anything, also NaN, which a weight of zero would keep.
+    uint32_t v_at = 0, cleared[kVSlots] = {};
+    bool ok = true;
+    for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
+      if (w.blocks() > 0) v_at += 2;           // Q
+      const int nb = w.blocks(), valid = nb ? w.s.len - (w.begin() + nb - 1) * kKeys : kKeys;
+      if (valid < kKeys) {                     // only a segment's last block can be the sequence's last
+        const uint32_t s = (v_at + nb - 1) % kVSlots;
+        uint32_t uses = 0;
+#pragma unroll
+        for (int e = 0; e < kVSlots; ++e)
+          if (s == e) uses = cleared[e]++;
+        if (!warp_wait(&ctl.v_land[s], uses & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
+        uint8_t* v = v_ring + s * kVTiles * kTile;
+        for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)
+#pragma unroll
+          for (int c = 0; c < kVTiles; ++c) *reinterpret_cast<uint4*>(v + c * kTile + e * 16) = make_uint4(0, 0, 0, 0);
+        sm100::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&ctl.v_full[s]);
+      }
+      v_at += nb;
+    }
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- tensor core
+    // One thread: nothing here is done by a warp together.
+    if (elect_one()) {
+      constexpr uint32_t idesc_qk = sm100::umma_idesc(kFmt, kRows, kKeys);
+      constexpr uint32_t idesc_pv = sm100::umma_idesc(kFmt, kRows, kHalf) | (1u << 16);   // V: keys down, columns along
+      const uint64_t q_desc = desc_sw128(sm100::smem_u32(q_smem), 16), n_desc = desc_sw128(sm100::smem_u32(n_ring), 16);
+      const uint64_t vk_desc = desc_sw128(sm100::smem_u32(v_ring), 16), vn_desc = desc_sw128(sm100::smem_u32(v_ring), kTile);
+      uint32_t n_slot = 0, n_phase = 0, v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
+      bool ok = true;
+      for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
+        const int nb = w.blocks();
+        if (nb == 0) continue;
+        if (!sm100::mbar_wait(&ctl.q_full, seg & 1, abort_flag, p.status, kWaitQ) ||
+            !sm100::mbar_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ))
+          break;
+        ++seg;
+        for (int h = 0; h < 2; ++h, ++v_qk, ++v_pv) sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);   // Q's two slots: read
+        sm100::tc_fence_after_sync();
+        for (int k = 0; k <= nb; ++k) {
+          if (k < nb) {                        // S = Q . K^T of block k
+            const uint32_t d = tmem + kColS + (g_qk & 1) * kKeys;
+#pragma unroll 1
+            for (int c = 0; c < kNTiles; ++c) {
+              if (!sm100::mbar_wait(&ctl.n_full[n_slot], n_phase, abort_flag, p.status, kWaitN)) { ok = false; break; }
+              const uint64_t a = q_desc + c * (kQChunk >> 4), b = n_desc + n_slot * (kTile >> 4);
 #pragma unroll
               for (int k4 = 0; k4 < 4; ++k4) sm100::umma_f16(d, a + 2 * k4, b + 2 * k4, idesc_qk, (c > 0 || k4 > 0) ? 1u : 0u);
-              sm100::umma_commit(&ctl.n_empty[s]);
+              sm100::umma_commit(&ctl.n_empty[n_slot]);
+              if (++n_slot == kNSlots) { n_slot = 0; n_phase ^= 1; }
             }
-            __syncwarp();
-          }
-          if (!ok) break;
-          const uint32_t s = g_qk % kVSlots;
-          if (!warp_wait(&ctl.v_full[s], (g_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
-          const int valid = w.s.len - (w.begin() + k) * kKeys;
-          if (valid < kKeys) {
-            // rows behind the sequence's end may hold anything, also NaN, which a weight of zero would keep
-            uint8_t* v = v_ring + s * kVTiles * kTile;
-            for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)
-#pragma unroll
-              for (int c = 0; c < kVTiles; ++c) *reinterpret_cast<uint4*>(v + c * kTile + e * 16) = make_uint4(0, 0, 0, 0);
-            sm100::fence_proxy_async();
-            __syncwarp();
-          }
-          if (lane == 0) {
+            if (!ok) break;
+            const uint32_t s = v_qk % kVSlots;
+            if (!sm100::mbar_wait(&ctl.v_full[s], (v_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
 #pragma unroll
             for (int c = 0; c < kVTiles; ++c) {
-              const uint64_t b = desc_sw128(v_addr + (s * kVTiles + c) * kTile, 16);
+              const uint64_t b = vk_desc + (s * kVTiles + c) * (kTile >> 4);
 #pragma unroll
               for (int k4 = 0; k4 < 4; ++k4) umma_ts(d, tmem + kColQ + c * 32 + k4 * 8, b + 2 * k4, idesc_qk, 1u);
             }
             sm100::umma_commit(&ctl.s_full[g_qk & 1]);
+            if (k + 1 == nb) sm100::umma_commit(&ctl.q_free);
+            ++g_qk;
+            ++v_qk;
           }
-          __syncwarp();
-          ++g_qk;
-        }
-        if (k > 0) {                           // O += P . V of block k - 1
-          const uint32_t sb = g_pv & 1, s = g_pv % kVSlots;
-          if (!warp_wait(&ctl.p_full[sb], (g_pv >> 1) & 1, abort_flag, p.status, kWaitP)) { ok = false; break; }
-          sm100::tc_fence_after_sync();
-          if (lane == 0) {
-            const uint64_t b = desc_sw128(v_addr + s * kVTiles * kTile, kTile);
+          if (k > 0) {                         // O += P . V of block k - 1
+            const uint32_t sb = g_pv & 1, s = v_pv % kVSlots;
+            if (!sm100::mbar_wait(&ctl.p_full[sb], (g_pv >> 1) & 1, abort_flag, p.status, kWaitP)) { ok = false; break; }
+            sm100::tc_fence_after_sync();
+            const uint64_t b = vn_desc + s * kVTiles * (kTile >> 4);
 #pragma unroll
             for (int k4 = 0; k4 < kKeys / 16; ++k4)
               umma_ts(tmem + kColO, tmem + kColS + sb * kKeys + k4 * 8, b + (uint64_t)k4 * (2048 >> 4), idesc_pv,
                       (k > 1 || k4 > 0) ? 1u : 0u);
             sm100::umma_commit(&ctl.v_empty[s]);
             sm100::umma_commit(&ctl.pv_done[sb]);
+            ++g_pv;
+            ++v_pv;
           }
-          __syncwarp();
-          ++g_pv;
         }
       }
     }
+    __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, one row per thread
     const int row = threadIdx.x;
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    const T* q = static_cast<const T*>(p.q);
-    uint32_t g = 0;
+    uint32_t g = 0, v_at = 0;                  // blocks and value slots so far
     bool ok = true;
-    const int own = half * kHalf, oth = kHalf - own;
-    auto load_q = [&](const Walk& w) {
-      const T* rows = q + w.t.row0 * kD;
-      const uint32_t dst = sm100::smem_u32(q_smem);
-      // the other half and the rotary columns (32 + 8 pieces of 16 bytes a row) as five swizzled tiles; a warp
-      // copies its own 32 rows
-#pragma unroll 8
-      for (int e = lane; e < 32 * 40; e += 32) {
-        const int r = warp * 32 + e / 40, c = e % 40, chunk = c >> 3;
-        cp_async_16(dst + chunk * kQChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                    rows + (r < w.t.rows ? (size_t)r * kD : 0) + (c < 32 ? oth + c * 8 : kDv + (c - 32) * 8), r < w.t.rows);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      const uint4* src = reinterpret_cast<const uint4*>(rows + (size_t)min(row, w.t.rows - 1) * kD + own);
+    const int own = half * kHalf;
+    // This half's columns of Q: from two slots of the value ring (two tiles of 64 columns, 128 rows each) to tensor
+    // memory, a row per thread.
+    auto take_q = [&]() {
+      for (int h = 0; h < 2; ++h, ++v_at) {
+        const uint32_t s = v_at % kVSlots;
+        if (!warp_wait(&ctl.v_full[s], (v_at / kVSlots) & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t u[32];
+        for (int c = 0; c < 2; ++c) {
+          const uint8_t* src = v_ring + s * kVTiles * kTile + c * kQChunk + row * 128;
+          uint32_t u[32];
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          uint4 x = __ldg(src + c * 8 + v);
-          if (row >= w.t.rows) x = make_uint4(0, 0, 0, 0);
-          u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
+          for (int v = 0; v < 8; ++v) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + ((v ^ (row & 7)) << 4));
+            u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
+          }
+          tmem_st_32x32(lanes + kColQ + (2 * h + c) * 32, u);
         }
-        tmem_st_32x32(lanes + kColQ + c * 32, u);
       }
       tmem_st_wait();
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      sm100::fence_proxy_async();
       sm100::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&ctl.q_ready);
     };
 
     Walk w(p, ctl);
-    if (w.live() && w.blocks() > 0) load_q(w);
+    if (w.live() && w.blocks() > 0) take_q();
     while (w.live() && ok) {
       const int nb = w.blocks();
       // what this row sees: cache rows [lo, hi)
-      const int tok = (int)((w.t.row0 + row) / p.H) - w.s.tok;
+      const int tok = (int)((unsigned)(w.t.row0 + row) / (unsigned)p.H) - w.s.tok;
       const bool live = row < w.t.rows;
       int hi = p.causal ? min(w.s.len, w.s.pos + tok + 1) : w.s.len;
       const int lo = p.window > 0 ? (int)max(0LL, (long long)w.s.pos + tok + 1 - p.window) : 0;
@@ -588,7 +683,9 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
       // Q of the next tile may go in as soon as the last scores are out
       Walk nx = w;
       nx.next(p);
-      if (nx.live() && nx.blocks() > 0) load_q(nx);
+      v_at += nb;
+      if (nx.live() && nx.blocks() > 0) take_q();
+      if (!ok) break;
       if (nb > 0) {
         if (!warp_wait(&ctl.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
         sm100::tc_fence_after_sync();
@@ -598,7 +695,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
         if (w.whole()) {
           const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;    // NaN stays NaN
           const bool zero = l_sum == 0.f;
-          T* dst = static_cast<T*>(p.out) + (w.t.row0 + row) * kDv + own;
+          T* dst = static_cast<T*>(p.out) + (size_t)(w.t.row0 + row) * kDv + own;
 #pragma unroll 1
           for (int c = 0; c < kHalf; c += 32) {
             uint32_t o[32];
@@ -665,10 +762,8 @@ __global__ void __launch_bounds__(128) mla_paged_merge_kernel(const Params p) {
   if (row >= m.rows) return;
   const int col = threadIdx.x * 4, half = col >= kHalf;
   auto slot_of = [&](int k) { return (size_t)k * 2 + (k == m.first ? 1 : 0); };
-  auto empty = [&](int k) { return m.total * k / p.pairs == m.total * (k + 1) / p.pairs; };
   float top = -INFINITY;
   for (int k = m.first; k <= pair; ++k) {
-    if (empty(k)) continue;
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot_of(k) * 2 + half) * p.rows_cap + row) * 2);
     if (ml.y != 0.f) top = fmaxf(top, ml.x);
   }
@@ -676,7 +771,6 @@ __global__ void __launch_bounds__(128) mla_paged_merge_kernel(const Params p) {
   float l = 0.f;
 #pragma unroll 4
   for (int k = m.first; k <= pair; ++k) {
-    if (empty(k)) continue;
     const size_t slot = slot_of(k);
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot * 2 + half) * p.rows_cap + row) * 2);
     const float4 o = *reinterpret_cast<const float4*>(p.part_o + (slot * p.rows_cap + row) * kDv + col);
@@ -691,7 +785,7 @@ __global__ void __launch_bounds__(128) mla_paged_merge_kernel(const Params p) {
   uint2 r;
   r.x = zero ? 0u : pack2<T>(acc.x * inv, acc.y * inv);
   r.y = zero ? 0u : pack2<T>(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (m.row0 + row) * kDv + col) = r;
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)(m.row0 + row) * kDv + col) = r;
   if (threadIdx.x == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
 }
 
@@ -701,9 +795,9 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 int rows_cap_of(int T, int H) { return (int)((long long)T * H < kRows ? (long long)T * H : kRows); }
 
 template <typename T>
-int launch(Params& p, const CUtensorMap& map, cudaStream_t stream) {
+int launch(Params& p, const CUtensorMap (&map)[3], cudaStream_t stream) {
   if (!cab::ensure_dynamic_smem<&mla_paged_attention_kernel<T>>(kSmemBytes)) return CAB_ERR_LAUNCH;
-  mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, map);
+  mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, map[0], map[1], map[2]);
   const int rc = cab::launch_status();
   if (rc != CAB_OK || p.pairs == 1) return rc;
   mla_paged_merge_kernel<T><<<dim3(p.pairs, p.rows_cap), 128, 0, stream>>>(p);
@@ -766,15 +860,19 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.meta = reinterpret_cast<Meta*>(ws + align256(rows * kDv * 4) + align256(rows * 2 * 2 * 4));
   p.status = status;
 
-  CUtensorMap map;
+  CUtensorMap map[3];
   sm100::EncodeTiledFn encode = sm100::encode_tiled_fn();
   if (!encode) return CAB_ERR_LAUNCH;
   const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)batch->page_size, (cuuint64_t)batch->num_pages};
   const cuuint64_t strides[2] = {(cuuint64_t)batch->token_stride * 2, (cuuint64_t)batch->page_stride * 2};
   const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
-  if (encode(&map, batch->dtype == CAB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+  const CUtensorMapDataType type =
+      batch->dtype == CAB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (encode(&map[0], type, 3,
              batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+      !sm100::make_tmap_2d_sw128(&map[1], q, type, 2, (uint64_t)T * H, kD, kRows, 64) ||
+      !sm100::make_tmap_2d_sw128(&map[2], q, type, 2, (uint64_t)T * H, kD, kQBox, 64))
     return CAB_ERR_BAD_ARGUMENT;
   if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
   return batch->dtype == CAB_F16 ? launch<__half>(p, map, stream) : launch<__nv_bfloat16>(p, map, stream);
