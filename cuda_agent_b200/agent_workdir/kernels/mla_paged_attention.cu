@@ -8,13 +8,16 @@
 // each accumulates 256 of the value columns and computes the scores for itself (832 column steps instead of
 // 544; the alternative, exchanging partial scores between the CTAs, costs more than the second Q.K^T here).
 // Tensor memory: O 256 columns, S two buffers of 64, 256 columns of Q as the A operand in 128. P (16 bit)
-// overwrites the S it came from and is the A operand of P.V. Shared memory: the other 320 columns of Q (80 KB)
-// and two rings for blocks of 64 cache rows: 64-column tiles that only Q.K^T reads (six of 8 KB), and this
-// CTA's 256 value columns, which P.V reads as well (three blocks of 32 KB). A tile slot is released as soon as
-// its last reader is done, so every load has about a block's time to land.
+// overwrites the S it came from and is the A operand of P.V. Shared memory: the other 320 columns of Q (80 KB),
+// and of each block of 64 cache rows the 320 columns that only Q.K^T reads (40 KB, two buffers) and this CTA's 256
+// value columns, which P.V reads as well (32 KB, two buffers).
+// The tensor core takes, for each block j, the first part of Q.K^T of block j+1 (320 columns), P.V of block j, and
+// the rest of Q.K^T of block j+1 (256 columns). So the softmax of block j has the first part's time, and a buffer
+// is asked for again about 2000 clk (values) and 3000 clk (the rest) before it is read: rows come from either
+// die's L2, and with single buffers for the 320 columns the wait for them doubled the kernel's time.
 //   warps 0-3  one (token, head) row per thread: softmax, result. The reference maximum of a row moves only
 //              when it would grow by more than 2^8, so O is hardly ever rescaled
-//   warp 4     issues Q.K^T of block j+1 before P.V of block j: the tensor core works while the softmax does
+//   warp 4     issues the tensor instructions
 //   warps 5, 7 TMA, each for one of the rings: one box per run of rows that lie in one page. Q comes the same way,
 //              its tensor-memory half through two slots of the value ring
 //   warp 6     clears the rows behind a sequence's end in its last block of V
@@ -37,8 +40,8 @@ constexpr int kD = 576, kDv = 512, kHalf = 256;
 constexpr int kRows = 128;                     // (token, head) rows per tile
 constexpr int kKeys = 64;                      // cache rows per block
 constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 128-byte swizzle
-constexpr int kNTiles = 5, kVTiles = 4;        // tiles of a block: the other value half and the rotary columns / own half
-constexpr int kNSlots = 6, kVSlots = 3;
+constexpr int kNTiles = 5, kVTiles = 4;        // 64-column tiles of a block: the other value half and the rotary columns / own half
+constexpr int kNSlots = 2, kVSlots = 2;
 constexpr int kQChunk = kRows * 128;
 constexpr int kThreads = 8 * 32;
 constexpr int kQBox = 16;                      // rows of the small box for Q
@@ -56,7 +59,7 @@ struct __align__(16) Control {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int kRingBytes = kNSlots * kTile + kVSlots * kVTiles * kTile;
+constexpr int kRingBytes = (kNSlots * kNTiles + kVSlots * kVTiles) * kTile;
 constexpr int kSmemBytes = kNTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
 static_assert(kSmemBytes <= 232448 && (kMaxBatch + 2) * 4 <= kRingBytes, "shared memory");
 
@@ -69,7 +72,11 @@ struct Params {
   void* out;
   float* lse;
   const int *page_table, *q_start, *kv_len;
-  int T, H, batch, max_pages, num_pages, page_size, box;
+  int T, H, batch, max_pages, num_pages, page_size;
+  int box, box_log2;                           // rows of a TMA box, all in one page
+  int step_pages, step_rows;                   // 64 rows further = so many pages and rows
+  uint32_t tile_bytes;                         // from one 64-column tile of a part to the next: 8192, or 1024 where the
+                                               // tiles of eight rows lie after one another
   int tail;                                    // write the tokens behind the last sequence as such that see nothing
   int causal, window, rows_cap, pairs;
   float scale_log2;
@@ -91,10 +98,10 @@ __device__ __forceinline__ int load_now(const int* p) {
   asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -118,8 +125,8 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t lbo) {
-  return (uint64_t)((smem_addr >> 4) & 0x3fff) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fff) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -147,6 +154,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&h);
   }
 }
+
+// Cache rows as (64 columns, row in the page, column tile, page): boxes of 1, 4 and 5 tiles; Q: boxes of 128 and 16 rows.
+struct Maps { CUtensorMap one, four, five, q, q16; };
 
 // A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
 struct Seq { int tok, n, len, pos; };
@@ -314,13 +324,12 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
-mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap map,
-                           const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q16) {
+mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = base;
   uint8_t* n_ring = base + kNTiles * kQChunk;
-  uint8_t* v_ring = n_ring + kNSlots * kTile;
+  uint8_t* v_ring = n_ring + kNSlots * kNTiles * kTile;
   Control& ctl = *reinterpret_cast<Control*>(v_ring + kVSlots * kVTiles * kTile);
   // the same in all lanes, and known to be: the tensor instructions take their operands from uniform registers
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -346,8 +355,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
     sm100::tmem_relinquish();
   }
   if (warp == 5 && lane == 0) {
-    sm100::prefetch_tensormap(&map);
-    sm100::prefetch_tensormap(&map_q);
+    sm100::prefetch_tensormap(&maps.one);
+    sm100::prefetch_tensormap(&maps.four);
+    sm100::prefetch_tensormap(&maps.five);
+    sm100::prefetch_tensormap(&maps.q);
+    sm100::prefetch_tensormap(&maps.q16);
   }
   find_run(p, ctl, reinterpret_cast<int*>(n_ring), pair);
   sm100::fence_proxy_async();                  // the rings were used as scratch
@@ -362,35 +374,51 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
     // ---------------------------------------------------------------- loads
     const int ring = warp == 7;                // 0: the tiles that only Q.K^T reads, 1: V
     const int other = half ? 0 : 4;            // first of the four column tiles of the other value half
-    uint32_t at = 0, g = 0, seg = 0;           // slots filled, blocks, segments so far
+    uint32_t at = 0, g = 0, seg = 0;           // value slots filled (with Q), blocks, segments so far
     uint32_t landed[kVSlots] = {};
     bool ok = true;
-    // pages of this lane's boxes (two when a box is a single row) in block j
-    int page[2];
+    // This lane's boxes in a block (two when a box is a single row): pages and rows from the block's first row on.
+    int box_pages[2], box_rows[2], page[2], first_page = 0, first_row = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned off = (unsigned)(lane + 32 * k) << p.box_log2;
+      box_pages[k] = off / (unsigned)p.page_size;
+      box_rows[k] = off % (unsigned)p.page_size;
+    }
     auto look = [&](const Walk& w, int j) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int key = j * kKeys + (lane + 32 * k) * p.box;       // lengths end below 2^31 - 256
-        const bool in = (lane + 32 * k) * p.box < kKeys && key < w.s.len;
-        page[k] = in ? load_now(p.page_table + (size_t)w.b * p.max_pages + (unsigned)key / (unsigned)p.page_size) : 0;
+        const int off = (lane + 32 * k) << p.box_log2;
+        const int at = first_page + box_pages[k] + (first_row + box_rows[k] >= p.page_size);
+        page[k] = off < kKeys && j * kKeys + off < w.s.len ? load_now(p.page_table + (size_t)w.b * p.max_pages + at) : 0;
       }
     };
+    auto step = [&]() {                        // to the next block
+      first_page += p.step_pages;
+      first_row += p.step_rows;
+      if (first_row >= p.page_size) { first_row -= p.page_size; ++first_page; }
+    };
     auto keep = [&](int parity) {              // one outside the pool: TMA fills with zeros
+      __syncwarp();
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const bool bad = (unsigned)page[k] >= (unsigned)p.num_pages;
-        if (bad && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
-        ctl.pages[ring][parity][lane + 32 * k] = bad ? p.num_pages : page[k];
+        if ((unsigned)page[k] >= (unsigned)p.num_pages) {
+          if (p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
+          page[k] = p.num_pages;
+        }
+        if (k == 0 || p.box == 1) ctl.pages[ring][parity][lane + 32 * k] = page[k];
       }
       __syncwarp();
     };
     for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
       const int nb = w.blocks();
       if (nb == 0) continue;
+      first_page = (unsigned)(w.begin() * kKeys) / (unsigned)p.page_size;
+      first_row = (unsigned)(w.begin() * kKeys) % (unsigned)p.page_size;
       look(w, w.begin());
       if (elect_one()) {                       // Q of this tile
         const int boxes = w.t.rows > 4 * kQBox ? 1 : (w.t.rows + kQBox - 1) / kQBox, rows = w.t.rows > 4 * kQBox ? kRows : kQBox;
-        const CUtensorMap* m = w.t.rows > 4 * kQBox ? &map_q : &map_q16;
+        const CUtensorMap* m = w.t.rows > 4 * kQBox ? &maps.q : &maps.q16;
         auto chunk = [&](uint8_t* dst, uint64_t* bar, int col) {
           for (int e = 0; e < boxes; ++e)
             tma_load_2d(sm100::smem_u32(dst) + e * rows * 128, m, bar, col, w.t.row0 + e * rows);
@@ -418,45 +446,56 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
       if (ring == 1) at += 2;
       keep(g & 1);
       for (int k = 0; k < nb; ++k, ++g) {
-        const int j = w.begin() + k;
+        const int j = w.begin() + k, row0 = first_row;
+        step();
         if (k + 1 < nb) look(w, j + 1);
         if (elect_one()) {
-          const int boxes = (min(kKeys, w.s.len - j * kKeys) + p.box - 1) / p.box, bytes = boxes * p.box * 128;
-          const int row0 = (unsigned)(j * kKeys) % (unsigned)p.page_size;
+          const int left = w.s.len - j * kKeys;
+          const int boxes = (min(kKeys, left) + p.box - 1) >> p.box_log2, bytes = boxes * p.box * 128;
           const int* list = ctl.pages[ring][g & 1];
-          auto tile = [&](uint8_t* dst, uint64_t* bar, int col) {
+          // `tiles` tiles of each box from column tile `from` on, as tiles t .. of a part of `all` tiles
+          auto load = [&](uint32_t dst, uint64_t* bar, int from, int tiles, int t, int all) {
+            const uint32_t box_bytes = p.tile_bytes == 1024 ? all * 1024 : p.box * 128;
+            const CUtensorMap* map = tiles == 1 ? &maps.one : tiles == 4 ? &maps.four : &maps.five;
+            dst += t * p.tile_bytes;
             int row = row0;
-            for (int e = 0; e < boxes; ++e) {
-              tma_load_3d(sm100::smem_u32(dst) + e * p.box * 128, &map, bar, col, row, list[e]);
+            for (int e = 0; e < boxes; ++e, dst += box_bytes) {
+              tma_load_4d(dst, map, bar, 0, row, from, list[e]);
               row += p.box;
               if (row == p.page_size) row = 0;
             }
           };
+          const bool joint = p.box >= 8;       // boxes of several tiles keep the eight-row groups that swizzling wants
+          auto part = [&](uint8_t* dst, uint64_t* bar, int from, int tiles, int t, int all) {
+            if (joint) load(sm100::smem_u32(dst), bar, from, tiles, t, all);
+            else for (int c = 0; c < tiles; ++c) load(sm100::smem_u32(dst), bar, from + c, 1, t + c, all);
+          };
           if (ring == 0) {
-            for (int c = 0; c < kNTiles; ++c) {
-              const uint32_t s = (at + c) % kNSlots, use = (at + c) / kNSlots;
-              ok = use == 0 || sm100::mbar_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
-              if (!ok) break;
-              sm100::mbar_arrive_expect_tx(&ctl.n_full[s], bytes);
-              tile(n_ring + s * kTile, &ctl.n_full[s], 64 * (c < 4 ? other + c : 8));
+            const uint32_t s = g % kNSlots, use = g / kNSlots;
+            ok = use == 0 || sm100::mbar_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
+            if (ok) {
+              uint8_t* dst = n_ring + s * kNTiles * kTile;
+              sm100::mbar_arrive_expect_tx(&ctl.n_full[s], kNTiles * bytes);
+              if (half == 0) part(dst, &ctl.n_full[s], 4, 5, 0, kNTiles);
+              else { part(dst, &ctl.n_full[s], 0, 4, 0, kNTiles); part(dst, &ctl.n_full[s], 8, 1, 4, kNTiles); }
             }
           } else {
             const uint32_t s = at % kVSlots, use = at / kVSlots;
             ok = use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
             if (ok) {
               // a last block that the sequence does not fill goes to the clearing warp first
-              const bool last = w.s.len - j * kKeys < kKeys;
+              const bool last = left < kKeys;
               uint64_t* land = last ? &ctl.v_land[s] : &ctl.v_full[s];
 #pragma unroll
               for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
               sm100::mbar_arrive_expect_tx(land, kVTiles * bytes);
-              for (int c = 0; c < kVTiles; ++c) tile(v_ring + (s * kVTiles + c) * kTile, land, 64 * (4 - other + c));
+              part(v_ring + s * kVTiles * kTile, land, 4 - other, kVTiles, 0, kVTiles);
             }
           }
         }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        at += ring == 0 ? kNTiles : 1;
+        ++at;
         if (k + 1 < nb) keep((g + 1) & 1);
       }
     }
@@ -465,10 +504,13 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
     if (__any_sync(0xffffffffu, !ok) && elect_one()) {
       int never = 0;
       const long long limit = 20000000LL;
-      const uint32_t slots = ring == 0 ? kNSlots : kVSlots, end = at + (ring == 0 ? kNTiles : 2);
-      for (uint32_t i = end > slots ? end - slots : 0; i < end; ++i) {
-        uint64_t* bar = ring == 0 ? &ctl.n_full[i % slots] : &ctl.v_full[i % slots];
-        sm100::mbar_wait_limited(bar, (i / slots) & 1, &never, nullptr, kWaitDrain, limit);
+      if (ring == 0) {
+        for (uint32_t i = g + 1 > kNSlots ? g + 1 - kNSlots : 0; i < g + 1; ++i)
+          sm100::mbar_wait_limited(&ctl.n_full[i % kNSlots], (i / kNSlots) & 1, &never, nullptr, kWaitDrain, limit);
+      } else {
+        const uint32_t end = at + 2;
+        for (uint32_t i = end > kVSlots ? end - kVSlots : 0; i < end; ++i)
+          sm100::mbar_wait_limited(&ctl.v_full[i % kVSlots], (i / kVSlots) & 1, &never, nullptr, kWaitDrain, limit);
       }
 #pragma unroll
       for (int e = 0; e < kVSlots; ++e)
@@ -492,9 +534,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
           if (s == e) uses = cleared[e]++;
         if (!warp_wait(&ctl.v_land[s], uses & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
         uint8_t* v = v_ring + s * kVTiles * kTile;
-        for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)
+        const uint32_t group = p.tile_bytes == 1024 ? kVTiles * 1024 : 1024;
+        for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)   // 16 bytes each, 64 to eight rows
 #pragma unroll
-          for (int c = 0; c < kVTiles; ++c) *reinterpret_cast<uint4*>(v + c * kTile + e * 16) = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < kVTiles; ++c)
+            *reinterpret_cast<uint4*>(v + c * p.tile_bytes + (e >> 6) * group + (e & 63) * 16) = make_uint4(0, 0, 0, 0);
         sm100::fence_proxy_async();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&ctl.v_full[s]);
@@ -507,9 +551,14 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
     if (elect_one()) {
       constexpr uint32_t idesc_qk = sm100::umma_idesc(kFmt, kRows, kKeys);
       constexpr uint32_t idesc_pv = sm100::umma_idesc(kFmt, kRows, kHalf) | (1u << 16);   // V: keys down, columns along
-      const uint64_t q_desc = desc_sw128(sm100::smem_u32(q_smem), 16), n_desc = desc_sw128(sm100::smem_u32(n_ring), 16);
-      const uint64_t vk_desc = desc_sw128(sm100::smem_u32(v_ring), 16), vn_desc = desc_sw128(sm100::smem_u32(v_ring), kTile);
-      uint32_t n_slot = 0, n_phase = 0, v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
+      // parts of a block, by what the boxes left: tiles of 8 KB, or the tiles of eight rows after one another
+      const bool by_rows = p.tile_bytes == 1024;
+      const uint64_t q_desc = desc_sw128(sm100::smem_u32(q_smem), 16, 1024);
+      const uint64_t n_desc = desc_sw128(sm100::smem_u32(n_ring), 16, by_rows ? kNTiles * 1024 : 1024);
+      const uint32_t v_group = by_rows ? kVTiles * 1024 : 1024, tile = p.tile_bytes >> 4;
+      const uint64_t vk_desc = desc_sw128(sm100::smem_u32(v_ring), 16, v_group);
+      const uint64_t vn_desc = desc_sw128(sm100::smem_u32(v_ring), p.tile_bytes, v_group);
+      uint32_t v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
       bool ok = true;
       for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
         const int nb = w.blocks();
@@ -521,30 +570,17 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
         for (int h = 0; h < 2; ++h, ++v_qk, ++v_pv) sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);   // Q's two slots: read
         sm100::tc_fence_after_sync();
         for (int k = 0; k <= nb; ++k) {
-          if (k < nb) {                        // S = Q . K^T of block k
-            const uint32_t d = tmem + kColS + (g_qk & 1) * kKeys;
-#pragma unroll 1
-            for (int c = 0; c < kNTiles; ++c) {
-              if (!sm100::mbar_wait(&ctl.n_full[n_slot], n_phase, abort_flag, p.status, kWaitN)) { ok = false; break; }
-              const uint64_t a = q_desc + c * (kQChunk >> 4), b = n_desc + n_slot * (kTile >> 4);
+          const uint32_t d = tmem + kColS + (g_qk & 1) * kKeys;
+          if (k < nb) {                        // S = Q . K^T of block k over 320 columns
+            const uint32_t s = g_qk % kNSlots;
+            if (!sm100::mbar_wait(&ctl.n_full[s], (g_qk / kNSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
+            const uint64_t b = n_desc + s * kNTiles * (kTile >> 4);
 #pragma unroll
-              for (int k4 = 0; k4 < 4; ++k4) sm100::umma_f16(d, a + 2 * k4, b + 2 * k4, idesc_qk, (c > 0 || k4 > 0) ? 1u : 0u);
-              sm100::umma_commit(&ctl.n_empty[n_slot]);
-              if (++n_slot == kNSlots) { n_slot = 0; n_phase ^= 1; }
-            }
-            if (!ok) break;
-            const uint32_t s = v_qk % kVSlots;
-            if (!sm100::mbar_wait(&ctl.v_full[s], (v_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
+            for (int c = 0; c < kNTiles; ++c)
 #pragma unroll
-            for (int c = 0; c < kVTiles; ++c) {
-              const uint64_t b = vk_desc + (s * kVTiles + c) * (kTile >> 4);
-#pragma unroll
-              for (int k4 = 0; k4 < 4; ++k4) umma_ts(d, tmem + kColQ + c * 32 + k4 * 8, b + 2 * k4, idesc_qk, 1u);
-            }
-            sm100::umma_commit(&ctl.s_full[g_qk & 1]);
-            if (k + 1 == nb) sm100::umma_commit(&ctl.q_free);
-            ++g_qk;
-            ++v_qk;
+              for (int k4 = 0; k4 < 4; ++k4)
+                sm100::umma_f16(d, q_desc + c * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk, (c > 0 || k4 > 0) ? 1u : 0u);
+            sm100::umma_commit(&ctl.n_empty[s]);
           }
           if (k > 0) {                         // O += P . V of block k - 1
             const uint32_t sb = g_pv & 1, s = v_pv % kVSlots;
@@ -553,12 +589,26 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ CUtensorMap m
             const uint64_t b = vn_desc + s * kVTiles * (kTile >> 4);
 #pragma unroll
             for (int k4 = 0; k4 < kKeys / 16; ++k4)
-              umma_ts(tmem + kColO, tmem + kColS + sb * kKeys + k4 * 8, b + (uint64_t)k4 * (2048 >> 4), idesc_pv,
+              umma_ts(tmem + kColO, tmem + kColS + sb * kKeys + k4 * 8, b + k4 * (v_group >> 3), idesc_pv,
                       (k > 1 || k4 > 0) ? 1u : 0u);
             sm100::umma_commit(&ctl.v_empty[s]);
             sm100::umma_commit(&ctl.pv_done[sb]);
             ++g_pv;
             ++v_pv;
+          }
+          if (k < nb) {                        // S += Q . K^T of block k over this CTA's value columns
+            const uint32_t s = v_qk % kVSlots;
+            if (!sm100::mbar_wait(&ctl.v_full[s], (v_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
+#pragma unroll
+            for (int c = 0; c < kVTiles; ++c) {
+              const uint64_t b = vk_desc + s * kVTiles * (kTile >> 4) + c * tile;
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) umma_ts(d, tmem + kColQ + c * 32 + k4 * 8, b + 2 * k4, idesc_qk, 1u);
+            }
+            sm100::umma_commit(&ctl.s_full[g_qk & 1]);
+            if (k + 1 == nb) sm100::umma_commit(&ctl.q_free);
+            ++g_qk;
+            ++v_qk;
           }
         }
       }
@@ -795,9 +845,9 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 int rows_cap_of(int T, int H) { return (int)((long long)T * H < kRows ? (long long)T * H : kRows); }
 
 template <typename T>
-int launch(Params& p, const CUtensorMap (&map)[3], cudaStream_t stream) {
+int launch(Params& p, const Maps& maps, cudaStream_t stream) {
   if (!cab::ensure_dynamic_smem<&mla_paged_attention_kernel<T>>(kSmemBytes)) return CAB_ERR_LAUNCH;
-  mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, map[0], map[1], map[2]);
+  mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, maps);
   const int rc = cab::launch_status();
   if (rc != CAB_OK || p.pairs == 1) return rc;
   mla_paged_merge_kernel<T><<<dim3(p.pairs, p.rows_cap), 128, 0, stream>>>(p);
@@ -841,9 +891,17 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.page_table = batch->page_table; p.q_start = batch->q_start; p.kv_len = batch->kv_len;
   p.T = T; p.H = H; p.batch = batch->batch; p.tail = tail;
   p.max_pages = batch->max_pages; p.num_pages = batch->num_pages; p.page_size = batch->page_size;
-  int box = 1;                                 // rows that are sure to lie in one page: a box of the tensor map
+  // Rows that are sure to lie in one page. 64: a box takes several tiles, each 8 KB. 8: several tiles too, and the
+  // tiles of eight rows lie after one another (eight is what the swizzle repeats after, so 16 and 32 go as 8: fewer
+  // instructions than a box per tile). Below: a box per tile.
+  int box = 1;
   while (box < kKeys && batch->page_size % (2 * box) == 0) box *= 2;
+  if (box > 8 && box < kKeys) box = 8;
   p.box = box;
+  p.box_log2 = 0;
+  while ((1 << p.box_log2) < box) ++p.box_log2;
+  p.step_pages = kKeys / batch->page_size; p.step_rows = kKeys % batch->page_size;
+  p.tile_bytes = box == 8 ? 1024 : kTile;
   p.causal = causal != 0;
   p.window = window < (long long)batch->max_pages * batch->page_size ? window : 0;   // wider than any history: none
   p.rows_cap = rows_cap_of(T, H);
@@ -860,20 +918,23 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.meta = reinterpret_cast<Meta*>(ws + align256(rows * kDv * 4) + align256(rows * 2 * 2 * 4));
   p.status = status;
 
-  CUtensorMap map[3];
+  Maps maps;
   sm100::EncodeTiledFn encode = sm100::encode_tiled_fn();
   if (!encode) return CAB_ERR_LAUNCH;
-  const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)batch->page_size, (cuuint64_t)batch->num_pages};
-  const cuuint64_t strides[2] = {(cuuint64_t)batch->token_stride * 2, (cuuint64_t)batch->page_stride * 2};
-  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
   const CUtensorMapDataType type =
       batch->dtype == CAB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (encode(&map[0], type, 3,
-             batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
-      !sm100::make_tmap_2d_sw128(&map[1], q, type, 2, (uint64_t)T * H, kD, kRows, 64) ||
-      !sm100::make_tmap_2d_sw128(&map[2], q, type, 2, (uint64_t)T * H, kD, kQBox, 64))
+  const cuuint64_t dims[4] = {64, (cuuint64_t)batch->page_size, kD / 64, (cuuint64_t)batch->num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)batch->token_stride * 2, 128, (cuuint64_t)batch->page_stride * 2};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  auto make = [&](CUtensorMap* map, int tiles) {
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, (cuuint32_t)tiles, 1};
+    return encode(map, type, 4, batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (!make(&maps.one, 1) || !make(&maps.four, 4) || !make(&maps.five, 5)) return CAB_ERR_BAD_ARGUMENT;
+  if (!sm100::make_tmap_2d_sw128(&maps.q, q, type, 2, (uint64_t)T * H, kD, kRows, 64) ||
+      !sm100::make_tmap_2d_sw128(&maps.q16, q, type, 2, (uint64_t)T * H, kD, kQBox, 64))
     return CAB_ERR_BAD_ARGUMENT;
   if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
-  return batch->dtype == CAB_F16 ? launch<__half>(p, map, stream) : launch<__nv_bfloat16>(p, map, stream);
+  return batch->dtype == CAB_F16 ? launch<__half>(p, maps, stream) : launch<__nv_bfloat16>(p, maps, stream);
 }
