@@ -7,19 +7,19 @@
 // A tile of 128 rows times 512 value columns of fp32 would take all of tensor memory, so two CTAs share a tile:
 // each accumulates 256 of the value columns and computes the scores for itself (832 column steps instead of
 // 544; the alternative, exchanging partial scores between the CTAs, costs more than the second Q.K^T here).
-// Tensor memory: O 256 columns, S two buffers of 64, 256 columns of Q as the A operand in 128. P (16 bit)
-// overwrites the S it came from and is the A operand of P.V. Shared memory: the other 320 columns of Q (80 KB),
-// and of each block of 64 cache rows the 320 columns that only Q.K^T reads (40 KB, two buffers) and this CTA's 256
-// value columns, which P.V reads as well (32 KB, two buffers).
-// The tensor core takes, for each block j, the first part of Q.K^T of block j+1 (320 columns), P.V of block j, and
-// the rest of Q.K^T of block j+1 (256 columns). So the softmax of block j has the first part's time, and a buffer
-// is asked for again about 2000 clk (values) and 3000 clk (the rest) before it is read: rows come from either
-// die's L2, and with single buffers for the 320 columns the wait for them doubled the kernel's time.
+// Tensor memory: O 256 columns, S 64, P (16 bit, the A operand of P.V) 32, and 160 for 320 columns of Q as the A
+// operand: this CTA's value half and the rotary columns. Shared memory: the other 256 columns of Q (64 KB) and rings
+// for what a block of 64 cache rows has: the other value half, which only Q.K^T reads, in two units of 128 columns
+// (16 KB, three slots), the rotary columns (8 KB, two slots), and this CTA's value half, which P.V reads as well
+// (32 KB, three slots). The tensor core takes Q.K^T of block j+1 and then P.V of block j, so the softmax of block j
+// has the time of a Q.K^T, and every slot is asked for again 2000 clk or more before it is read: a row comes from
+// either die's L2, 1600 to 2800 clk away under load. (With one buffer for the part that only Q.K^T reads, the wait
+// for it doubled the kernel's time; with P.V between the parts of Q.K^T and two slots a softmax of 1100 clk showed.)
 //   warps 0-3  one (token, head) row per thread: softmax, result. The reference maximum of a row moves only
 //              when it would grow by more than 2^8, so O is hardly ever rescaled
 //   warp 4     issues the tensor instructions
-//   warps 5, 7 TMA, each for one of the rings: one box per run of rows that lie in one page. Q comes the same way,
-//              its tensor-memory half through two slots of the value ring
+//   warps 5, 7 TMA, one for the other half's ring, one for the other two rings: one box per run of rows that lie in one
+//              page. Q comes the same way, its tensor-memory part through two slots of either of the latter rings
 //   warp 6     clears the rows behind a sequence's end in its last block of V
 // Whoever issues tensor or TMA instructions does so in one elected thread, waits included: the operands then sit
 // in uniform registers, and a wait polled by 32 lanes costs some 300 clk more than one polled by a single lane.
@@ -40,18 +40,20 @@ constexpr int kD = 576, kDv = 512, kHalf = 256;
 constexpr int kRows = 128;                     // (token, head) rows per tile
 constexpr int kKeys = 64;                      // cache rows per block
 constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 128-byte swizzle
-constexpr int kNTiles = 5, kVTiles = 4;        // 64-column tiles of a block: the other value half and the rotary columns / own half
-constexpr int kNSlots = 2, kVSlots = 2;
+// 64-column tiles of a block: units of the other value half, the rotary columns, own value half
+constexpr int kNTiles = 2, kNUnits = 2, kVTiles = 4, kQTiles = kNTiles * kNUnits;
+constexpr int kNSlots = 3, kRSlots = 2, kVSlots = 3;
 constexpr int kQChunk = kRows * 128;
 constexpr int kThreads = 8 * 32;
 constexpr int kQBox = 16;                      // rows of the small box for Q
-constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384, kTmemCols = 512;
+constexpr uint32_t kColO = 0, kColS = 256, kColP = 320, kColQ = 352, kTmemCols = 512;
 constexpr float kRescale = 8.f;
 constexpr int kMaxBatch = 16384;
-enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitDrain };
+enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitRead };
 
 struct __align__(16) Control {
-  uint64_t n_full[kNSlots], n_empty[kNSlots], v_full[kVSlots], v_empty[kVSlots], v_land[kVSlots], s_full[2], p_full[2], pv_done[2], q_ready, q_full, q_free;
+  uint64_t n_full[kNSlots], n_empty[kNSlots], r_full[kRSlots], r_empty[kRSlots], v_full[kVSlots], v_empty[kVSlots],
+      v_land[kVSlots], s_full, s_read, p_full, pv_done, q_ready, q_full, q_free;
   long long scan[kThreads / 32], total;
   long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
   int seq, tile;                               // its first tile
@@ -59,8 +61,8 @@ struct __align__(16) Control {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int kRingBytes = (kNSlots * kNTiles + kVSlots * kVTiles) * kTile;
-constexpr int kSmemBytes = kNTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
+constexpr int kRingBytes = (kNSlots * kNTiles + kRSlots + kVSlots * kVTiles) * kTile;
+constexpr int kSmemBytes = kQTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
 static_assert(kSmemBytes <= 232448 && (kMaxBatch + 2) * 4 <= kRingBytes, "shared memory");
 
 // What the merge kernel has to know of the tile that a pair ends: its first (token, head) row, its rows, and the pair
@@ -155,8 +157,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Cache rows as (64 columns, row in the page, column tile, page): boxes of 1, 4 and 5 tiles; Q: boxes of 128 and 16 rows.
-struct Maps { CUtensorMap one, four, five, q, q16; };
+// Cache rows as (64 columns, row in the page, column tile, page): boxes of 1, 2 and 4 tiles; Q: boxes of 128, 64
+// and 16 rows.
+struct Maps { CUtensorMap one, two, four, q, q64, q16; };
 
 // A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
 struct Seq { int tok, n, len, pos; };
@@ -328,8 +331,9 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = base;
-  uint8_t* n_ring = base + kNTiles * kQChunk;
-  uint8_t* v_ring = n_ring + kNSlots * kNTiles * kTile;
+  uint8_t* n_ring = base + kQTiles * kQChunk;
+  uint8_t* r_ring = n_ring + kNSlots * kNTiles * kTile;
+  uint8_t* v_ring = r_ring + kRSlots * kTile;
   Control& ctl = *reinterpret_cast<Control*>(v_ring + kVSlots * kVTiles * kTile);
   // the same in all lanes, and known to be: the tensor instructions take their operands from uniform registers
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -338,12 +342,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < kNSlots; ++s) { sm100::mbar_init(&ctl.n_full[s], 1); sm100::mbar_init(&ctl.n_empty[s], 1); }
     for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_full[s], 1); sm100::mbar_init(&ctl.v_empty[s], 1); sm100::mbar_init(&ctl.v_land[s], 1); }
-    // by block parity. pv_done too: a softmax thread may wait for P.V of block j while that of j - 1 is not done
-    for (int s = 0; s < 2; ++s) {
-      sm100::mbar_init(&ctl.s_full[s], 1);
-      sm100::mbar_init(&ctl.p_full[s], 4);
-      sm100::mbar_init(&ctl.pv_done[s], 1);
-    }
+    for (int s = 0; s < kRSlots; ++s) { sm100::mbar_init(&ctl.r_full[s], 1); sm100::mbar_init(&ctl.r_empty[s], 1); }
+    sm100::mbar_init(&ctl.s_full, 1);
+    sm100::mbar_init(&ctl.s_read, 4);
+    sm100::mbar_init(&ctl.p_full, 4);
+    sm100::mbar_init(&ctl.pv_done, 1);
     sm100::mbar_init(&ctl.q_ready, 4);
     sm100::mbar_init(&ctl.q_full, 1);
     sm100::mbar_init(&ctl.q_free, 1);
@@ -355,11 +358,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     sm100::tmem_relinquish();
   }
   if (warp == 5 && lane == 0) {
-    sm100::prefetch_tensormap(&maps.one);
-    sm100::prefetch_tensormap(&maps.four);
-    sm100::prefetch_tensormap(&maps.five);
-    sm100::prefetch_tensormap(&maps.q);
-    sm100::prefetch_tensormap(&maps.q16);
+    for (const CUtensorMap* m : {&maps.one, &maps.two, &maps.four, &maps.q, &maps.q64, &maps.q16}) sm100::prefetch_tensormap(m);
   }
   find_run(p, ctl, reinterpret_cast<int*>(n_ring), pair);
   sm100::fence_proxy_async();                  // the rings were used as scratch
@@ -372,9 +371,9 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 
   if (warp == 5 || warp == 7) {
     // ---------------------------------------------------------------- loads
-    const int ring = warp == 7;                // 0: the tiles that only Q.K^T reads, 1: V
+    const int ring = warp == 7;                // 0: the other value half, 1: own half and the rotary columns
     const int other = half ? 0 : 4;            // first of the four column tiles of the other value half
-    uint32_t at = 0, g = 0, seg = 0;           // value slots filled (with Q), blocks, segments so far
+    uint32_t at = 0, r_at = 0, g = 0, seg = 0; // slots of ring 0 or of V (with Q), of the rotary ring, blocks, segments
     uint32_t landed[kVSlots] = {};
     bool ok = true;
     // This lane's boxes in a block (two when a box is a single row): pages and rows from the block's first row on.
@@ -426,11 +425,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         if (ring == 0) {
           ok = seg == 0 || sm100::mbar_wait(&ctl.q_free, (seg - 1) & 1, abort_flag, p.status, kWaitQ);
           if (ok) {
-            sm100::mbar_arrive_expect_tx(&ctl.q_full, kNTiles * boxes * rows * 128);
-            for (int c = 0; c < kNTiles; ++c) chunk(q_smem + c * kQChunk, &ctl.q_full, 64 * (c < 4 ? other + c : 8));
+            sm100::mbar_arrive_expect_tx(&ctl.q_full, kQTiles * boxes * rows * 128);
+            for (int c = 0; c < kQTiles; ++c) chunk(q_smem + c * kQChunk, &ctl.q_full, 64 * (other + c));
           }
         } else {
-          for (int h = 0; h < 2 && ok; ++h) {
+          for (int h = 0; h < 2 && ok; ++h) {  // two tiles of this half's columns
             const uint32_t s = (at + h) % kVSlots, use = (at + h) / kVSlots;
             ok = use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
             if (!ok) break;
@@ -438,12 +437,27 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             for (int c = 0; c < 2; ++c)
               chunk(v_ring + s * kVTiles * kTile + c * kQChunk, &ctl.v_full[s], 64 * (4 - other + 2 * h + c));
           }
+          for (int h = 0; h < 2 && ok; ++h) {  // 64 rows of the rotary columns
+            const uint32_t s = (r_at + h) % kRSlots, use = (r_at + h) / kRSlots;
+            ok = use == 0 || sm100::mbar_wait(&ctl.r_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
+            if (!ok) break;
+            uint8_t* dst = r_ring + s * kTile;
+            if (rows == kRows) {
+              sm100::mbar_arrive_expect_tx(&ctl.r_full[s], kTile);
+              tma_load_2d(sm100::smem_u32(dst), &maps.q64, &ctl.r_full[s], kDv, w.t.row0 + 64 * h);
+            } else if (h == 0) {
+              sm100::mbar_arrive_expect_tx(&ctl.r_full[s], boxes * rows * 128);
+              chunk(dst, &ctl.r_full[s], kDv);
+            } else {
+              sm100::mbar_arrive(&ctl.r_full[s]);
+            }
+          }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       ++seg;
-      if (ring == 1) at += 2;
+      if (ring == 1) { at += 2; r_at += 2; }
       keep(g & 1);
       for (int k = 0; k < nb; ++k, ++g) {
         const int j = w.begin() + k, row0 = first_row;
@@ -456,7 +470,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
           // `tiles` tiles of each box from column tile `from` on, as tiles t .. of a part of `all` tiles
           auto load = [&](uint32_t dst, uint64_t* bar, int from, int tiles, int t, int all) {
             const uint32_t box_bytes = p.tile_bytes == 1024 ? all * 1024 : p.box * 128;
-            const CUtensorMap* map = tiles == 1 ? &maps.one : tiles == 4 ? &maps.four : &maps.five;
+            const CUtensorMap* map = tiles == 1 ? &maps.one : tiles == 2 ? &maps.two : &maps.four;
             dst += t * p.tile_bytes;
             int row = row0;
             for (int e = 0; e < boxes; ++e, dst += box_bytes) {
@@ -471,17 +485,24 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             else for (int c = 0; c < tiles; ++c) load(sm100::smem_u32(dst), bar, from + c, 1, t + c, all);
           };
           if (ring == 0) {
-            const uint32_t s = g % kNSlots, use = g / kNSlots;
-            ok = use == 0 || sm100::mbar_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
-            if (ok) {
-              uint8_t* dst = n_ring + s * kNTiles * kTile;
+            for (int u = 0; u < kNUnits && ok; ++u) {
+              const uint32_t s = (at + u) % kNSlots, use = (at + u) / kNSlots;
+              ok = use == 0 || sm100::mbar_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
+              if (!ok) break;
               sm100::mbar_arrive_expect_tx(&ctl.n_full[s], kNTiles * bytes);
-              if (half == 0) part(dst, &ctl.n_full[s], 4, 5, 0, kNTiles);
-              else { part(dst, &ctl.n_full[s], 0, 4, 0, kNTiles); part(dst, &ctl.n_full[s], 8, 1, 4, kNTiles); }
+              part(n_ring + s * kNTiles * kTile, &ctl.n_full[s], other + u * kNTiles, kNTiles, 0, kNTiles);
             }
           } else {
+            {
+              const uint32_t s = r_at % kRSlots, use = r_at / kRSlots;
+              ok = use == 0 || sm100::mbar_wait(&ctl.r_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
+              if (ok) {
+                sm100::mbar_arrive_expect_tx(&ctl.r_full[s], bytes);
+                part(r_ring + s * kTile, &ctl.r_full[s], 8, 1, 0, 1);
+              }
+            }
             const uint32_t s = at % kVSlots, use = at / kVSlots;
-            ok = use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
+            ok = ok && (use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree));
             if (ok) {
               // a last block that the sequence does not fill goes to the clearing warp first
               const bool last = left < kKeys;
@@ -495,7 +516,8 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        ++at;
+        at += ring == 0 ? kNUnits : 1;
+        r_at += ring;
         if (k + 1 < nb) keep((g + 1) & 1);
       }
     }
@@ -503,19 +525,21 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     // round of the slots is waited for (a slot of which nothing is missing answers at once, or the limit ends it).
     if (__any_sync(0xffffffffu, !ok) && elect_one()) {
       int never = 0;
-      const long long limit = 20000000LL;
+      // the last `slots` uses before `end` of a ring
+      auto drain = [&](uint64_t* bars, uint32_t slots, uint32_t end) {
+        for (uint32_t i = end > slots ? end - slots : 0; i < end; ++i)
+          sm100::mbar_wait_limited(bars + i % slots, (i / slots) & 1, &never, nullptr, kWaitQ, 20000000LL);
+      };
       if (ring == 0) {
-        for (uint32_t i = g + 1 > kNSlots ? g + 1 - kNSlots : 0; i < g + 1; ++i)
-          sm100::mbar_wait_limited(&ctl.n_full[i % kNSlots], (i / kNSlots) & 1, &never, nullptr, kWaitDrain, limit);
+        drain(ctl.n_full, kNSlots, at + kNUnits);
+        if (seg > 0) drain(&ctl.q_full, 1, seg);
       } else {
-        const uint32_t end = at + 2;
-        for (uint32_t i = end > kVSlots ? end - kVSlots : 0; i < end; ++i)
-          sm100::mbar_wait_limited(&ctl.v_full[i % kVSlots], (i / kVSlots) & 1, &never, nullptr, kWaitDrain, limit);
-      }
+        drain(ctl.v_full, kVSlots, at + 2);
+        drain(ctl.r_full, kRSlots, r_at + 2);
 #pragma unroll
-      for (int e = 0; e < kVSlots; ++e)
-        if (landed[e]) sm100::mbar_wait_limited(&ctl.v_land[e], (landed[e] - 1) & 1, &never, nullptr, kWaitDrain, limit);
-      if (ring == 0 && seg > 0) sm100::mbar_wait_limited(&ctl.q_full, (seg - 1) & 1, &never, nullptr, kWaitDrain, limit);
+        for (int e = 0; e < kVSlots; ++e)
+          if (landed[e]) drain(&ctl.v_land[e], 1, landed[e]);
+      }
     }
     __syncwarp();
   } else if (warp == 6) {
@@ -555,10 +579,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       const bool by_rows = p.tile_bytes == 1024;
       const uint64_t q_desc = desc_sw128(sm100::smem_u32(q_smem), 16, 1024);
       const uint64_t n_desc = desc_sw128(sm100::smem_u32(n_ring), 16, by_rows ? kNTiles * 1024 : 1024);
+      const uint64_t r_desc = desc_sw128(sm100::smem_u32(r_ring), 16, 1024);
       const uint32_t v_group = by_rows ? kVTiles * 1024 : 1024, tile = p.tile_bytes >> 4;
       const uint64_t vk_desc = desc_sw128(sm100::smem_u32(v_ring), 16, v_group);
       const uint64_t vn_desc = desc_sw128(sm100::smem_u32(v_ring), p.tile_bytes, v_group);
-      uint32_t v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
+      uint32_t n_at = 0, r_at = 0, v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
       bool ok = true;
       for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
         const int nb = w.blocks();
@@ -567,36 +592,37 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             !sm100::mbar_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ))
           break;
         ++seg;
-        for (int h = 0; h < 2; ++h, ++v_qk, ++v_pv) sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);   // Q's two slots: read
+        for (int h = 0; h < 2; ++h, ++v_qk, ++v_pv, ++r_at) {    // the slots that Q came through were read
+          sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);
+          sm100::mbar_arrive(&ctl.r_empty[r_at % kRSlots]);
+        }
         sm100::tc_fence_after_sync();
         for (int k = 0; k <= nb; ++k) {
-          const uint32_t d = tmem + kColS + (g_qk & 1) * kKeys;
-          if (k < nb) {                        // S = Q . K^T of block k over 320 columns
-            const uint32_t s = g_qk % kNSlots;
-            if (!sm100::mbar_wait(&ctl.n_full[s], (g_qk / kNSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
-            const uint64_t b = n_desc + s * kNTiles * (kTile >> 4);
-#pragma unroll
-            for (int c = 0; c < kNTiles; ++c)
-#pragma unroll
-              for (int k4 = 0; k4 < 4; ++k4)
-                sm100::umma_f16(d, q_desc + c * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk, (c > 0 || k4 > 0) ? 1u : 0u);
-            sm100::umma_commit(&ctl.n_empty[s]);
-          }
-          if (k > 0) {                         // O += P . V of block k - 1
-            const uint32_t sb = g_pv & 1, s = v_pv % kVSlots;
-            if (!sm100::mbar_wait(&ctl.p_full[sb], (g_pv >> 1) & 1, abort_flag, p.status, kWaitP)) { ok = false; break; }
+          if (k < nb) {                        // S = Q . K^T of block k
+            if (g_qk > 0 && !sm100::mbar_wait(&ctl.s_read, (g_qk - 1) & 1, abort_flag, p.status, kWaitRead)) { ok = false; break; }
             sm100::tc_fence_after_sync();
-            const uint64_t b = vn_desc + s * kVTiles * (kTile >> 4);
+            const uint32_t d = tmem + kColS;
 #pragma unroll
-            for (int k4 = 0; k4 < kKeys / 16; ++k4)
-              umma_ts(tmem + kColO, tmem + kColS + sb * kKeys + k4 * 8, b + k4 * (v_group >> 3), idesc_pv,
-                      (k > 1 || k4 > 0) ? 1u : 0u);
-            sm100::umma_commit(&ctl.v_empty[s]);
-            sm100::umma_commit(&ctl.pv_done[sb]);
-            ++g_pv;
-            ++v_pv;
-          }
-          if (k < nb) {                        // S += Q . K^T of block k over this CTA's value columns
+            for (int u = 0; u < kNUnits; ++u, ++n_at) {
+              const uint32_t s = n_at % kNSlots;
+              if (!sm100::mbar_wait(&ctl.n_full[s], (n_at / kNSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
+              const uint64_t b = n_desc + s * kNTiles * (kTile >> 4);
+#pragma unroll
+              for (int c = 0; c < kNTiles; ++c)
+#pragma unroll
+                for (int k4 = 0; k4 < 4; ++k4)
+                  sm100::umma_f16(d, q_desc + (u * kNTiles + c) * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk,
+                                  (u > 0 || c > 0 || k4 > 0) ? 1u : 0u);
+              sm100::umma_commit(&ctl.n_empty[s]);
+            }
+            if (!ok) break;
+            const uint32_t sr = r_at % kRSlots;
+            if (!sm100::mbar_wait(&ctl.r_full[sr], (r_at / kRSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4)
+              umma_ts(d, tmem + kColQ + kVTiles * 32 + k4 * 8, r_desc + sr * (kTile >> 4) + 2 * k4, idesc_qk, 1u);
+            sm100::umma_commit(&ctl.r_empty[sr]);
+            ++r_at;
             const uint32_t s = v_qk % kVSlots;
             if (!sm100::mbar_wait(&ctl.v_full[s], (v_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
 #pragma unroll
@@ -605,10 +631,23 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 #pragma unroll
               for (int k4 = 0; k4 < 4; ++k4) umma_ts(d, tmem + kColQ + c * 32 + k4 * 8, b + 2 * k4, idesc_qk, 1u);
             }
-            sm100::umma_commit(&ctl.s_full[g_qk & 1]);
+            sm100::umma_commit(&ctl.s_full);
             if (k + 1 == nb) sm100::umma_commit(&ctl.q_free);
             ++g_qk;
             ++v_qk;
+          }
+          if (k > 0) {                         // O += P . V of block k - 1
+            const uint32_t s = v_pv % kVSlots;
+            if (!sm100::mbar_wait(&ctl.p_full, g_pv & 1, abort_flag, p.status, kWaitP)) { ok = false; break; }
+            sm100::tc_fence_after_sync();
+            const uint64_t b = vn_desc + s * kVTiles * (kTile >> 4);
+#pragma unroll
+            for (int k4 = 0; k4 < kKeys / 16; ++k4)
+              umma_ts(tmem + kColO, tmem + kColP + k4 * 8, b + k4 * (v_group >> 3), idesc_pv, (k > 1 || k4 > 0) ? 1u : 0u);
+            sm100::umma_commit(&ctl.v_empty[s]);
+            sm100::umma_commit(&ctl.pv_done);
+            ++g_pv;
+            ++v_pv;
           }
         }
       }
@@ -618,27 +657,31 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     // ---------------------------------------------------------------- softmax, one row per thread
     const int row = threadIdx.x;
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    uint32_t g = 0, v_at = 0;                  // blocks and value slots so far
+    uint32_t g = 0, v_at = 0, r_at = 0;        // blocks, value slots and rotary slots so far
     bool ok = true;
     const int own = half * kHalf;
-    // This half's columns of Q: from two slots of the value ring (two tiles of 64 columns, 128 rows each) to tensor
-    // memory, a row per thread.
+    // Columns of Q to tensor memory, a row per thread: this half's from two slots of the value ring (two tiles of 64
+    // columns, 128 rows each), the rotary ones from two slots of their ring (64 rows each).
+    auto take_tile = [&](const uint8_t* src, int r, int c) {
+      uint32_t u[32];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src + r * 128 + ((v ^ (r & 7)) << 4));
+        u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
+      }
+      tmem_st_32x32(lanes + kColQ + c * 32, u);
+    };
     auto take_q = [&]() {
       for (int h = 0; h < 2; ++h, ++v_at) {
         const uint32_t s = v_at % kVSlots;
         if (!warp_wait(&ctl.v_full[s], (v_at / kVSlots) & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          const uint8_t* src = v_ring + s * kVTiles * kTile + c * kQChunk + row * 128;
-          uint32_t u[32];
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            const uint4 x = *reinterpret_cast<const uint4*>(src + ((v ^ (row & 7)) << 4));
-            u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
-          }
-          tmem_st_32x32(lanes + kColQ + (2 * h + c) * 32, u);
-        }
+        for (int c = 0; c < 2; ++c) take_tile(v_ring + s * kVTiles * kTile + c * kQChunk, row, 2 * h + c);
       }
+      const uint32_t at = r_at + (warp >> 1), s = at % kRSlots;
+      if (!warp_wait(&ctl.r_full[s], (at / kRSlots) & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
+      take_tile(r_ring + s * kTile, row & 63, kVTiles);
+      r_at += 2;
       tmem_st_wait();
       sm100::tc_fence_before_sync();
       __syncwarp();
@@ -658,14 +701,20 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       const bool warp_live = warp * 32 < w.t.rows;
       float m_ref = -INFINITY, l_sum = 0.f;
       for (int k = 0; k < nb; ++k, ++g) {
-        const uint32_t sb = g & 1;
-        if (!warp_wait(&ctl.s_full[sb], (g >> 1) & 1, abort_flag, p.status, kWaitS)) { ok = false; break; }
+        if (!warp_wait(&ctl.s_full, g & 1, abort_flag, p.status, kWaitS)) { ok = false; break; }
         sm100::tc_fence_after_sync();
+        uint32_t u0[32], u1[32];
         if (warp_live) {
-          uint32_t u0[32], u1[32];
-          sm100::tmem_ld_32x32(lanes + kColS + sb * kKeys, u0);
-          sm100::tmem_ld_32x32(lanes + kColS + sb * kKeys + 32, u1);
+          sm100::tmem_ld_32x32(lanes + kColS, u0);
+          sm100::tmem_ld_32x32(lanes + kColS + 32, u1);
           sm100::tmem_ld_wait();
+        }
+        sm100::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&ctl.s_read);        // the next block's scores may overwrite them
+        uint32_t pk[32];
+        float factor = 1.f;
+        if (warp_live) {
           const int key0 = (w.begin() + k) * kKeys;
           if (!__all_sync(0xffffffffu, lo <= key0 && key0 + kKeys <= hi)) {
             const unsigned a = (unsigned)(key0 - lo), span = hi > lo ? (unsigned)(hi - lo) : 0u;
@@ -682,7 +731,6 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             m1 = fmaxf(m1, __uint_as_float(u1[i]));
           }
           const float m_blk = fmaxf(m0, m1) * p.scale_log2;      // scale > 0: the maximum commutes with it
-          float factor = 1.f;
           if (m_blk > -INFINITY) {
             if (m_ref == -INFINITY) {
               m_ref = m_blk;                   // O is zero or not begun: nothing to rescale
@@ -692,7 +740,6 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             }
           }
           const float neg = m_ref == -INFINITY ? 0.f : -m_ref;   // masked scores: exp2(-inf) = 0
-          uint32_t pk[32];
           float s0 = 0.f, s1 = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -708,10 +755,13 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             pk[16 + (i >> 1)] = pack2<T>(c, d);
           }
           l_sum = l_sum * factor + (s0 + s1);
-          if (__any_sync(0xffffffffu, factor != 1.f)) {
-            // only from the second block of a segment on: O holds the blocks up to k - 1
-            if (!warp_wait(&ctl.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
-            sm100::tc_fence_after_sync();
+        }
+        // P of the block before, and O, are free when its P.V is done (which it mostly is: it follows the scores). Warps
+        // without rows wait as well: an arrival on p_full must not come before the last one was taken.
+        if (k > 0 && !warp_wait(&ctl.pv_done, (g - 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
+        if (warp_live) {
+          sm100::tc_fence_after_sync();
+          if (__any_sync(0xffffffffu, factor != 1.f)) {        // only from the second block of a segment on
 #pragma unroll 1
             for (int c = 0; c < kHalf; c += 32) {
               uint32_t o[32];
@@ -722,22 +772,23 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
               tmem_st_32x32(lanes + kColO + c, o);
             }
           }
-          tmem_st_32x32(lanes + kColS + sb * kKeys, pk);
+          tmem_st_32x32(lanes + kColP, pk);
           tmem_st_wait();
         }
         sm100::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&ctl.p_full[sb]);
+        if (lane == 0) sm100::mbar_arrive(&ctl.p_full);
       }
       if (!ok) break;
       // Q of the next tile may go in as soon as the last scores are out
       Walk nx = w;
       nx.next(p);
       v_at += nb;
+      r_at += nb;
       if (nx.live() && nx.blocks() > 0) take_q();
       if (!ok) break;
       if (nb > 0) {
-        if (!warp_wait(&ctl.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
+        if (!warp_wait(&ctl.pv_done, (g - 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
         sm100::tc_fence_after_sync();
       }
       if (warp_live) {
@@ -931,8 +982,9 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
     return encode(map, type, 4, batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
-  if (!make(&maps.one, 1) || !make(&maps.four, 4) || !make(&maps.five, 5)) return CAB_ERR_BAD_ARGUMENT;
+  if (!make(&maps.one, 1) || !make(&maps.two, 2) || !make(&maps.four, 4)) return CAB_ERR_BAD_ARGUMENT;
   if (!sm100::make_tmap_2d_sw128(&maps.q, q, type, 2, (uint64_t)T * H, kD, kRows, 64) ||
+      !sm100::make_tmap_2d_sw128(&maps.q64, q, type, 2, (uint64_t)T * H, kD, 64, 64) ||
       !sm100::make_tmap_2d_sw128(&maps.q16, q, type, 2, (uint64_t)T * H, kD, kQBox, 64))
     return CAB_ERR_BAD_ARGUMENT;
   if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
