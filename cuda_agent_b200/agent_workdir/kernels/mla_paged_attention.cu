@@ -22,7 +22,8 @@
 //              page. Q comes the same way, its tensor-memory part through two slots of either of the latter rings
 //   warp 6     clears the rows behind a sequence's end in its last block of V
 // Whoever issues tensor or TMA instructions does so in one elected thread, waits included: the operands then sit
-// in uniform registers, and a wait polled by 32 lanes costs some 300 clk more than one polled by a single lane.
+// in uniform registers, and a wait polled by 32 lanes costs some 300 clk more than one polled by a single lane. A
+// TMA instruction takes its thread 65 clk, whatever its box.
 // The work of a call (tiles x blocks of 64 rows) is cut into equal runs, one for each pair of CTAs, wherever
 // that cuts a tile; each CTA finds its run itself from q_start and kv_len. Tiles cut by a boundary leave
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
@@ -57,7 +58,7 @@ struct __align__(16) Control {
   long long scan[kThreads / 32], total;
   long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
   int seq, tile;                               // its first tile
-  int pages[2][2][kKeys];                      // [ring][block parity]: the pages of a block's boxes
+  alignas(16) int pages[2][2][kKeys];          // [producer][block parity]: the pages of a block's boxes
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -88,23 +89,26 @@ struct Params {
   int* status;
 };
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1)
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // Issued where it stands, so that the load is under way while other work is done.
 __device__ __forceinline__ int load_now(const int* p) {
   int v;
   asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -365,6 +369,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   sm100::tc_fence_before_sync();
   __syncthreads();
   sm100::tc_fence_after_sync();
+  cudaTriggerProgrammaticLaunchCompletion();   // the merge kernel may be set up; it reads nothing before this grid's end
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);
   volatile int* abort_flag = &ctl.abort_flag;
   constexpr uint32_t kFmt = std::is_same_v<T, __half> ? 0 : 1;
@@ -376,20 +381,22 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     uint32_t at = 0, r_at = 0, g = 0, seg = 0; // slots of ring 0 or of V (with Q), of the rotary ring, blocks, segments
     uint32_t landed[kVSlots] = {};
     bool ok = true;
+    const uint32_t n_base = sm100::smem_u32(n_ring), r_base = sm100::smem_u32(r_ring), v_base = sm100::smem_u32(v_ring);
     // This lane's boxes in a block (two when a box is a single row): pages and rows from the block's first row on.
-    int box_pages[2], box_rows[2], page[2], first_page = 0, first_row = 0;
+    int box_pages[2], box_rows[2], next[2], first_page = 0, first_row = 0;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const unsigned off = (unsigned)(lane + 32 * k) << p.box_log2;
       box_pages[k] = off / (unsigned)p.page_size;
       box_rows[k] = off % (unsigned)p.page_size;
     }
-    auto look = [&](const Walk& w, int j) {
+    auto look = [&](const Walk& w, int j) {    // asks for the pages of block j
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int off = (lane + 32 * k) << p.box_log2;
         const int at = first_page + box_pages[k] + (first_row + box_rows[k] >= p.page_size);
-        page[k] = off < kKeys && j * kKeys + off < w.s.len ? load_now(p.page_table + (size_t)w.b * p.max_pages + at) : 0;
+        if (off < kKeys && j * kKeys + off < w.s.len) next[k] = load_now(p.page_table + (size_t)w.b * p.max_pages + at);
+        else next[k] = 0;
       }
     };
     auto step = [&]() {                        // to the next block
@@ -397,17 +404,21 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       first_row += p.step_rows;
       if (first_row >= p.page_size) { first_row -= p.page_size; ++first_page; }
     };
-    auto keep = [&](int parity) {              // one outside the pool: TMA fills with zeros
+    auto keep = [&](uint32_t parity) {         // one outside the pool: TMA fills with zeros
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if ((unsigned)page[k] >= (unsigned)p.num_pages) {
+        if ((unsigned)next[k] >= (unsigned)p.num_pages) {
           if (p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
-          page[k] = p.num_pages;
+          next[k] = p.num_pages;
         }
-        if (k == 0 || p.box == 1) ctl.pages[ring][parity][lane + 32 * k] = page[k];
+        if (k == 0 || p.box == 1) ctl.pages[ring][parity][lane + 32 * k] = next[k];
       }
       __syncwarp();
+    };
+    // a slot of a ring, free again for its use number `at`
+    auto room = [&](uint64_t* empty, uint32_t slots, uint32_t at) {
+      return at < slots || sm100::mbar_wait(empty + at % slots, (at / slots - 1) & 1, abort_flag, p.status, kWaitNFree);
     };
     for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
       const int nb = w.blocks();
@@ -416,41 +427,34 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       first_row = (unsigned)(w.begin() * kKeys) % (unsigned)p.page_size;
       look(w, w.begin());
       if (elect_one()) {                       // Q of this tile
-        const int boxes = w.t.rows > 4 * kQBox ? 1 : (w.t.rows + kQBox - 1) / kQBox, rows = w.t.rows > 4 * kQBox ? kRows : kQBox;
-        const CUtensorMap* m = w.t.rows > 4 * kQBox ? &maps.q : &maps.q16;
-        auto chunk = [&](uint8_t* dst, uint64_t* bar, int col) {
-          for (int e = 0; e < boxes; ++e)
-            tma_load_2d(sm100::smem_u32(dst) + e * rows * 128, m, bar, col, w.t.row0 + e * rows);
+        const bool many = w.t.rows > 4 * kQBox;
+        const int boxes = many ? 1 : (w.t.rows + kQBox - 1) / kQBox, rows = many ? kRows : kQBox;
+        auto chunk = [&](uint32_t dst, uint32_t bar, int col) {
+          if (many) tma_load_2d(dst, &maps.q, bar, col, w.t.row0);
+          else for (int e = 0; e < boxes; ++e) tma_load_2d(dst + e * rows * 128, &maps.q16, bar, col, w.t.row0 + e * rows);
         };
         if (ring == 0) {
           ok = seg == 0 || sm100::mbar_wait(&ctl.q_free, (seg - 1) & 1, abort_flag, p.status, kWaitQ);
           if (ok) {
-            sm100::mbar_arrive_expect_tx(&ctl.q_full, kQTiles * boxes * rows * 128);
-            for (int c = 0; c < kQTiles; ++c) chunk(q_smem + c * kQChunk, &ctl.q_full, 64 * (other + c));
+            const uint32_t bar = sm100::smem_u32(&ctl.q_full);
+            expect_bytes(bar, kQTiles * boxes * rows * 128);
+            for (int c = 0; c < kQTiles; ++c) chunk(sm100::smem_u32(q_smem) + c * kQChunk, bar, 64 * (other + c));
           }
         } else {
           for (int h = 0; h < 2 && ok; ++h) {  // two tiles of this half's columns
-            const uint32_t s = (at + h) % kVSlots, use = (at + h) / kVSlots;
-            ok = use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
+            ok = room(ctl.v_empty, kVSlots, at + h);
             if (!ok) break;
-            sm100::mbar_arrive_expect_tx(&ctl.v_full[s], 2 * boxes * rows * 128);
-            for (int c = 0; c < 2; ++c)
-              chunk(v_ring + s * kVTiles * kTile + c * kQChunk, &ctl.v_full[s], 64 * (4 - other + 2 * h + c));
+            const uint32_t s = (at + h) % kVSlots, bar = sm100::smem_u32(&ctl.v_full[s]);
+            expect_bytes(bar, 2 * boxes * rows * 128);
+            for (int c = 0; c < 2; ++c) chunk(v_base + s * kVTiles * kTile + c * kQChunk, bar, 64 * (4 - other + 2 * h + c));
           }
           for (int h = 0; h < 2 && ok; ++h) {  // 64 rows of the rotary columns
-            const uint32_t s = (r_at + h) % kRSlots, use = (r_at + h) / kRSlots;
-            ok = use == 0 || sm100::mbar_wait(&ctl.r_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree);
+            ok = room(ctl.r_empty, kRSlots, r_at + h);
             if (!ok) break;
-            uint8_t* dst = r_ring + s * kTile;
-            if (rows == kRows) {
-              sm100::mbar_arrive_expect_tx(&ctl.r_full[s], kTile);
-              tma_load_2d(sm100::smem_u32(dst), &maps.q64, &ctl.r_full[s], kDv, w.t.row0 + 64 * h);
-            } else if (h == 0) {
-              sm100::mbar_arrive_expect_tx(&ctl.r_full[s], boxes * rows * 128);
-              chunk(dst, &ctl.r_full[s], kDv);
-            } else {
-              sm100::mbar_arrive(&ctl.r_full[s]);
-            }
+            const uint32_t s = (r_at + h) % kRSlots, bar = sm100::smem_u32(&ctl.r_full[s]);
+            expect_bytes(bar, many ? kTile : h == 0 ? boxes * rows * 128 : 0);
+            if (many) tma_load_2d(r_base + s * kTile, &maps.q64, bar, kDv, w.t.row0 + 64 * h);
+            else if (h == 0) chunk(r_base + s * kTile, bar, kDv);
           }
         }
       }
@@ -467,50 +471,59 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
           const int left = w.s.len - j * kKeys;
           const int boxes = (min(kKeys, left) + p.box - 1) >> p.box_log2, bytes = boxes * p.box * 128;
           const int* list = ctl.pages[ring][g & 1];
-          // `tiles` tiles of each box from column tile `from` on, as tiles t .. of a part of `all` tiles
-          auto load = [&](uint32_t dst, uint64_t* bar, int from, int tiles, int t, int all) {
-            const uint32_t box_bytes = p.tile_bytes == 1024 ? all * 1024 : p.box * 128;
-            const CUtensorMap* map = tiles == 1 ? &maps.one : tiles == 2 ? &maps.two : &maps.four;
-            dst += t * p.tile_bytes;
-            int row = row0;
-            for (int e = 0; e < boxes; ++e, dst += box_bytes) {
-              tma_load_4d(dst, map, bar, 0, row, from, list[e]);
-              row += p.box;
-              if (row == p.page_size) row = 0;
-            }
-          };
-          const bool joint = p.box >= 8;       // boxes of several tiles keep the eight-row groups that swizzling wants
-          auto part = [&](uint8_t* dst, uint64_t* bar, int from, int tiles, int t, int all) {
-            if (joint) load(sm100::smem_u32(dst), bar, from, tiles, t, all);
-            else for (int c = 0; c < tiles; ++c) load(sm100::smem_u32(dst), bar, from + c, 1, t + c, all);
-          };
-          if (ring == 0) {
-            for (int u = 0; u < kNUnits && ok; ++u) {
-              const uint32_t s = (at + u) % kNSlots, use = (at + u) / kNSlots;
-              ok = use == 0 || sm100::mbar_wait(&ctl.n_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
-              if (!ok) break;
-              sm100::mbar_arrive_expect_tx(&ctl.n_full[s], kNTiles * bytes);
-              part(n_ring + s * kNTiles * kTile, &ctl.n_full[s], other + u * kNTiles, kNTiles, 0, kNTiles);
-            }
-          } else {
-            {
-              const uint32_t s = r_at % kRSlots, use = r_at / kRSlots;
-              ok = use == 0 || sm100::mbar_wait(&ctl.r_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitNFree);
-              if (ok) {
-                sm100::mbar_arrive_expect_tx(&ctl.r_full[s], bytes);
-                part(r_ring + s * kTile, &ctl.r_full[s], 8, 1, 0, 1);
+          // page and row of up to eight boxes of eight rows, or of the one box of 64
+          int pg[8], rw[8];
+          if (p.box >= 8) {
+            const int4 a = *reinterpret_cast<const int4*>(list), b = *reinterpret_cast<const int4*>(list + 4);
+            pg[0] = a.x; pg[1] = a.y; pg[2] = a.z; pg[3] = a.w; pg[4] = b.x; pg[5] = b.y; pg[6] = b.z; pg[7] = b.w;
+            rw[0] = row0;
+#pragma unroll
+            for (int e = 1; e < 8; ++e) rw[e] = rw[e - 1] + 8 == p.page_size ? 0 : rw[e - 1] + 8;
+          }
+          // `tiles` tiles of each box from column tile `from` on
+          auto part = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int from, int tiles) {
+            if (p.box == kKeys) {
+              tma_load_4d(dst, map, bar, 0, rw[0], from, pg[0]);
+            } else if (p.box == 8) {           // boxes of several tiles keep the eight-row groups that swizzling wants
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (e < boxes) tma_load_4d(dst + e * tiles * 1024, map, bar, 0, rw[e], from, pg[e]);
+            } else {
+              for (int c = 0; c < tiles; ++c) {
+                int row = row0;
+                for (int e = 0; e < boxes; ++e) {
+                  tma_load_4d(dst + c * kTile + e * p.box * 128, &maps.one, bar, 0, row, from + c, list[e]);
+                  row += p.box;
+                  if (row == p.page_size) row = 0;
+                }
               }
             }
-            const uint32_t s = at % kVSlots, use = at / kVSlots;
-            ok = ok && (use == 0 || sm100::mbar_wait(&ctl.v_empty[s], (use - 1) & 1, abort_flag, p.status, kWaitVFree));
+          };
+          if (ring == 0) {
+            for (int u = 0; u < kNUnits; ++u) {
+              ok = room(ctl.n_empty, kNSlots, at + u);
+              if (!ok) break;
+              const uint32_t s = (at + u) % kNSlots, bar = sm100::smem_u32(&ctl.n_full[s]);
+              expect_bytes(bar, kNTiles * bytes);
+              part(n_base + s * kNTiles * kTile, &maps.two, bar, other + u * kNTiles, kNTiles);
+            }
+          } else {
+            ok = room(ctl.r_empty, kRSlots, r_at);
             if (ok) {
+              const uint32_t s = r_at % kRSlots, bar = sm100::smem_u32(&ctl.r_full[s]);
+              expect_bytes(bar, bytes);
+              part(r_base + s * kTile, &maps.one, bar, 8, 1);
+              ok = room(ctl.v_empty, kVSlots, at);
+            }
+            if (ok) {
+              const uint32_t s = at % kVSlots;
               // a last block that the sequence does not fill goes to the clearing warp first
               const bool last = left < kKeys;
-              uint64_t* land = last ? &ctl.v_land[s] : &ctl.v_full[s];
+              const uint32_t bar = sm100::smem_u32(last ? &ctl.v_land[s] : &ctl.v_full[s]);
 #pragma unroll
               for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
-              sm100::mbar_arrive_expect_tx(land, kVTiles * bytes);
-              part(v_ring + s * kVTiles * kTile, land, 4 - other, kVTiles, 0, kVTiles);
+              expect_bytes(bar, kVTiles * bytes);
+              part(v_base + s * kVTiles * kTile, &maps.four, bar, 4 - other, kVTiles);
             }
           }
         }
@@ -521,9 +534,9 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         if (k + 1 < nb) keep((g + 1) & 1);
       }
     }
-    // Giving up: nothing that is on its way may land after the CTA has ended. What was asked for in the last
-    // round of the slots is waited for (a slot of which nothing is missing answers at once, or the limit ends it).
-    if (__any_sync(0xffffffffu, !ok) && elect_one()) {
+    // Giving up: nothing that is on its way may land after the CTA has ended. The last use of every slot is waited
+    // for, with a limit.
+    if (!ok && elect_one()) {                  // counted: what was asked for, and up to a block more
       int never = 0;
       // the last `slots` uses before `end` of a ring
       auto drain = [&](uint64_t* bars, uint32_t slots, uint32_t end) {
@@ -854,31 +867,45 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   }
 }
 
-// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own maximum m_k.
-// One CTA per row, four columns per thread; parts in the order of the pairs.
+// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own maximum m_k. 128
+// threads per row, four columns each; the parts' maxima and sums are read side by side, their columns eight at a
+// time, and added in the order of the pairs.
+constexpr int kMergeRows = 4;
 template <typename T>
-__global__ void __launch_bounds__(128) mla_paged_merge_kernel(const Params p) {
-  const int pair = blockIdx.x, row = blockIdx.y;
+__global__ void __launch_bounds__(128 * kMergeRows) mla_paged_merge_kernel(const Params p) {
+  __shared__ float2 s_ml[kMergeRows][2][cab::kNumSMs / 2];
+  cudaGridDependencySynchronize();
+  const int pair = blockIdx.x, sub = threadIdx.x >> 7, tid = threadIdx.x & 127;
   const Meta m = p.meta[pair];
-  if (row >= m.rows) return;
-  const int col = threadIdx.x * 4, half = col >= kHalf;
-  auto slot_of = [&](int k) { return (size_t)k * 2 + (k == m.first ? 1 : 0); };
+  if ((int)blockIdx.y * kMergeRows >= m.rows) return;
+  const int row = blockIdx.y * kMergeRows + sub, parts = pair - m.first + 1;
+  const bool live = row < m.rows;
+  auto slot_of = [&](int k) { return (size_t)(m.first + k) * 2 + (k == 0 ? 1 : 0); };
+  if (live)
+    for (int e = tid; e < 2 * parts; e += 128)
+      s_ml[sub][e & 1][e >> 1] = *reinterpret_cast<const float2*>(p.part_ml + ((slot_of(e >> 1) * 2 + (e & 1)) * p.rows_cap + row) * 2);
+  __syncthreads();
+  if (!live) return;
+  const int col = tid * 4, half = col >= kHalf;
+  const float2* ml = s_ml[sub][half];
   float top = -INFINITY;
-  for (int k = m.first; k <= pair; ++k) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot_of(k) * 2 + half) * p.rows_cap + row) * 2);
-    if (ml.y != 0.f) top = fmaxf(top, ml.x);
-  }
+  for (int k = 0; k < parts; ++k)
+    if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-#pragma unroll 4
-  for (int k = m.first; k <= pair; ++k) {
-    const size_t slot = slot_of(k);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot * 2 + half) * p.rows_cap + row) * 2);
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (slot * p.rows_cap + row) * kDv + col);
-    const float f = ml.y != 0.f ? exp2_approx(ml.x - top) : 0.f;
-    if (f != 0.f) {                            // also true for NaN
-      acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
-      l += f * ml.y;
+  for (int k0 = 0; k0 < parts; k0 += 8) {
+    float4 o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k0 + e < parts) o[e] = __ldcs(reinterpret_cast<const float4*>(p.part_o + (slot_of(k0 + e) * p.rows_cap + row) * kDv + col));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (k0 + e >= parts) break;
+      const float f = ml[k0 + e].y != 0.f ? exp2_approx(ml[k0 + e].x - top) : 0.f;
+      if (f != 0.f) {                          // also true for NaN
+        acc.x += f * o[e].x; acc.y += f * o[e].y; acc.z += f * o[e].z; acc.w += f * o[e].w;
+        l += f * ml[k0 + e].y;
+      }
     }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
@@ -887,7 +914,7 @@ __global__ void __launch_bounds__(128) mla_paged_merge_kernel(const Params p) {
   r.x = zero ? 0u : pack2<T>(acc.x * inv, acc.y * inv);
   r.y = zero ? 0u : pack2<T>(acc.z * inv, acc.w * inv);
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)(m.row0 + row) * kDv + col) = r;
-  if (threadIdx.x == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
+  if (tid == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
 }
 
 constexpr int kPairs = cab::kNumSMs / 2;       // the workspace is sized for this many, a smaller device runs fewer
@@ -901,7 +928,17 @@ int launch(Params& p, const Maps& maps, cudaStream_t stream) {
   mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, maps);
   const int rc = cab::launch_status();
   if (rc != CAB_OK || p.pairs == 1) return rc;
-  mla_paged_merge_kernel<T><<<dim3(p.pairs, p.rows_cap), 128, 0, stream>>>(p);
+  // launched while the first kernel runs; it waits for that one's end itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows);
+  cfg.blockDim = dim3(128 * kMergeRows);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, mla_paged_merge_kernel<T>, static_cast<const Params>(p)) != cudaSuccess) return CAB_ERR_LAUNCH;
   return cab::launch_status();
 }
 

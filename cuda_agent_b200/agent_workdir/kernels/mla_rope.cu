@@ -5,7 +5,9 @@
 // sines and cosines of its tokens once, in shared memory, and uses them for all the heads it handles. The angle
 // is formed and reduced to a fraction of a turn in 64 bits (at position 10^6 a 32-bit product is off by 0.03
 // radian); sine and cosine of the fraction are 32-bit, as is the rotation; one rounding at the end.
-// Columns move in 16-byte pieces where pointers, strides and R allow it, else pair by pair.
+// Columns move in 16-byte pieces where pointers, strides and R allow it, else pair by pair. A thread keeps one place
+// in the row and steps through the rows of its CTA, so nothing is divided in the loop; its first rows are asked
+// for before the sines and cosines are made.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -23,6 +25,24 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two 16-bit values as one word: a conversion instruction rounds both.
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 __device__ __forceinline__ float2 turn_of(int position, double freq, float mscale, bool inverse) {
   const double t = (double)position * (freq * 0.15915494309189533577);   // turns
@@ -43,18 +63,42 @@ struct __align__(sizeof(T) * N) Vec { T v[N]; };
 // One unit of a head: with `interleaved` N consecutive columns (N / 2 pairs), else N columns of either half.
 template <typename T, int N, bool kInterleaved>
 struct Unit {
-  static constexpr int kVecs = kInterleaved ? 1 : 2;
+  static constexpr int kVecs = kInterleaved ? 1 : 2, kPairs = kInterleaved ? N / 2 : N;
+  struct alignas(kPairs % 2 ? 8 : 16) Angles { float2 v[kPairs]; };
   Vec<T, N> d[kVecs];
+  // `cs`: those of the token's first pair
+  static __device__ __forceinline__ Angles angles(const float2* cs, int unit) {
+    return *reinterpret_cast<const Angles*>(cs + unit * kPairs);
+  }
   __device__ __forceinline__ void load(const T* x, int unit, int half) {
     d[0] = *reinterpret_cast<const Vec<T, N>*>(x + unit * N);
     if constexpr (!kInterleaved) d[1] = *reinterpret_cast<const Vec<T, N>*>(x + half + unit * N);
   }
-  __device__ __forceinline__ void turn(const float2* cs, int unit) {
-    if constexpr (kInterleaved) {
+  __device__ __forceinline__ void turn(const Angles& cs) {
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&d[0]);
+      if constexpr (kInterleaved) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float2 x = unpack2<T>(w[i]);
+          rotate(x.x, x.y, cs.v[i]);
+          w[i] = pack2<T>(x.x, x.y);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float2 x = unpack2<T>(w[i]), y = unpack2<T>(w[N / 2 + i]);
+          rotate(x.x, y.x, cs.v[2 * i]);
+          rotate(x.y, y.y, cs.v[2 * i + 1]);
+          w[i] = pack2<T>(x.x, x.y);
+          w[N / 2 + i] = pack2<T>(y.x, y.y);
+        }
+      }
+    } else if constexpr (kInterleaved) {
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
         float a = to_f(d[0].v[2 * i]), b = to_f(d[0].v[2 * i + 1]);
-        rotate(a, b, cs[unit * (N / 2) + i]);
+        rotate(a, b, cs.v[i]);
         d[0].v[2 * i] = from_f<T>(a);
         d[0].v[2 * i + 1] = from_f<T>(b);
       }
@@ -62,7 +106,7 @@ struct Unit {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         float a = to_f(d[0].v[i]), b = to_f(d[kVecs - 1].v[i]);
-        rotate(a, b, cs[unit * N + i]);
+        rotate(a, b, cs.v[i]);
         d[0].v[i] = from_f<T>(a);
         d[kVecs - 1].v[i] = from_f<T>(b);
       }
@@ -86,44 +130,101 @@ struct RopeParams {
   int inverse;
 };
 
-// The units of `tokens` tokens x heads [h0, h1), four in flight per thread.
+// The rows (token, head) of a CTA, tokens x heads, of `units` units each: a thread takes the same unit of every
+// (kThreads / units)-th row, four rows at a time.
 template <typename T, int N, bool kInterleaved>
-__device__ __forceinline__ void rotate_heads(T* out, const T* x, const float2* cs, int tokens, int h0, int h1, int R,
-                                             long long xt, long long xh, long long ot, long long oh) {
-  const int half = R / 2, units = (kInterleaved ? R : half) / N, heads = h1 - h0;
-  const int total = tokens * heads * units;
-  for (int e0 = threadIdx.x; e0 < total; e0 += 4 * kThreads) {
-    Unit<T, N, kInterleaved> u[4];
-    int tok[4], head[4], unit[4];
+struct RowWalk {
+  static constexpr int kBatch = kInterleaved ? 4 : 2;            // 64 bytes of a wide walk in flight per thread
+  const T* x;
+  T* out;
+  int half, unit, tok, head, heads, left, step_tok, step_head;   // left: rows of this thread still to come
+  long long xo, oo, x_step, o_step, x_wrap, o_wrap;
+  Unit<T, N, kInterleaved> u[kBatch];
+  long long at[kBatch];
+  int cs_at[kBatch];
+
+  __device__ __forceinline__ RowWalk(T* out_, const T* x_, int tokens, int heads_, int R, long long xt, long long xh,
+                                     long long ot, long long oh)
+      : x(x_), out(out_), half(R / 2), heads(heads_) {
+    const int units = (kInterleaved ? R : half) / N;
+    // (rows of more units than threads: the kernel comes again for the other units)
+    const int step = units < kThreads ? kThreads / units : 1;
+    unit = units < kThreads ? threadIdx.x % units : threadIdx.x;
+    const int first = units < kThreads ? threadIdx.x / units : 0, rows = tokens * heads;
+    left = first < step && first < rows ? (rows - first + step - 1) / step : 0;
+    if (unit >= units) left = 0;
+    tok = first / heads;
+    head = first % heads;
+    step_tok = step / heads;
+    step_head = step % heads;
+    xo = tok * xt + head * xh;
+    oo = tok * ot + head * oh;
+    x_step = step_tok * xt + step_head * xh;
+    o_step = step_tok * ot + step_head * oh;
+    x_wrap = xt - heads * xh;
+    o_wrap = ot - heads * oh;
+  }
+  __device__ __forceinline__ void load() {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = e0 + k * kThreads;
-      if (e >= total) break;
-      unit[k] = e % units;
-      const int th = e / units;
-      tok[k] = th / heads;
-      head[k] = h0 + th % heads;
-      u[k].load(x + tok[k] * xt + head[k] * xh, unit[k], half);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (e0 + k * kThreads >= total) break;
-      u[k].turn(cs + tok[k] * half, unit[k]);
-      u[k].store(out + tok[k] * ot + head[k] * oh, unit[k], half);
+    for (int k = 0; k < kBatch; ++k) {
+      if (k < left) {
+        u[k].load(x + xo, unit, half);
+        at[k] = oo;
+        cs_at[k] = tok * half;
+      }
+      xo += x_step;
+      oo += o_step;
+      tok += step_tok;
+      head += step_head;
+      if (head >= heads) {
+        head -= heads;
+        ++tok;
+        xo += x_wrap;
+        oo += o_wrap;
+      }
     }
   }
-}
+  __device__ __forceinline__ void store(const float2* cs) {
+    // the rows of a batch are mostly one token's, which turns them alike
+    auto angles = Unit<T, N, kInterleaved>::angles(cs + cs_at[0], unit);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (k < left) {
+        if (k > 0 && cs_at[k] != cs_at[k - 1]) angles = Unit<T, N, kInterleaved>::angles(cs + cs_at[k], unit);
+        u[k].turn(angles);
+        u[k].store(out + at[k], unit, half);
+      }
+    left -= kBatch;
+  }
+  __device__ __forceinline__ void rest(const float2* cs) {       // after the first load()
+    while (left > 0) {
+      store(cs);
+      if (left > 0) load();
+    }
+  }
+};
 
 template <typename T, int N, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) mla_rope_kernel(const RopeParams p) {
-  __shared__ float2 cs[kAngles];
+__global__ void __launch_bounds__(kThreads, 4) mla_rope_kernel(const RopeParams p) {
+  __shared__ __align__(16) float2 cs[kAngles];
   const int t0 = blockIdx.x * p.tokens, tokens = min(p.tokens, p.T - t0), half = p.R / 2;
+  const int h0 = blockIdx.y * p.heads, h1 = min(p.H, h0 + p.heads);
+  T* out = static_cast<T*>(p.out) + t0 * p.ot + h0 * p.oh;
+  const T* x = static_cast<const T*>(p.x) + t0 * p.xt + h0 * p.xh;
+  RowWalk<T, N, kInterleaved> w(out, x, tokens, h1 - h0, p.R, p.xt, p.xh, p.ot, p.oh);
+  w.load();
   for (int e = threadIdx.x; e < tokens * half; e += kThreads)
     cs[e] = turn_of(__ldg(p.positions + t0 + e / half), __ldg(p.freq + e % half), p.mscale, p.inverse != 0);
   __syncthreads();
-  const int h0 = blockIdx.y * p.heads, h1 = min(p.H, h0 + p.heads);
-  rotate_heads<T, N, kInterleaved>(static_cast<T*>(p.out) + t0 * p.ot, static_cast<const T*>(p.x) + t0 * p.xt, cs, tokens,
-                                   h0, h1, p.R, p.xt, p.xh, p.ot, p.oh);
+  w.rest(cs);
+  // rows of more units than threads have: the others
+  for (int unit = threadIdx.x + kThreads; unit < (kInterleaved ? p.R : half) / N; unit += kThreads) {
+    RowWalk<T, N, kInterleaved> more(out, x, tokens, h1 - h0, p.R, p.xt, p.xh, p.ot, p.oh);
+    more.unit = unit;
+    more.left = tokens * (h1 - h0);
+    more.load();
+    more.rest(cs);
+  }
 }
 
 constexpr int kLatent = 512, kRot = 64;
@@ -141,16 +242,29 @@ struct AppendParams {
 
 // kVec: every row and stride allows 16-byte accesses. Head group 0 of a token also writes the token's cache row.
 template <typename T, bool kInterleaved, bool kVec>
-__global__ void __launch_bounds__(kThreads) mla_rope_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const AppendParams p) {
   constexpr int N = kVec ? 8 : (kInterleaved ? 2 : 1);
   constexpr int half = kRot / 2;
-  __shared__ float2 cs[kAngles];
+  __shared__ __align__(16) float2 cs[kAngles];
   __shared__ int s_pos[kAngles / half];
   __shared__ long long s_row[kAngles / half];  // where the cache row begins, -1: nowhere
   const int t0 = blockIdx.x * p.r.tokens;
   const int end = min(max(__ldg(p.q_start + p.batch), 0), p.r.T);     // tokens behind the last sequence stay as they are
   const int tokens = min(p.r.tokens, end - t0);
   if (tokens <= 0) return;
+  // what does not depend on the tables is asked for before they are read
+  const int h0 = blockIdx.y * p.r.heads, h1 = min(p.r.H, h0 + p.r.heads);
+  RowWalk<T, N, kInterleaved> w(static_cast<T*>(p.r.out) + t0 * p.r.ot + h0 * p.r.oh,
+                                static_cast<const T*>(p.r.x) + t0 * p.r.xt + h0 * p.r.xh, tokens, max(h1 - h0, 1), kRot,
+                                p.r.xt, p.r.xh, p.r.ot, p.r.oh);
+  if (h1 <= h0) w.left = 0;                    // no heads: only the cache is written
+  w.load();
+  constexpr int C = kVec ? 8 : 1;
+  const T* c = static_cast<const T*>(p.c_kv) + t0 * p.ct;
+  Vec<T, C> latent;
+  const bool copies = blockIdx.y == 0;
+  if (copies && threadIdx.x < tokens * (kLatent / C))
+    latent = *reinterpret_cast<const Vec<T, C>*>(c + threadIdx.x / (kLatent / C) * p.ct + threadIdx.x % (kLatent / C) * C);
   if (threadIdx.x < tokens) {
     const int t = t0 + threadIdx.x;
     int lo = 0, hi = p.batch;                  // last b with q_start[b] <= t
@@ -169,18 +283,16 @@ __global__ void __launch_bounds__(kThreads) mla_rope_append_kernel(const AppendP
   __syncthreads();
   for (int e = threadIdx.x; e < tokens * half; e += kThreads)
     cs[e] = turn_of(s_pos[e / half], __ldg(p.r.freq + e % half), p.r.mscale, false);
-  if (blockIdx.y == 0) {                       // the latent part of the rows: a copy
-    constexpr int C = kVec ? 8 : 1;
+  if (copies) {                                // the latent part of the rows: a copy
     T* rows = static_cast<T*>(p.rows);
-    const T* c = static_cast<const T*>(p.c_kv) + t0 * p.ct;
     for (int e = threadIdx.x; e < tokens * (kLatent / C); e += kThreads) {
       const int t = e / (kLatent / C), col = e % (kLatent / C) * C;
-      if (s_row[t] >= 0)
-        *reinterpret_cast<Vec<T, C>*>(rows + s_row[t] + col) = *reinterpret_cast<const Vec<T, C>*>(c + t * p.ct + col);
+      if (e != threadIdx.x) latent = *reinterpret_cast<const Vec<T, C>*>(c + t * p.ct + col);
+      if (s_row[t] >= 0) *reinterpret_cast<Vec<T, C>*>(rows + s_row[t] + col) = latent;
     }
   }
   __syncthreads();
-  if (blockIdx.y == 0) {
+  if (copies) {
     constexpr int units = (kInterleaved ? kRot : half) / N;
     const T* k = static_cast<const T*>(p.k_pe) + t0 * p.kt;
     for (int e = threadIdx.x; e < tokens * units; e += kThreads) {
@@ -188,21 +300,18 @@ __global__ void __launch_bounds__(kThreads) mla_rope_append_kernel(const AppendP
       if (s_row[t] < 0) continue;
       Unit<T, N, kInterleaved> u;
       u.load(k + t * p.kt, unit, half);
-      u.turn(cs + t * half, unit);
+      u.turn(Unit<T, N, kInterleaved>::angles(cs + t * half, unit));
       u.store(static_cast<T*>(p.rows) + s_row[t] + kLatent, unit, half);
     }
   }
-  const int h0 = blockIdx.y * p.r.heads, h1 = min(p.r.H, h0 + p.r.heads);
-  if (h0 < h1)
-    rotate_heads<T, N, kInterleaved>(static_cast<T*>(p.r.out) + t0 * p.r.ot, static_cast<const T*>(p.r.x) + t0 * p.r.xt, cs,
-                                     tokens, h0, h1, kRot, p.r.xt, p.r.xh, p.r.ot, p.r.oh);
+  w.rest(cs);
 }
 
-// Tokens and heads per CTA: about 2048 units (8 a thread), fewer where the call is too small to fill the device.
+// Tokens and heads per CTA: about 1024 units (four a thread), fewer where the call is too small to fill the device.
 void split(RopeParams& p, int units_per_head, dim3& grid) {
   const int half = p.R / 2;
   const long long per_token = (long long)(p.H > 0 ? p.H : 1) * units_per_head;
-  long long tokens = 2048 / per_token;
+  long long tokens = 4 * kThreads / per_token;
   const long long most = kAngles / half < 1 ? 1 : kAngles / half;
   if (tokens > most) tokens = most;
   const long long fill = ((long long)p.T + 4 * cab::kNumSMs - 1) / (4 * cab::kNumSMs);
@@ -217,7 +326,7 @@ void split(RopeParams& p, int units_per_head, dim3& grid) {
     if (smallest < 1) smallest = 1;
     heads = (heads + groups_wanted - 1) / groups_wanted;
     if (heads < smallest) heads = smallest;
-    long long largest = 4096 / units_per_head;
+    long long largest = 8 * kThreads / units_per_head;
     if (largest < 1) largest = 1;
     if (heads > largest) heads = largest;
   }
