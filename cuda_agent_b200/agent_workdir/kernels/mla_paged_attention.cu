@@ -23,7 +23,9 @@
 //   warp 6     clears the rows behind a sequence's end in its last block of V
 // Whoever issues tensor or TMA instructions does so in one elected thread, waits included: the operands then sit
 // in uniform registers, and a wait polled by 32 lanes costs some 300 clk more than one polled by a single lane. A
-// TMA instruction takes its thread 65 clk, whatever its box.
+// TMA instruction takes its thread 65 clk, whatever its box. A wait that is over already still costs 150 to 200 clk
+// while the tensor core keeps shared memory busy, so everything a block loads lands on one barrier: the issuing
+// thread waits three times a block (scores read, rows there, P there); with seven waits it was the bottleneck.
 // The work of a call (tiles x blocks of 64 rows) is cut into equal runs, one for each pair of CTAs, wherever
 // that cuts a tile; each CTA finds its run itself from q_start and kv_len. Tiles cut by a boundary leave
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
@@ -43,7 +45,7 @@ constexpr int kKeys = 64;                      // cache rows per block
 constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 128-byte swizzle
 // 64-column tiles of a block: units of the other value half, the rotary columns, own value half
 constexpr int kNTiles = 2, kNUnits = 2, kVTiles = 4, kQTiles = kNTiles * kNUnits;
-constexpr int kNSlots = 3, kRSlots = 2, kVSlots = 3;
+constexpr int kNSlots = 3, kRSlots = 2, kVSlots = 3, kAhead = 4;   // no ring reaches further than three blocks ahead
 constexpr int kQChunk = kRows * 128;
 constexpr int kThreads = 8 * 32;
 constexpr int kQBox = 16;                      // rows of the small box for Q
@@ -53,8 +55,10 @@ constexpr int kMaxBatch = 16384;
 enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitRead };
 
 struct __align__(16) Control {
-  uint64_t n_full[kNSlots], n_empty[kNSlots], r_full[kRSlots], r_empty[kRSlots], v_full[kVSlots], v_empty[kVSlots],
-      v_land[kVSlots], s_full, s_read, p_full, pv_done, q_ready, q_full, q_free;
+  // full: by block, the other half's rows, the rotary columns and this half's rows; q_full, q_part: Q's shared and its
+  // tensor-memory part have landed
+  uint64_t full[kAhead], n_empty[kNSlots], r_empty[kRSlots], v_empty[kVSlots], v_land[kVSlots], s_full, s_read, p_full, pv_done,
+      q_ready, q_full, q_part, q_free;
   long long scan[kThreads / 32], total;
   long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
   int seq, tile;                               // its first tile
@@ -344,15 +348,17 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kNSlots; ++s) { sm100::mbar_init(&ctl.n_full[s], 1); sm100::mbar_init(&ctl.n_empty[s], 1); }
-    for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_full[s], 1); sm100::mbar_init(&ctl.v_empty[s], 1); sm100::mbar_init(&ctl.v_land[s], 1); }
-    for (int s = 0; s < kRSlots; ++s) { sm100::mbar_init(&ctl.r_full[s], 1); sm100::mbar_init(&ctl.r_empty[s], 1); }
+    for (int s = 0; s < kAhead; ++s) sm100::mbar_init(&ctl.full[s], 3);
+    for (int s = 0; s < kNSlots; ++s) sm100::mbar_init(&ctl.n_empty[s], 1);
+    for (int s = 0; s < kRSlots; ++s) sm100::mbar_init(&ctl.r_empty[s], 1);
+    for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_empty[s], 1); sm100::mbar_init(&ctl.v_land[s], 1); }
     sm100::mbar_init(&ctl.s_full, 1);
     sm100::mbar_init(&ctl.s_read, 4);
     sm100::mbar_init(&ctl.p_full, 4);
     sm100::mbar_init(&ctl.pv_done, 1);
     sm100::mbar_init(&ctl.q_ready, 4);
     sm100::mbar_init(&ctl.q_full, 1);
+    sm100::mbar_init(&ctl.q_part, 1);
     sm100::mbar_init(&ctl.q_free, 1);
     ctl.abort_flag = 0;
     sm100::mbar_fence_init();
@@ -441,20 +447,21 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             for (int c = 0; c < kQTiles; ++c) chunk(sm100::smem_u32(q_smem) + c * kQChunk, bar, 64 * (other + c));
           }
         } else {
-          for (int h = 0; h < 2 && ok; ++h) {  // two tiles of this half's columns
-            ok = room(ctl.v_empty, kVSlots, at + h);
-            if (!ok) break;
-            const uint32_t s = (at + h) % kVSlots, bar = sm100::smem_u32(&ctl.v_full[s]);
-            expect_bytes(bar, 2 * boxes * rows * 128);
-            for (int c = 0; c < 2; ++c) chunk(v_base + s * kVTiles * kTile + c * kQChunk, bar, 64 * (4 - other + 2 * h + c));
-          }
-          for (int h = 0; h < 2 && ok; ++h) {  // 64 rows of the rotary columns
-            ok = room(ctl.r_empty, kRSlots, r_at + h);
-            if (!ok) break;
-            const uint32_t s = (r_at + h) % kRSlots, bar = sm100::smem_u32(&ctl.r_full[s]);
-            expect_bytes(bar, many ? kTile : h == 0 ? boxes * rows * 128 : 0);
-            if (many) tma_load_2d(r_base + s * kTile, &maps.q64, bar, kDv, w.t.row0 + 64 * h);
-            else if (h == 0) chunk(r_base + s * kTile, bar, kDv);
+          // this half's columns through two value slots (two tiles each), the rotary ones through two slots (64 rows each)
+          ok = room(ctl.r_empty, kRSlots, r_at) && room(ctl.r_empty, kRSlots, r_at + 1) && room(ctl.v_empty, kVSlots, at) &&
+               room(ctl.v_empty, kVSlots, at + 1);
+          if (ok) {
+            const uint32_t bar = sm100::smem_u32(&ctl.q_part);
+            expect_bytes(bar, (kVTiles + 1) * boxes * rows * 128);
+            for (int c = 0; c < kVTiles; ++c)
+              chunk(v_base + (at + (c >> 1)) % kVSlots * kVTiles * kTile + (c & 1) * kQChunk, bar, 64 * (4 - other + c));
+            const uint32_t r0 = r_base + r_at % kRSlots * kTile, r1 = r_base + (r_at + 1) % kRSlots * kTile;
+            if (many) {
+              tma_load_2d(r0, &maps.q64, bar, kDv, w.t.row0);
+              tma_load_2d(r1, &maps.q64, bar, kDv, w.t.row0 + 64);
+            } else {
+              chunk(r0, bar, kDv);
+            }
           }
         }
       }
@@ -499,31 +506,30 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
               }
             }
           };
+          const uint32_t bar = sm100::smem_u32(&ctl.full[g % kAhead]);
           if (ring == 0) {
             for (int u = 0; u < kNUnits; ++u) {
               ok = room(ctl.n_empty, kNSlots, at + u);
               if (!ok) break;
-              const uint32_t s = (at + u) % kNSlots, bar = sm100::smem_u32(&ctl.n_full[s]);
-              expect_bytes(bar, kNTiles * bytes);
-              part(n_base + s * kNTiles * kTile, &maps.two, bar, other + u * kNTiles, kNTiles);
+              if (u == 0) expect_bytes(bar, kQTiles * bytes);
+              part(n_base + (at + u) % kNSlots * kNTiles * kTile, &maps.two, bar, other + u * kNTiles, kNTiles);
             }
           } else {
             ok = room(ctl.r_empty, kRSlots, r_at);
             if (ok) {
-              const uint32_t s = r_at % kRSlots, bar = sm100::smem_u32(&ctl.r_full[s]);
               expect_bytes(bar, bytes);
-              part(r_base + s * kTile, &maps.one, bar, 8, 1);
+              part(r_base + r_at % kRSlots * kTile, &maps.one, bar, 8, 1);
               ok = room(ctl.v_empty, kVSlots, at);
             }
             if (ok) {
               const uint32_t s = at % kVSlots;
               // a last block that the sequence does not fill goes to the clearing warp first
               const bool last = left < kKeys;
-              const uint32_t bar = sm100::smem_u32(last ? &ctl.v_land[s] : &ctl.v_full[s]);
+              const uint32_t vbar = last ? sm100::smem_u32(&ctl.v_land[s]) : bar;
 #pragma unroll
               for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
-              expect_bytes(bar, kVTiles * bytes);
-              part(v_base + s * kVTiles * kTile, &maps.four, bar, 4 - other, kVTiles);
+              expect_bytes(vbar, kVTiles * bytes);
+              part(v_base + s * kVTiles * kTile, &maps.four, vbar, 4 - other, kVTiles);
             }
           }
         }
@@ -543,12 +549,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         for (uint32_t i = end > slots ? end - slots : 0; i < end; ++i)
           sm100::mbar_wait_limited(bars + i % slots, (i / slots) & 1, &never, nullptr, kWaitQ, 20000000LL);
       };
+      drain(ctl.full, kAhead, g + 1);
       if (ring == 0) {
-        drain(ctl.n_full, kNSlots, at + kNUnits);
         if (seg > 0) drain(&ctl.q_full, 1, seg);
       } else {
-        drain(ctl.v_full, kVSlots, at + 2);
-        drain(ctl.r_full, kRSlots, r_at + 2);
+        if (seg > 0) drain(&ctl.q_part, 1, seg);
 #pragma unroll
         for (int e = 0; e < kVSlots; ++e)
           if (landed[e]) drain(&ctl.v_land[e], 1, landed[e]);
@@ -558,7 +563,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   } else if (warp == 6) {
     // ---------------------------------------------------------------- rows behind a sequence's end
     // They may hold anything, also NaN, which a weight of zero would keep.
-    uint32_t v_at = 0, cleared[kVSlots] = {};
+    uint32_t v_at = 0, g = 0, cleared[kVSlots] = {};
     bool ok = true;
     for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
       if (w.blocks() > 0) v_at += 2;           // Q
@@ -578,9 +583,10 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             *reinterpret_cast<uint4*>(v + c * p.tile_bytes + (e >> 6) * group + (e & 63) * 16) = make_uint4(0, 0, 0, 0);
         sm100::fence_proxy_async();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&ctl.v_full[s]);
+        if (lane == 0) sm100::mbar_arrive(&ctl.full[(g + nb - 1) % kAhead]);
       }
       v_at += nb;
+      g += nb;
     }
   } else if (warp == 4) {
     // ---------------------------------------------------------------- tensor core
@@ -612,13 +618,13 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         sm100::tc_fence_after_sync();
         for (int k = 0; k <= nb; ++k) {
           if (k < nb) {                        // S = Q . K^T of block k
+            if (!sm100::mbar_wait(&ctl.full[g_qk % kAhead], (g_qk / kAhead) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
             if (g_qk > 0 && !sm100::mbar_wait(&ctl.s_read, (g_qk - 1) & 1, abort_flag, p.status, kWaitRead)) { ok = false; break; }
             sm100::tc_fence_after_sync();
             const uint32_t d = tmem + kColS;
 #pragma unroll
             for (int u = 0; u < kNUnits; ++u, ++n_at) {
               const uint32_t s = n_at % kNSlots;
-              if (!sm100::mbar_wait(&ctl.n_full[s], (n_at / kNSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
               const uint64_t b = n_desc + s * kNTiles * (kTile >> 4);
 #pragma unroll
               for (int c = 0; c < kNTiles; ++c)
@@ -628,16 +634,13 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
                                   (u > 0 || c > 0 || k4 > 0) ? 1u : 0u);
               sm100::umma_commit(&ctl.n_empty[s]);
             }
-            if (!ok) break;
             const uint32_t sr = r_at % kRSlots;
-            if (!sm100::mbar_wait(&ctl.r_full[sr], (r_at / kRSlots) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4)
               umma_ts(d, tmem + kColQ + kVTiles * 32 + k4 * 8, r_desc + sr * (kTile >> 4) + 2 * k4, idesc_qk, 1u);
             sm100::umma_commit(&ctl.r_empty[sr]);
             ++r_at;
             const uint32_t s = v_qk % kVSlots;
-            if (!sm100::mbar_wait(&ctl.v_full[s], (v_qk / kVSlots) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
 #pragma unroll
             for (int c = 0; c < kVTiles; ++c) {
               const uint64_t b = vk_desc + s * kVTiles * (kTile >> 4) + c * tile;
@@ -670,7 +673,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     // ---------------------------------------------------------------- softmax, one row per thread
     const int row = threadIdx.x;
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    uint32_t g = 0, v_at = 0, r_at = 0;        // blocks, value slots and rotary slots so far
+    uint32_t g = 0, v_at = 0, r_at = 0, seg = 0;   // blocks, value slots, rotary slots and tiles with blocks so far
     bool ok = true;
     const int own = half * kHalf;
     // Columns of Q to tensor memory, a row per thread: this half's from two slots of the value ring (two tiles of 64
@@ -685,16 +688,14 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       tmem_st_32x32(lanes + kColQ + c * 32, u);
     };
     auto take_q = [&]() {
-      for (int h = 0; h < 2; ++h, ++v_at) {
-        const uint32_t s = v_at % kVSlots;
-        if (!warp_wait(&ctl.v_full[s], (v_at / kVSlots) & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
+      if (!warp_wait(&ctl.q_part, seg & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) take_tile(v_ring + s * kVTiles * kTile + c * kQChunk, row, 2 * h + c);
-      }
-      const uint32_t at = r_at + (warp >> 1), s = at % kRSlots;
-      if (!warp_wait(&ctl.r_full[s], (at / kRSlots) & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
-      take_tile(r_ring + s * kTile, row & 63, kVTiles);
+      for (int c = 0; c < kVTiles; ++c)
+        take_tile(v_ring + (v_at + (c >> 1)) % kVSlots * kVTiles * kTile + (c & 1) * kQChunk, row, c);
+      take_tile(r_ring + (r_at + (warp >> 1)) % kRSlots * kTile, row & 63, kVTiles);
+      v_at += 2;
       r_at += 2;
+      ++seg;
       tmem_st_wait();
       sm100::tc_fence_before_sync();
       __syncwarp();
