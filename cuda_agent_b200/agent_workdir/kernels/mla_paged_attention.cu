@@ -54,6 +54,12 @@ constexpr float kRescale = 8.f;
 constexpr int kMaxBatch = 16384;
 enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitRead };
 
+// A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
+struct Seq { int tok, n, len, pos; };
+// Blocks [first, first + count) of 64 cache rows that some row of tile i sees; `units` = max(count, 1) is what
+// the tile counts as when the work is divided, so that a tile that sees nothing is still written.
+struct Item { int row0, rows, first, count, units; };
+
 struct __align__(16) Control {
   // full: by block, the other half's rows, the rotary columns and this half's rows; q_full, q_part: Q's shared and its
   // tensor-memory part have landed
@@ -62,9 +68,11 @@ struct __align__(16) Control {
   long long scan[kThreads / 32], total;
   long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
   int seq, tile;                               // its first tile
+  Seq first_seq;
+  Item first_item;
   alignas(16) int pages[2][2][kKeys];          // [producer][block parity]: the pages of a block's boxes
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, settled;
 };
 constexpr int kRingBytes = (kNSlots * kNTiles + kRSlots + kVSlots * kVTiles) * kTile;
 constexpr int kSmemBytes = kQTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
@@ -169,8 +177,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // and 16 rows.
 struct Maps { CUtensorMap one, two, four, q, q64, q16; };
 
-// A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
-struct Seq { int tok, n, len, pos; };
 __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   Seq s;
   const int a = min(max(__ldg(p.q_start + b), 0), p.T);
@@ -184,9 +190,6 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
 __device__ __forceinline__ int tiles_of(const Params& p, int n) {
   return (int)(((unsigned)n * (unsigned)p.H + kRows - 1) / kRows);    // T * H < 2^31
 }
-// Blocks [first, first + count) of 64 cache rows that some row of tile i sees; `units` = max(count, 1) is what
-// the tile counts as when the work is divided, so that a tile that sees nothing is still written.
-struct Item { int row0, rows, first, count, units; };
 __device__ __forceinline__ Item item_of(const Params& p, const Seq& s, int i) {
   Item t;
   const int r0 = i * kRows, left = s.n * p.H - r0;
@@ -210,11 +213,11 @@ struct Walk {
   int u0, u1;                                  // units of the tile that belong to this run
   __device__ __forceinline__ Walk(const Params& p, const Control& c)
       : b(c.seq), i(c.tile), x(c.x0), x1(c.x1), item_x(c.item_x) {
-    if (x < x1) load(p);
+    s = c.first_seq;
+    t = c.first_item;
+    if (x < x1) cut();
   }
-  __device__ __forceinline__ void load(const Params& p) {
-    s = seq_of(p, b);
-    t = item_of(p, s, i);
+  __device__ __forceinline__ void cut() {
     u0 = (int)(x - item_x);
     u1 = (int)min((long long)t.units, x1 - item_x);
   }
@@ -229,7 +232,8 @@ struct Walk {
       if (++b < p.batch) s = seq_of(p, b);
     }
     if (b >= p.batch) { x = x1; return; }
-    load(p);
+    t = item_of(p, s, i);
+    cut();
   }
   // blocks of this segment, as block numbers of the sequence
   __device__ __forceinline__ int begin() const { return t.first + u0; }
@@ -268,10 +272,76 @@ __device__ __forceinline__ long long block_scan(Control& ctl, long long v) {
   return before + x - v;
 }
 
+// The run of a pair, from what all tiles together count (W >= 1).
+struct Run { int pairs; long long x0, x1; };
+__device__ __forceinline__ Run run_of(long long W, int pair, int all) {
+  Run r;
+  r.pairs = (int)min((long long)all, W);       // no run is empty but those of the pairs behind
+  if (pair >= r.pairs) { r.x0 = r.x1 = W; return r; }
+  if (W < (1 << 24)) {
+    r.x0 = (unsigned)W * (unsigned)pair / (unsigned)r.pairs;
+    r.x1 = (unsigned)W * (unsigned)(pair + 1) / (unsigned)r.pairs;
+  } else {
+    r.x0 = W * pair / r.pairs;
+    r.x1 = W * (pair + 1) / r.pairs;
+  }
+  return r;
+}
+// Tile i of sequence b, which begins at `at`, is where the run begins.
+__device__ __forceinline__ void found(const Params& p, Control& ctl, const Run& r, long long W, int pair, long long at, int b,
+                                      int i, const Seq& s, const Item& t) {
+  ctl.x0 = r.x0; ctl.x1 = r.x1; ctl.item_x = at; ctl.seq = b; ctl.tile = i;
+  ctl.first_seq = s;
+  ctl.first_item = t;
+  // the pair that ends a cut tile says so to the merge kernel
+  Meta m{t.row0, 0, 0};
+  if (r.x0 > at && at + t.units <= r.x1) {
+    m.rows = t.rows;
+    m.first = (int)(((at + 1) * r.pairs - 1) / W);             // the last pair that begins at or before `at`
+  }
+  if ((blockIdx.x & 1) == 0) p.meta[pair] = m;
+}
+
 // Where pair `pair` begins: thread-parallel over the sequences, then over the tiles. `pre`: batch + 1 ints of
-// shared memory that nothing else uses yet.
+// shared memory that nothing else uses yet. A decode step of up to 32 sequences (no more than eight tiles each) is
+// settled by one warp without barriers, 1000 clk sooner.
 __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
   const int tid = threadIdx.x;
+  if (p.batch <= 32) {
+    bool done = true;
+    if (tid < 32) {
+      Seq s{0, 0, 0, 0};
+      if (tid < p.batch) s = seq_of(p, tid);
+      const int tiles = tiles_of(p, s.n);
+      done = __all_sync(0xffffffffu, tiles <= 8);
+      if (done) {
+        int sum = 0;
+        for (int i = 0; i < tiles; ++i) sum += item_of(p, s, i).units;
+        long long at = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(0xffffffffu, at, o);
+          if (tid >= o) at += y;
+        }
+        const long long W = __shfl_sync(0xffffffffu, at, 31);
+        at -= sum;
+        const Run r = run_of(max(W, 1LL), pair, p.pairs);
+        if (r.x0 < r.x1 && W > 0) {
+          for (int i = 0; i < tiles && at <= r.x0; ++i) {
+            const Item t = item_of(p, s, i);
+            if (r.x0 < at + t.units) found(p, ctl, r, W, pair, at, tid, i, s, t);
+            at += t.units;
+          }
+        } else if (tid == 0) {
+          ctl.x0 = ctl.x1 = 0;
+          if ((blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0};
+        }
+      }
+      if (tid == 0) ctl.settled = done;
+    }
+    __syncthreads();
+    if (ctl.settled) return;
+  }
   {
     const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
     long long sum = 0;
@@ -284,7 +354,7 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
   }
   const int tiles = (int)min(ctl.total, (long long)0x7fffffff);
   if (tid == 0) pre[p.batch] = tiles;
-  if (tid == 0) { ctl.x0 = ctl.x1 = ctl.item_x = 0; ctl.seq = ctl.tile = 0; }
+  if (tid == 0) ctl.x0 = ctl.x1 = 0;
   __syncthreads();
   const int per = (tiles + kThreads - 1) / kThreads;
   const int i0 = (int)min((long long)tid * per, (long long)tiles), i1 = min(i0 + per, tiles);
@@ -308,28 +378,20 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
   }
   long long at = block_scan(ctl, sum);
   const long long W = ctl.total;
-  const int pairs = (int)min((long long)p.pairs, W);           // no run is empty but those of the pairs behind
-  const long long x0 = pair < pairs ? W * pair / pairs : W, x1 = pair < pairs ? W * (pair + 1) / pairs : W;
-  if (x0 < x1 && at <= x0 && x0 < at + sum) {
+  const Run r = run_of(max(W, 1LL), pair, p.pairs);
+  if (W > 0 && r.x0 < r.x1 && at <= r.x0 && r.x0 < at + sum) {
     Seq s = seq_of(p, b);
     for (int i = i0; i < i1; ++i) {
       while (pre[b + 1] <= i) s = seq_of(p, ++b);
       const Item t = item_of(p, s, i - pre[b]);
-      if (x0 < at + t.units) {
-        ctl.x0 = x0; ctl.x1 = x1; ctl.item_x = at; ctl.seq = b; ctl.tile = i - pre[b];
-        // the pair that ends a cut tile says so to the merge kernel
-        Meta m{t.row0, 0, 0};
-        if (x0 > at && at + t.units <= x1) {
-          m.rows = t.rows;
-          m.first = (int)(((at + 1) * pairs - 1) / W);         // the last pair that begins at or before `at`
-        }
-        if ((blockIdx.x & 1) == 0) p.meta[pair] = m;
+      if (r.x0 < at + t.units) {
+        found(p, ctl, r, W, pair, at, b, i - pre[b], s, t);
         break;
       }
       at += t.units;
     }
   }
-  if (x0 >= x1 && tid == 0 && (blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0};
+  if ((W == 0 || r.x0 >= r.x1) && tid == 0 && (blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0};
   __syncthreads();
 }
 
@@ -435,32 +497,35 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       if (elect_one()) {                       // Q of this tile
         const bool many = w.t.rows > 4 * kQBox;
         const int boxes = many ? 1 : (w.t.rows + kQBox - 1) / kQBox, rows = many ? kRows : kQBox;
-        auto chunk = [&](uint32_t dst, uint32_t bar, int col) {
-          if (many) tma_load_2d(dst, &maps.q, bar, col, w.t.row0);
-          else for (int e = 0; e < boxes; ++e) tma_load_2d(dst + e * rows * 128, &maps.q16, bar, col, w.t.row0 + e * rows);
-        };
-        if (ring == 0) {
+        const CUtensorMap* map = many ? &maps.q : &maps.q16;
+        // ring 0: its tiles of Q to where they stay. Ring 1: this half's columns through two value slots (two tiles
+        // each), the rotary ones through two slots of their ring (64 rows each)
+        if (ring == 0)
           ok = seg == 0 || sm100::mbar_wait(&ctl.q_free, (seg - 1) & 1, abort_flag, p.status, kWaitQ);
-          if (ok) {
-            const uint32_t bar = sm100::smem_u32(&ctl.q_full);
-            expect_bytes(bar, kQTiles * boxes * rows * 128);
-            for (int c = 0; c < kQTiles; ++c) chunk(sm100::smem_u32(q_smem) + c * kQChunk, bar, 64 * (other + c));
-          }
-        } else {
-          // this half's columns through two value slots (two tiles each), the rotary ones through two slots (64 rows each)
+        else
           ok = room(ctl.r_empty, kRSlots, r_at) && room(ctl.r_empty, kRSlots, r_at + 1) && room(ctl.v_empty, kVSlots, at) &&
                room(ctl.v_empty, kVSlots, at + 1);
-          if (ok) {
-            const uint32_t bar = sm100::smem_u32(&ctl.q_part);
-            expect_bytes(bar, (kVTiles + 1) * boxes * rows * 128);
-            for (int c = 0; c < kVTiles; ++c)
-              chunk(v_base + (at + (c >> 1)) % kVSlots * kVTiles * kTile + (c & 1) * kQChunk, bar, 64 * (4 - other + c));
-            const uint32_t r0 = r_base + r_at % kRSlots * kTile, r1 = r_base + (r_at + 1) % kRSlots * kTile;
-            if (many) {
-              tma_load_2d(r0, &maps.q64, bar, kDv, w.t.row0);
-              tma_load_2d(r1, &maps.q64, bar, kDv, w.t.row0 + 64);
-            } else {
-              chunk(r0, bar, kDv);
+        if (ok) {
+          const uint32_t bar = sm100::smem_u32(ring == 0 ? &ctl.q_full : &ctl.q_part);
+          expect_bytes(bar, (kVTiles + ring) * boxes * rows * 128);
+#pragma unroll 1
+          for (int c = 0; c < kVTiles + ring; ++c) {
+            uint32_t dst = sm100::smem_u32(q_smem) + c * kQChunk;
+            int col = 64 * (other + c), n = boxes, step = rows;
+            if (ring == 1) {
+              dst = v_base + (at + (c >> 1)) % kVSlots * kVTiles * kTile + (c & 1) * kQChunk;
+              col = 64 * (4 - other + c);
+              if (c == kVTiles) {
+                dst = r_base + r_at % kRSlots * kTile;
+                col = kDv;
+                if (many) { map = &maps.q64; n = 2; step = 64; }
+              }
+            }
+#pragma unroll 1
+            for (int e = 0; e < n; ++e) {
+              if (c == kVTiles && many) dst = r_base + (r_at + e) % kRSlots * kTile;
+              tma_load_2d(dst, map, bar, col, w.t.row0 + e * step);
+              dst += step * 128;
             }
           }
         }
@@ -487,49 +552,42 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 #pragma unroll
             for (int e = 1; e < 8; ++e) rw[e] = rw[e - 1] + 8 == p.page_size ? 0 : rw[e - 1] + 8;
           }
-          // `tiles` tiles of each box from column tile `from` on
-          auto part = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int from, int tiles) {
+          // two pieces: the units of ring 0, or the rotary columns and V
+          const uint32_t bar = sm100::smem_u32(&ctl.full[g % kAhead]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bool rot = ring == 1 && u == 0, val = ring == 1 && u == 1;
+            const uint32_t use = ring == 0 ? at + u : rot ? r_at : at, slots = ring == 0 ? kNSlots : rot ? kRSlots : kVSlots;
+            ok = room(ring == 0 ? ctl.n_empty : rot ? ctl.r_empty : ctl.v_empty, slots, use);
+            if (!ok) break;
+            const int tiles = ring == 0 ? kNTiles : rot ? 1 : kVTiles;
+            const int from = ring == 0 ? other + u * kNTiles : rot ? 8 : 4 - other;
+            const uint32_t s = use % slots;
+            const uint32_t dst = ring == 0 ? n_base + s * kNTiles * kTile : rot ? r_base + s * kTile : v_base + s * kVTiles * kTile;
+            // a last block of V that the sequence does not fill goes to the clearing warp first
+            const bool last = val && left < kKeys;
+            const uint32_t on = last ? sm100::smem_u32(&ctl.v_land[s]) : bar;
+#pragma unroll
+            for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
+            if (ring == 1 || u == 0) expect_bytes(on, (ring == 0 ? kQTiles : tiles) * bytes);
+            const CUtensorMap* map = p.box < 8 || tiles == 1 ? &maps.one : tiles == 2 ? &maps.two : &maps.four;
             if (p.box == kKeys) {
-              tma_load_4d(dst, map, bar, 0, rw[0], from, pg[0]);
+              tma_load_4d(dst, map, on, 0, rw[0], from, pg[0]);
             } else if (p.box == 8) {           // boxes of several tiles keep the eight-row groups that swizzling wants
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                if (e < boxes) tma_load_4d(dst + e * tiles * 1024, map, bar, 0, rw[e], from, pg[e]);
+                if (e < boxes) tma_load_4d(dst + e * tiles * 1024, map, on, 0, rw[e], from, pg[e]);
             } else {
+#pragma unroll 1
               for (int c = 0; c < tiles; ++c) {
                 int row = row0;
+#pragma unroll 1
                 for (int e = 0; e < boxes; ++e) {
-                  tma_load_4d(dst + c * kTile + e * p.box * 128, &maps.one, bar, 0, row, from + c, list[e]);
+                  tma_load_4d(dst + c * kTile + e * p.box * 128, map, on, 0, row, from + c, list[e]);
                   row += p.box;
                   if (row == p.page_size) row = 0;
                 }
               }
-            }
-          };
-          const uint32_t bar = sm100::smem_u32(&ctl.full[g % kAhead]);
-          if (ring == 0) {
-            for (int u = 0; u < kNUnits; ++u) {
-              ok = room(ctl.n_empty, kNSlots, at + u);
-              if (!ok) break;
-              if (u == 0) expect_bytes(bar, kQTiles * bytes);
-              part(n_base + (at + u) % kNSlots * kNTiles * kTile, &maps.two, bar, other + u * kNTiles, kNTiles);
-            }
-          } else {
-            ok = room(ctl.r_empty, kRSlots, r_at);
-            if (ok) {
-              expect_bytes(bar, bytes);
-              part(r_base + r_at % kRSlots * kTile, &maps.one, bar, 8, 1);
-              ok = room(ctl.v_empty, kVSlots, at);
-            }
-            if (ok) {
-              const uint32_t s = at % kVSlots;
-              // a last block that the sequence does not fill goes to the clearing warp first
-              const bool last = left < kKeys;
-              const uint32_t vbar = last ? sm100::smem_u32(&ctl.v_land[s]) : bar;
-#pragma unroll
-              for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
-              expect_bytes(vbar, kVTiles * bytes);
-              part(v_base + s * kVTiles * kTile, &maps.four, vbar, 4 - other, kVTiles);
             }
           }
         }
