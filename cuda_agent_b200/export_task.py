@@ -5,7 +5,7 @@ The reference's loop works on ONE directory: it compiles every ``*.cu`` / ``*.cp
 (agent_workdir/utils/verification.py:8-9) and is driven by ``cd`` alone. This package keeps several tasks in
 one workspace; ``export`` writes the directory the reference's loop expects for one of them:
 
-    python -m cuda_agent_b200.export_task <task> <dest>      # task: gdn | mla | moe | moe_ep
+    python -m cuda_agent_b200.export_task <task> <dest>      # task: gdn | mla | mla_paged | moe | moe_ep
     cd <dest>
     TORCH_CUDA_ARCH_LIST=10.0a bash utils/compile.sh --torch-load
     python3 -m utils.verification
@@ -33,11 +33,12 @@ WORKDIR = PKG / "agent_workdir"
 TASKS = {
     "gdn": ("gdn", "CAB_GDN_CONFIG"),
     "mla": ("mla", "CAB_MLA_CONFIG"),
+    "mla_paged": ("mla_paged", "CAB_MLA_PAGED_CONFIG"),
     "moe": ("moe", "CAB_MOE_CONFIG"),
     "moe_ep": ("moe", "CAB_MOE_CONFIG"),
 }
 # the smallest configuration of each eager model that the CUDA operator accepts
-DEFAULT_CONFIG = {"gdn": 0, "mla": 1, "moe": 0, "moe_ep": 1}
+DEFAULT_CONFIG = {"gdn": 0, "mla": 1, "mla_paged": 0, "moe": 0, "moe_ep": 1}
 
 
 def export(task: str, dest: Path, config: int | None = None) -> Path:

@@ -1,0 +1,192 @@
+"""The paged latent cache without a GPU: the eager model against float64 loops, rotary frequencies, refusals that come
+before anything touches a device."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from conftest import load_oracle
+
+
+@pytest.fixture(scope="module")
+def capi(built_libs):
+    from cuda_agent_b200 import capi
+    capi.lib()
+    return capi
+
+
+def test_eager_model_against_loops():
+    m = load_oracle("mla_paged", {"CAB_MLA_PAGED_CONFIG": 0})
+    new, rows, heads, page = [3, 1], [3, 9], 2, 4
+    q, q_pe, c_kv, k_pe, cache, table, start, kv = m.make_inputs(new, rows, heads, page, torch.Generator().manual_seed(1))
+    out, lse, after = m.Model(heads, page)(q, q_pe, c_kv, k_pe, cache, table, start, kv)
+    want = cache.clone()
+    t = 0
+    for b, n in enumerate(new):
+        for i in range(n):
+            pos = rows[b] - n + i
+            turn = [pos * 10000.0 ** (-e / 32) for e in range(32)]
+
+            def rot(x):
+                y = []
+                for e, a in enumerate(turn):
+                    u, v = float(x[2 * e]), float(x[2 * e + 1])
+                    y += [u * math.cos(a) - v * math.sin(a), v * math.cos(a) + u * math.sin(a)]
+                return torch.tensor(y, dtype=torch.float64).to(torch.bfloat16)
+            want[table[b, pos // page].long(), pos % page] = torch.cat((c_kv[t], rot(k_pe[t])))
+            for h in range(heads):
+                x = torch.cat((q[t, h, :512], rot(q_pe[t, h]))).double()
+                seen = torch.stack([want[table[b, j // page].long(), j % page].double() for j in range(pos + 1)])
+                s = (seen @ x) * 192 ** -0.5
+                w = torch.exp(s - s.max())
+                got = out[t, h].double()
+                exact = (w / w.sum()) @ seen[:, :512]
+                # bf16 roundings of the result, and of rotated values by another last bit at most
+                assert ((got - exact).abs() <= 2.0 ** -8 * exact.abs() + 2e-2).all()
+                assert abs(float(lse[t, h]) - float(s.max() + torch.log(w.sum()))) <= 2e-2
+            t += 1
+    assert ((after.double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs()).all()
+
+
+def test_frequencies():
+    from cuda_agent_b200.paged import rope_frequencies
+    f, m = rope_frequencies(64, device="cpu")
+    assert f.dtype == torch.float64 and m == 1.0 and f[0] == 1.0
+    assert abs(float(f[31]) - 10000.0 ** (-62 / 64)) < 1e-15
+    lin, _ = rope_frequencies(64, scaling="linear", factor=4.0, device="cpu")
+    assert torch.equal(lin, f / 4)
+    ntk, _ = rope_frequencies(64, scaling="ntk", factor=4.0, device="cpu")
+    assert ntk[0] == 1.0 and abs(float(ntk[31] / f[31]) - 0.25) < 1e-12 and (ntk[1:] < f[1:]).all()
+    yarn, m = rope_frequencies(64, scaling="yarn", factor=40.0, original_length=4096, device="cpu")
+    assert abs(m - (0.1 * math.log(40.0) + 1)) < 1e-15
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.allclose(yarn[turns > 32 * 1.4], f[turns > 32 * 1.4], rtol=1e-14)
+    assert torch.allclose(yarn[turns < 1 / 1.4], f[turns < 1 / 1.4] / 40, rtol=1e-14)
+    assert ((yarn <= f * (1 + 1e-15)) & (yarn >= f / 40 * (1 - 1e-15))).all()
+    same, m = rope_frequencies(64, scaling="yarn", factor=1.0, device="cpu")
+    assert torch.allclose(same, f, rtol=1e-15) and m == 1.0
+    for bad in (dict(rot=63), dict(rot=0), dict(rot=64, scaling="log"), dict(rot=64, factor=0.5), dict(rot=64, base=1.0),
+                dict(rot=2, scaling="ntk"), dict(rot=64, original_length=0)):
+        with pytest.raises(ValueError):
+            rope_frequencies(**bad, device="cpu")
+
+
+def batch(capi, **kw):
+    fake = 0x10000                                   # aligned, never dereferenced: the checks fail first
+    b = capi.MlaPagedBatch(fake, 64 * 576, 576, 10, 64, fake, fake, fake, 2, 4, 0)
+    for k, v in kw.items():
+        setattr(b, k, v)
+    return ctypes.byref(b)
+
+
+OK, BAD, MISALIGNED, LARGE = 0, 1, 2, 4
+
+
+def test_attention_refuses_before_the_device(capi):
+    f, p = capi.lib().mla_paged_attention_launcher, 0x10000
+    need = capi.mla_paged_workspace_bytes(8, 16)
+
+    def call(out=p, lse=p, q=p, b=None, T=8, H=16, scale=0.07, window=0, ws=p, nbytes=need):
+        return f(out, lse, q, b if b is not None else batch(capi), T, H, scale, 1, window, ws, nbytes, None, 0, None)
+
+    assert call(T=0) == OK and call(b=batch(capi, batch=0)) == OK
+    for kw in (dict(T=-1), dict(H=0), dict(out=None), dict(q=None), dict(ws=None), dict(nbytes=need - 1), dict(scale=0.0),
+               dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1)):
+        assert call(**kw) == BAD, kw
+    assert f(p, p, p, None, 8, 16, 0.07, 1, 0, p, need, None, 0, None) == BAD
+    for kw in (dict(rows=None), dict(page_table=None), dict(q_start=None), dict(kv_len=None), dict(batch=-1), dict(num_pages=0),
+               dict(page_size=0), dict(max_pages=0), dict(dtype=2), dict(dtype=7), dict(token_stride=575), dict(token_stride=580),
+               dict(page_stride=4), dict(page_stride=64 * 576 + 1)):
+        assert call(b=batch(capi, **kw)) == BAD, kw
+    for kw in (dict(out=p + 8), dict(q=p + 2), dict(ws=p + 4), dict(b=batch(capi, rows=p + 8))):
+        assert call(**kw) == MISALIGNED, kw
+    assert call(T=1 << 24, H=128, nbytes=1 << 40) == LARGE
+    assert call(b=batch(capi, batch=16385)) == LARGE
+    assert call(b=batch(capi, max_pages=1 << 26, page_size=64)) == LARGE
+
+
+def test_rope_refuses_before_the_device(capi):
+    f, p = capi.lib().mla_rope_launcher, 0x10000
+
+    def call(out=p, x=p, pos=p, freq=p, T=4, H=2, R=64, st=128, sh=64, dtype=0, inter=0):
+        return f(out, x, pos, freq, T, H, R, st, sh, st, sh, dtype, inter, 0, 1.0, 0, None)
+
+    assert call(T=0) == OK and call(H=0) == OK
+    for kw in (dict(T=-1), dict(R=63), dict(R=0), dict(out=None), dict(x=None), dict(pos=None), dict(freq=None), dict(dtype=3)):
+        assert call(**kw) == BAD, kw
+    assert call(R=2050) == LARGE
+    for kw in (dict(x=p + 1), dict(x=p + 2, inter=1), dict(sh=63, inter=1), dict(x=p + 2, dtype=2), dict(x=p + 4, dtype=2, inter=1)):
+        assert call(**kw) == MISALIGNED, kw
+    g = capi.lib().mla_rope_append_launcher
+
+    def append(qo=p, q=p, c=p, k=p, b=None, freq=p, T=4, H=2, inter=0, kt=64):
+        return g(qo, q, c, k, b if b is not None else batch(capi), freq, T, H, 128, 64, 128, 64, 512, kt, inter, 1.0, None, 0, None)
+
+    assert append(T=0) == OK and append(b=batch(capi, batch=0)) == OK
+    for kw in (dict(T=-1), dict(H=-1), dict(qo=None), dict(q=None), dict(c=None), dict(k=None), dict(freq=None),
+               dict(b=batch(capi, token_stride=570)), dict(b=batch(capi, page_size=0)), dict(b=batch(capi, dtype=2))):
+        assert append(**kw) == BAD, kw
+    assert append(b=batch(capi, rows=p + 8)) == MISALIGNED and append(k=p + 2, inter=1) == MISALIGNED
+    assert append(inter=1, kt=65) == MISALIGNED
+
+
+def test_pages_refuse_before_the_device(capi):
+    lib, p = capi.lib(), 0x10000
+    assert lib.mla_pages_scratch_bytes(0, 4) == 0 and lib.mla_pages_scratch_bytes(10, 4) >= 4 * (16 + 30 + 15)
+
+    def copy(pages=p, ls=1000, layers=2, P=10, pb=100, src=p, dst=p, n=3, scratch=p):
+        return lib.mla_pages_copy_launcher(pages, ls, layers, P, pb, src, dst, n, scratch, None, 0, None)
+
+    assert copy(n=0) == OK and copy(layers=0) == OK
+    for kw in (dict(n=-1), dict(P=0), dict(pages=None), dict(pb=0), dict(ls=999), dict(src=None), dict(dst=None),
+               dict(scratch=None), dict(layers=-1)):
+        assert copy(**kw) == BAD, kw
+    assert copy(n=(1 << 20) + 1) == LARGE and copy(scratch=p + 4) == MISALIGNED
+
+    def extend(t=p, le=p, rc=p, slots=4, mp=4, P=10, ps=16, seqs=p, new=p, n=3, scratch=p):
+        return lib.mla_pages_extend_launcher(t, le, rc, slots, mp, P, ps, seqs, new, n, scratch, None, 0, None)
+
+    assert extend(n=0) == OK
+    for kw in (dict(n=-1), dict(t=None), dict(le=None), dict(rc=None), dict(slots=0), dict(mp=0), dict(P=0), dict(ps=0),
+               dict(seqs=None), dict(new=None), dict(scratch=None)):
+        assert extend(**kw) == BAD, kw
+    assert extend(n=(1 << 20) + 1) == LARGE and extend(scratch=p + 8) == MISALIGNED
+    free = lib.mla_pages_free_launcher
+    assert free(p, p, p, 4, 4, 10, 16, p, 0, None, 0, None) == OK
+    assert free(p, p, p, 4, 4, 10, 16, None, 1, None, 0, None) == BAD
+    assert free(p, p, p, 4, 4, 10, 0, p, 1, None, 0, None) == BAD
+    fork = lib.mla_pages_fork_launcher
+    assert fork(p, 1000, 2, 100, p, p, p, 4, 4, 10, 16, p, p, 0, p, None, 0, None) == OK
+    assert fork(None, 1000, 2, 100, p, p, p, 4, 4, 10, 16, p, p, 1, p, None, 0, None) == BAD
+    assert fork(p, 1000, 2, 100, p, p, p, 4, 4, 10, 16, p, None, 1, p, None, 0, None) == BAD
+    compact = lib.mla_pages_compact_launcher
+    assert compact(p, 1000, 2, 100, p, p, p, 4, 4, 10, 16, None, None, 0, None) == BAD
+    assert compact(p, 999, 2, 100, p, p, p, 4, 4, 10, 16, p, None, 0, None) == BAD
+
+
+def test_extension_refuses_cpu_tensors(built_libs):
+    import cuda_agent_b200
+    ext = cuda_agent_b200.load_extension()
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    x, cache = torch.zeros(2, 3, 64), torch.zeros(4, 16, 576, dtype=torch.bfloat16)
+    for bad in (lambda: ext.mla_rope_forward(x, i(2), torch.zeros(32, dtype=torch.float64)),
+                lambda: ext.mla_rope_append_forward(x, x, x, cache, i(1, 4), i(2), i(1), x),
+                lambda: ext.mla_paged_attention_forward(cache, cache, i(1, 4), i(2), i(1), 0.07),
+                lambda: ext.mla_pages_copy(cache[None], i(1), i(1)), lambda: ext.mla_pages_extend(i(2, 4), i(2), i(4), i(1), i(1), 16),
+                lambda: ext.mla_pages_fork(cache[None], i(2, 4), i(2), i(4), i(1), i(1)),
+                lambda: ext.mla_pages_free(i(2, 4), i(2), i(4), i(1), 16),
+                lambda: ext.mla_pages_compact(cache[None], i(2, 4), i(2), i(4))):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            bad()
+
+
+def test_cache_class_refuses(built_libs):
+    from cuda_agent_b200.paged import PagedLatentCache
+    for kw in (dict(layers=0), dict(pages=0), dict(page_size=0), dict(slots=0), dict(max_rows=0), dict(dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            PagedLatentCache(**{**dict(layers=1, pages=4, page_size=16, slots=2, max_rows=64, device="cpu"), **kw})
+    c = PagedLatentCache(2, 5, 16, 3, 70, device="cpu")
+    assert c.page_table.shape == (3, 5) and (c.page_table == -1).all() and c.pages_free() == 5
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        c.extend([0], [4])
