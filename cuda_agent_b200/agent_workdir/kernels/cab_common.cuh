@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "../../../include/cuda_agent_b200.h"
@@ -47,6 +48,17 @@ inline bool ensure_dynamic_smem(int bytes) {
     done[dev] = true;
   }
   return true;
+}
+
+// SMs of the current device, asked for once per device; 0 on failure.
+inline int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = -1, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 __device__ __forceinline__ float warp_sum(float x) {

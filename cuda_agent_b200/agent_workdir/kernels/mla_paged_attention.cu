@@ -432,6 +432,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   if (warp == 5 && lane == 0) {
     for (const CUtensorMap* m : {&maps.one, &maps.two, &maps.four, &maps.q, &maps.q64, &maps.q16}) sm100::prefetch_tensormap(m);
   }
+  cudaGridDependencySynchronize();             // up to here nothing of what earlier work wrote was read
   find_run(p, ctl, reinterpret_cast<int*>(n_ring), pair);
   sm100::fence_proxy_async();                  // the rings were used as scratch
   sm100::tc_fence_before_sync();
@@ -933,6 +934,7 @@ constexpr int kMergeRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(128 * kMergeRows) mla_paged_merge_kernel(const Params p) {
   __shared__ float2 s_ml[kMergeRows][2][cab::kNumSMs / 2];
+  cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   const int pair = blockIdx.x, sub = threadIdx.x >> 7, tid = threadIdx.x & 127;
   const Meta m = p.meta[pair];
@@ -984,20 +986,26 @@ int rows_cap_of(int T, int H) { return (int)((long long)T * H < kRows ? (long lo
 template <typename T>
 int launch(Params& p, const Maps& maps, cudaStream_t stream) {
   if (!cab::ensure_dynamic_smem<&mla_paged_attention_kernel<T>>(kSmemBytes)) return CAB_ERR_LAUNCH;
-  mla_paged_attention_kernel<T><<<2 * p.pairs, kThreads, kSmemBytes, stream>>>(p, maps);
-  const int rc = cab::launch_status();
-  if (rc != CAB_OK || p.pairs == 1) return rc;
-  // launched while the first kernel runs; it waits for that one's end itself
+  // Either kernel is set up while the one before it ends, and waits for that end itself before it reads or writes
+  // anything (cudaGridDependencySynchronize): some 2 us less for a decode step.
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows);
-  cfg.blockDim = dim3(128 * kMergeRows);
+  cfg.gridDim = dim3(2 * p.pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, mla_paged_merge_kernel<T>, static_cast<const Params>(p)) != cudaSuccess) return CAB_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, mla_paged_attention_kernel<T>, static_cast<const Params>(p), maps) != cudaSuccess)
+    return CAB_ERR_LAUNCH;
+  if (p.pairs > 1) {
+    cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows);
+    cfg.blockDim = dim3(128 * kMergeRows);
+    cfg.dynamicSmemBytes = 0;
+    if (cudaLaunchKernelEx(&cfg, mla_paged_merge_kernel<T>, static_cast<const Params>(p)) != cudaSuccess) return CAB_ERR_LAUNCH;
+  }
   return cab::launch_status();
 }
 
@@ -1053,10 +1061,8 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.window = window < (long long)batch->max_pages * batch->page_size ? window : 0;   // wider than any history: none
   p.rows_cap = rows_cap_of(T, H);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2)
-    return CAB_ERR_LAUNCH;
+  const int sms = cab::sm_count();
+  if (sms < 2) return CAB_ERR_LAUNCH;
   p.pairs = sms / 2 < kPairs ? sms / 2 : kPairs;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const size_t rows = (size_t)kPairs * 2 * p.rows_cap;

@@ -15,6 +15,9 @@
 // Registered with the other mla ops, by mla_binding.cpp.
 #include "binding_common.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+
 namespace {
 using cab_binding::check_cuda_contig;
 using cab_binding::check_same_device;
@@ -35,6 +38,12 @@ void check_view(const torch::Tensor& t, const char* name, int64_t dims) {
   TORCH_CHECK(t.dim() == dims, name, " must have ", cab_binding::text(dims), " dimensions");
   TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, ": the last dimension must be contiguous");
 }
+
+// Outputs and scratch memory without the dispatcher: a decode step's calls are short.
+torch::Tensor fresh(at::IntArrayRef sizes, const torch::Tensor& like, c10::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+c10::DataPtr scratch_bytes(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 // A stride that is never used must not cost the wide accesses.
 int64_t stride_of(const torch::Tensor& t, int64_t d) { return t.size(d) <= 1 ? 0 : t.stride(d); }
@@ -136,7 +145,7 @@ torch::Tensor mla_rope_forward(torch::Tensor x, torch::Tensor positions, torch::
   check_same_device(x, positions, "x", "positions");
   check_same_device(x, freq, "x", "freq");
   c10::cuda::CUDAGuard guard(x.device());
-  torch::Tensor out = out_arg.has_value() ? *out_arg : torch::empty({T, H, R}, x.options());
+  torch::Tensor out = out_arg.has_value() ? *out_arg : fresh({T, H, R}, x, x.scalar_type());
   if (out_arg.has_value()) {
     check_view(out, "out", 3);
     TORCH_CHECK(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type(), "out must have the shape and type of x");
@@ -214,7 +223,7 @@ std::tuple<torch::Tensor, torch::Tensor> mla_paged_attention_forward(
     check_same_device(cache, out, "cache", "out");
     TORCH_CHECK(!out.numel() || (!out.is_alias_of(q) && !out.is_alias_of(cache)), "out must not share storage with q or the cache");
   } else {
-    out = torch::empty({T, H, 512}, q.options());
+    out = fresh({T, H, 512}, q, q.scalar_type());
     config |= 256;                             // tokens behind the last sequence: zeros in a fresh output
   }
   if (lse_arg.has_value()) {
@@ -225,13 +234,14 @@ std::tuple<torch::Tensor, torch::Tensor> mla_paged_attention_forward(
     TORCH_CHECK(out_arg.has_value(), "lse is given together with out");
   } else {
     lse = out_arg.has_value() ? torch::full({T, H}, -INFINITY, q.options().dtype(torch::kFloat32))
-                              : torch::empty({T, H}, q.options().dtype(torch::kFloat32));
+                              : fresh({T, H}, q, torch::kFloat32);
   }
   const size_t bytes = mla_paged_attention_workspace_bytes(to_int(T, "T"), to_int(H, "H"));
-  torch::Tensor workspace = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8)), status;
+  const c10::DataPtr workspace = scratch_bytes(bytes);
+  torch::Tensor status;
   if (check) status = torch::empty({1}, q_start.options());
   check_status(mla_paged_attention_launcher(out.data_ptr(), ptr<float>(lse), q.data_ptr(), &batch, (int)T, (int)H,
-                                            (float)softmax_scale, causal, (int)window, bytes ? workspace.data_ptr() : nullptr,
+                                            (float)softmax_scale, causal, (int)window, workspace.get(),
                                             bytes, check ? ptr<int>(status) : nullptr, config, current_stream()),
                "mla_paged_attention_forward");
   if (check) raise_status(status, "mla_paged_attention_forward");
@@ -282,9 +292,8 @@ int list_of(const torch::Tensor& t, const char* name, const torch::Tensor& like)
   check_same_device(t, like, name, "the pool");
   return to_int(t.size(0), name);
 }
-torch::Tensor scratch_for(int num_pages, int n, const torch::Tensor& like) {
-  return torch::empty({(int64_t)mla_pages_scratch_bytes(num_pages, n)}, like.options().dtype(torch::kUInt8));
-}
+// On the current device and stream.
+c10::DataPtr scratch_for(int num_pages, int n) { return scratch_bytes(mla_pages_scratch_bytes(num_pages, n)); }
 torch::Tensor status_if(bool check, const torch::Tensor& like) {
   return check ? torch::empty({1}, like.options().dtype(torch::kInt32)) : torch::Tensor();
 }
@@ -295,9 +304,10 @@ torch::Tensor mla_pages_copy(torch::Tensor pages, torch::Tensor src, torch::Tens
   const int n = list_of(src, "src", pages);
   TORCH_CHECK(list_of(dst, "dst", pages) == n, "src and dst must be equally long");
   c10::cuda::CUDAGuard guard(pages.device());
-  auto scratch = scratch_for(p.num_pages, n, pages), status = status_if(check, pages);
+  const auto scratch = scratch_for(p.num_pages, n);
+  const auto status = status_if(check, pages);
   check_status(mla_pages_copy_launcher(p.data, p.layer_stride, p.layers, p.num_pages, p.page_bytes, ptr<const int>(src),
-                                       ptr<const int>(dst), n, scratch.data_ptr(), status_ptr(status), 0, current_stream()),
+                                       ptr<const int>(dst), n, scratch.get(), status_ptr(status), 0, current_stream()),
                "mla_pages_copy");
   if (check) raise_status(status, "mla_pages_copy");
   return pages;
@@ -310,10 +320,11 @@ void mla_pages_extend(torch::Tensor page_table, torch::Tensor length, torch::Ten
   TORCH_CHECK(list_of(new_length, "new_length", length) == n, "seqs and new_length must be equally long");
   TORCH_CHECK(!new_length.is_alias_of(length), "new_length must not be length itself");
   c10::cuda::CUDAGuard guard(length.device());
-  auto scratch = scratch_for(q.num_pages, n, length), status = status_if(check, length);
+  const auto scratch = scratch_for(q.num_pages, n);
+  const auto status = status_if(check, length);
   check_status(mla_pages_extend_launcher(ptr<int>(page_table), ptr<int>(length), ptr<int>(refcount), q.slots, q.max_pages,
                                          q.num_pages, to_int(page_size, "page_size"), ptr<const int>(seqs),
-                                         ptr<const int>(new_length), n, scratch.data_ptr(), status_ptr(status), 0,
+                                         ptr<const int>(new_length), n, scratch.get(), status_ptr(status), 0,
                                          current_stream()),
                "mla_pages_extend");
   if (check) raise_status(status, "mla_pages_extend");
@@ -328,10 +339,11 @@ void mla_pages_fork(torch::Tensor pages, torch::Tensor page_table, torch::Tensor
   const int n = list_of(src, "src", length);
   TORCH_CHECK(list_of(dst, "dst", length) == n, "src and dst must be equally long");
   c10::cuda::CUDAGuard guard(length.device());
-  auto scratch = scratch_for(q.num_pages, n, length), status = status_if(check, length);
+  const auto scratch = scratch_for(q.num_pages, n);
+  const auto status = status_if(check, length);
   check_status(mla_pages_fork_launcher(p.data, p.layer_stride, p.layers, p.page_bytes, ptr<int>(page_table), ptr<int>(length),
                                        ptr<int>(refcount), q.slots, q.max_pages, q.num_pages, p.page_size,
-                                       ptr<const int>(src), ptr<const int>(dst), n, scratch.data_ptr(), status_ptr(status), 0,
+                                       ptr<const int>(src), ptr<const int>(dst), n, scratch.get(), status_ptr(status), 0,
                                        current_stream()),
                "mla_pages_fork");
   if (check) raise_status(status, "mla_pages_fork");
@@ -357,10 +369,11 @@ void mla_pages_compact(torch::Tensor pages, torch::Tensor page_table, torch::Ten
   TORCH_CHECK(q.num_pages == p.num_pages, "refcount must have an entry for each page");
   check_same_device(pages, length, "pages", "length");
   c10::cuda::CUDAGuard guard(length.device());
-  auto scratch = scratch_for(q.num_pages, 0, length), status = status_if(check, length);
+  const auto scratch = scratch_for(q.num_pages, 0);
+  const auto status = status_if(check, length);
   check_status(mla_pages_compact_launcher(p.data, p.layer_stride, p.layers, p.page_bytes, ptr<int>(page_table),
                                           ptr<const int>(length), ptr<int>(refcount), q.slots, q.max_pages, q.num_pages,
-                                          p.page_size, scratch.data_ptr(), status_ptr(status), 0, current_stream()),
+                                          p.page_size, scratch.get(), status_ptr(status), 0, current_stream()),
                "mla_pages_compact");
   if (check) raise_status(status, "mla_pages_compact");
 }
