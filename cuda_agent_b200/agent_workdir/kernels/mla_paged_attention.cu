@@ -4,29 +4,33 @@
 // head) pairs of a sequence are the rows of one matrix, and 128 of them make a tile whatever the head count:
 // one token with 128 heads, eight tokens with 16, or a decode step's 16 rows in a tile that is mostly empty.
 //
-// A tile of 128 rows times 512 value columns of fp32 would take all of tensor memory, so two CTAs share a tile:
-// each accumulates 256 of the value columns and computes the scores for itself (832 column steps instead of
-// 544; the alternative, exchanging partial scores between the CTAs, costs more than the second Q.K^T here).
-// Tensor memory: O 256 columns, S 64, P (16 bit, the A operand of P.V) 32, and 160 for 320 columns of Q as the A
-// operand: this CTA's value half and the rotary columns. Shared memory: the other 256 columns of Q (64 KB) and rings
-// for what a block of 64 cache rows has: the other value half, which only Q.K^T reads, in two units of 128 columns
-// (16 KB, three slots), the rotary columns (8 KB, two slots), and this CTA's value half, which P.V reads as well
-// (32 KB, three slots). The tensor core takes Q.K^T of block j+1 and then P.V of block j, so the softmax of block j
-// has the time of a Q.K^T, and every slot is asked for again 2000 clk or more before it is read: a row comes from
-// either die's L2, 1600 to 2800 clk away under load. (With one buffer for the part that only Q.K^T reads, the wait
-// for it doubled the kernel's time; with P.V between the parts of Q.K^T and two slots a softmax of 1100 clk showed.)
-//   warps 0-3  one (token, head) row per thread: softmax, result. The reference maximum of a row moves only
-//              when it would grow by more than 2^8, so O is hardly ever rescaled
+// A tile of 128 rows times 512 value columns of fp32 would take all of tensor memory, so a cluster of two CTAs shares
+// a tile. Each accumulates 256 of the value columns over all keys, and forms the scores of every other 64 keys over all
+// 576 columns: a step of 128 keys is 64 for either CTA. What crosses between them is P, 16 KB a step and direction.
+// (The same tile without an exchange, each CTA forming all scores for itself, took 832 column steps a key instead
+// of 544 and 4800 clk for 128 keys at best; it ran on the power limit at the tensor rate of a library product.)
+//   tensor memory  O 256 columns, S 64, P of the own keys 32 (16 bit, the A operand of P.V), 160 for 320 columns of
+//                  Q as the A operand: this CTA's value half and the rotary columns
+//   shared memory  the other 256 columns of Q (64 KB); of the own keys the other value half in two units of 128
+//                  columns (16 KB each), the rotary columns (8 KB) and the own value half (32 KB, two slots); of the
+//                  other CTA's keys the own value half (32 KB); the other CTA's P (16 KB)
+//   tensor core    Q.K^T of step j+1, P.V of step j with the own keys, P.V with the other CTA's. So the softmax of
+//                  step j has the time of a Q.K^T, and every slot is asked for again 1500 clk or more before it is
+//                  read: a row comes from either die's L2, 1000 to 1500 clk away
+// Both CTAs must weigh a row's keys against one reference m, or their parts of O would not add up. m is a whole
+// number (log2 units), moved only when a score exceeds it by more than the type of P can take (2^64 for bf16, 2^10 for
+// fp16) and in a tile's first step, so P is computed against the m of the step before while a flag from either CTA
+// travels: only if one says so do the two exchange their rows' maxima, move m, rescale O and compute P again.
+//   warps 0-3  one (token, head) row per thread: softmax, exchange, result
 //   warp 4     issues the tensor instructions
-//   warps 5, 7 TMA, one for the other half's ring, one for the other two rings: one box per run of rows that lie in one
-//              page. Q comes the same way, its tensor-memory part through two slots of either of the latter rings
-//   warp 6     clears the rows behind a sequence's end in its last block of V
+//   warps 5, 7 TMA: 5 for the other value half, 7 for the rest, one box per run of rows that lie in one page. Q comes
+//              the same way, its tensor-memory part through a slot of either value ring and the buffer for P
+//   warp 6     clears the rows behind a sequence's end in its last step's value rows
 // Whoever issues tensor or TMA instructions does so in one elected thread, waits included: the operands then sit
 // in uniform registers, and a wait polled by 32 lanes costs some 300 clk more than one polled by a single lane. A
 // TMA instruction takes its thread 65 clk, whatever its box. A wait that is over already still costs 150 to 200 clk
-// while the tensor core keeps shared memory busy, so everything a block loads lands on one barrier: the issuing
-// thread waits three times a block (scores read, rows there, P there); with seven waits it was the bottleneck.
-// The work of a call (tiles x blocks of 64 rows) is cut into equal runs, one for each pair of CTAs, wherever
+// while the tensor core keeps shared memory busy, so what is loaded together lands on one barrier.
+// The work of a call (tiles x steps of 128 rows) is cut into equal runs, one for each pair of CTAs, wherever
 // that cuts a tile; each CTA finds its run itself from q_start and kv_len. Tiles cut by a boundary leave
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
 // Every wait is bounded.
@@ -41,41 +45,49 @@ namespace {
 
 constexpr int kD = 576, kDv = 512, kHalf = 256;
 constexpr int kRows = 128;                     // (token, head) rows per tile
-constexpr int kKeys = 64;                      // cache rows per block
+constexpr int kKeys = 64;                      // cache rows of a CTA in a step
+constexpr int kStep = 2 * kKeys;               // and of both
 constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 128-byte swizzle
-// 64-column tiles of a block: units of the other value half, the rotary columns, own value half
-constexpr int kNTiles = 2, kNUnits = 2, kVTiles = 4, kQTiles = kNTiles * kNUnits;
-constexpr int kNSlots = 3, kRSlots = 2, kVSlots = 3, kAhead = 4;   // no ring reaches further than three blocks ahead
+// 64-column tiles: units of the other value half, own value half
+constexpr int kNTiles = 2, kNUnits = 2, kVTiles = 4;
+// of Q: in shared memory (all of the other value half but its first), in tensor memory (own value half, rotary, that first)
+constexpr int kQTiles = kNTiles * kNUnits - 1, kTTiles = kVTiles + 2;
+constexpr int kVSlots = 2;
 constexpr int kQChunk = kRows * 128;
 constexpr int kThreads = 8 * 32;
 constexpr int kQBox = 16;                      // rows of the small box for Q
-constexpr uint32_t kColO = 0, kColS = 256, kColP = 320, kColQ = 352, kTmemCols = 512;
-constexpr float kRescale = 8.f;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kTmemCols = 512;
+static_assert(kColQ + kTTiles * 32 == kTmemCols, "tensor memory");
 constexpr int kMaxBatch = 16384;
-enum { kWaitN = 211, kWaitNFree, kWaitV, kWaitVFree, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitRead };
+enum { kWaitN = 211, kWaitFree, kWaitV, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitRead, kWaitPeer };
 
 // A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
 struct Seq { int tok, n, len, pos; };
-// Blocks [first, first + count) of 64 cache rows that some row of tile i sees; `units` = max(count, 1) is what
+// Steps [first, first + count) of 128 cache rows that some row of tile i sees; `units` = max(count, 1) is what
 // the tile counts as when the work is divided, so that a tile that sees nothing is still written.
 struct Item { int row0, rows, first, count, units; };
 
 struct __align__(16) Control {
-  // full: by block, the other half's rows, the rotary columns and this half's rows; q_full, q_part: Q's shared and its
-  // tensor-memory part have landed
-  uint64_t full[kAhead], n_empty[kNSlots], r_empty[kRSlots], v_empty[kVSlots], v_land[kVSlots], s_full, s_read, p_full, pv_done,
-      q_ready, q_full, q_part, q_free;
+  // n_full: the other half's rows and the rotary columns; v_full: own half's rows of the own keys (by step), t_full: of the
+  // other CTA's; x_full: the other CTA's P; q_full, q_part: Q's shared and its tensor-memory part. *_land: before clearing.
+  // From the other CTA: x_full, x_first (its buffer may be written: Q came through), flag_full, max_full, sum_full (by
+  // lane quadrant). From both: pv_done
+  uint64_t n_full, n_empty[kNUnits], r_empty, v_full[2], v_empty[kVSlots], v_land[kVSlots], t_full, t_empty, t_land, x_full, x_first,
+      s_full, s_read, p_full, pv_done, q_ready, q_full, q_part, q_free, flag_full[2][4], max_full[4], sum_full[4];
+  float row_max[kRows], row_sum[kRows];         // from the other CTA
+  int flag[2][4];                              // [step parity][lane quadrant] from the other CTA
   long long scan[kThreads / 32], total;
   long long x0, x1, item_x;                    // this pair's run, and where its first tile begins
   int seq, tile;                               // its first tile
   Seq first_seq;
   Item first_item;
-  alignas(16) int pages[2][2][kKeys];          // [producer][block parity]: the pages of a block's boxes
+  alignas(16) int pages[2][2][2][kKeys];       // [producer][step parity][own / other keys]: the pages of the boxes
   uint32_t tmem_base;
   int abort_flag, settled;
 };
-constexpr int kRingBytes = (kNSlots * kNTiles + kRSlots + kVSlots * kVTiles) * kTile;
-constexpr int kSmemBytes = kQTiles * kQChunk + kRingBytes + (int)sizeof(Control) + 1024;
+constexpr int kRingBytes = (kNUnits * kNTiles + 1 + (kVSlots + 1) * kVTiles) * kTile;
+constexpr int kPBytes = kRows * 128;           // P of a CTA: 128 rows x 64 keys
+constexpr int kSmemBytes = kQTiles * kQChunk + kRingBytes + 2 * kPBytes + (int)sizeof(Control) + 1024;
 static_assert(kSmemBytes <= 232448 && (kMaxBatch + 2) * 4 <= kRingBytes, "shared memory");
 
 // What the merge kernel has to know of the tile that a pair ends: its first (token, head) row, its rows, and the pair
@@ -89,7 +101,7 @@ struct Params {
   const int *page_table, *q_start, *kv_len;
   int T, H, batch, max_pages, num_pages, page_size;
   int box, box_log2;                           // rows of a TMA box, all in one page
-  int step_pages, step_rows;                   // 64 rows further = so many pages and rows
+  int step_pages, step_rows;                   // a step further = so many pages and rows
   uint32_t tile_bytes;                         // from one 64-column tile of a part to the next: 8192, or 1024 where the
                                                // tiles of eight rows lie after one another
   int tail;                                    // write the tokens behind the last sequence as such that see nothing
@@ -152,6 +164,25 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A commit that arrives on the same barrier of both CTAs.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(sm100::smem_u32(bar)), "h"((uint16_t)3)
+               : "memory");
+}
+// A word for another CTA, which counts four bytes on its barrier. (An arrival with release semantics at cluster scope
+// takes a thread 1100 clk here.)
+__device__ __forceinline__ void send_word(uint32_t cluster_dst, uint32_t cluster_bar, uint32_t v) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+               ::"r"(cluster_dst), "r"(v), "r"(cluster_bar)
+               : "memory");
+}
+// Copies from this CTA's shared memory to another's; the bytes count on that CTA's barrier when they are there.
+__device__ __forceinline__ void bulk_copy_to(uint32_t cluster_dst, const void* src, uint32_t bytes, uint32_t cluster_bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(cluster_dst), "r"(sm100::smem_u32(src)), "r"(bytes), "r"(cluster_bar)
+               : "memory");
+}
 // One lane of a converged warp, always the same one.
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
@@ -173,9 +204,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Cache rows as (64 columns, row in the page, column tile, page): boxes of 1, 2 and 4 tiles; Q: boxes of 128, 64
+// Cache rows as (64 columns, row in the page, column tile, page): boxes of 1, 2 and 4 tiles; Q: boxes of 128
 // and 16 rows.
-struct Maps { CUtensorMap one, two, four, q, q64, q16; };
+struct Maps { CUtensorMap one, two, four, q, q16; };
 
 __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   Seq s;
@@ -198,8 +229,8 @@ __device__ __forceinline__ Item item_of(const Params& p, const Seq& s, int i) {
   const int t0 = (unsigned)r0 / (unsigned)p.H, t1 = (unsigned)(r0 + t.rows - 1) / (unsigned)p.H;
   const int hi = p.causal ? min(s.len, s.pos + t1 + 1) : s.len;
   const int lo = p.window > 0 ? (int)max(0LL, (long long)s.pos + t0 + 1 - p.window) : 0;
-  t.first = lo / kKeys;
-  t.count = hi > lo ? (hi + kKeys - 1) / kKeys - t.first : 0;
+  t.first = lo / kStep;
+  t.count = hi > lo ? (hi + kStep - 1) / kStep - t.first : 0;
   t.units = max(t.count, 1);
   return t;
 }
@@ -235,7 +266,7 @@ struct Walk {
     t = item_of(p, s, i);
     cut();
   }
-  // blocks of this segment, as block numbers of the sequence
+  // steps of this segment, as step numbers of the sequence
   __device__ __forceinline__ int begin() const { return t.first + u0; }
   __device__ __forceinline__ int blocks() const { return t.count == 0 ? 0 : u1 - u0; }
   __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == t.units; }
@@ -245,6 +276,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   // one lane polls: a try_wait by 32 lanes costs some 300 clk more, which is the time of seven tensor instructions
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = sm100::mbar_wait(bar, parity, abort_flag, status, where);
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
+}
+
+// The same for a barrier on which the other CTA counts `bytes` (0: arrives).
+__device__ __forceinline__ bool warp_wait_peer(uint64_t* bar, uint32_t parity, uint32_t bytes, volatile int* abort_flag, int* status) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) {
+    if (bytes > 0) expect_bytes(sm100::smem_u32(bar), bytes);
+    ok = sm100::mbar_wait_cluster(bar, parity, abort_flag, status, kWaitPeer);
+  }
   ok = __shfl_sync(0xffffffffu, ok, 0);
   __syncwarp();
   return ok != 0;
@@ -396,32 +439,35 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = base;
   uint8_t* n_ring = base + kQTiles * kQChunk;
-  uint8_t* r_ring = n_ring + kNSlots * kNTiles * kTile;
-  uint8_t* v_ring = r_ring + kRSlots * kTile;
-  Control& ctl = *reinterpret_cast<Control*>(v_ring + kVSlots * kVTiles * kTile);
+  uint8_t* r_tile = n_ring + kNUnits * kNTiles * kTile;
+  uint8_t* v_ring = r_tile + kTile;
+  uint8_t* t_tiles = v_ring + kVSlots * kVTiles * kTile;
+  uint8_t* x_tile = t_tiles + kVTiles * kTile;
+  uint8_t* p_tile = x_tile + kPBytes;
+  Control& ctl = *reinterpret_cast<Control*>(p_tile + kPBytes);
   // the same in all lanes, and known to be: the tensor instructions take their operands from uniform registers
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
+  const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;     // half: the rank in the cluster
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kAhead; ++s) sm100::mbar_init(&ctl.full[s], 3);
-    for (int s = 0; s < kNSlots; ++s) sm100::mbar_init(&ctl.n_empty[s], 1);
-    for (int s = 0; s < kRSlots; ++s) sm100::mbar_init(&ctl.r_empty[s], 1);
+    sm100::mbar_init(&ctl.n_full, kNUnits + 1);
+    for (int s = 0; s < kNUnits; ++s) sm100::mbar_init(&ctl.n_empty[s], 1);
+    sm100::mbar_init(&ctl.r_empty, 1);
+    for (int s = 0; s < 2; ++s) sm100::mbar_init(&ctl.v_full[s], 1);
     for (int s = 0; s < kVSlots; ++s) { sm100::mbar_init(&ctl.v_empty[s], 1); sm100::mbar_init(&ctl.v_land[s], 1); }
-    sm100::mbar_init(&ctl.s_full, 1);
-    sm100::mbar_init(&ctl.s_read, 4);
-    sm100::mbar_init(&ctl.p_full, 4);
-    sm100::mbar_init(&ctl.pv_done, 1);
-    sm100::mbar_init(&ctl.q_ready, 4);
-    sm100::mbar_init(&ctl.q_full, 1);
-    sm100::mbar_init(&ctl.q_part, 1);
-    sm100::mbar_init(&ctl.q_free, 1);
+    for (uint64_t* b : {&ctl.t_full, &ctl.t_empty, &ctl.t_land, &ctl.x_full, &ctl.x_first, &ctl.s_full, &ctl.q_full, &ctl.q_part,
+                        &ctl.q_free})
+      sm100::mbar_init(b, 1);
+    sm100::mbar_init(&ctl.pv_done, 2);
+    for (uint64_t* b : {&ctl.s_read, &ctl.p_full, &ctl.q_ready}) sm100::mbar_init(b, 4);
+    for (int s = 0; s < 4; ++s)
+      for (uint64_t* b : {&ctl.flag_full[0][s], &ctl.flag_full[1][s], &ctl.max_full[s], &ctl.sum_full[s]}) sm100::mbar_init(b, 1);
     ctl.abort_flag = 0;
     sm100::mbar_fence_init();
   }
@@ -430,13 +476,14 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     sm100::tmem_relinquish();
   }
   if (warp == 5 && lane == 0) {
-    for (const CUtensorMap* m : {&maps.one, &maps.two, &maps.four, &maps.q, &maps.q64, &maps.q16}) sm100::prefetch_tensormap(m);
+    for (const CUtensorMap* m : {&maps.one, &maps.two, &maps.four, &maps.q, &maps.q16}) sm100::prefetch_tensormap(m);
   }
   cudaGridDependencySynchronize();             // up to here nothing of what earlier work wrote was read
   find_run(p, ctl, reinterpret_cast<int*>(n_ring), pair);
   sm100::fence_proxy_async();                  // the rings were used as scratch
   sm100::tc_fence_before_sync();
   __syncthreads();
+  sm100::cluster_sync_all();                   // both CTAs' barriers exist before anything arrives on them
   sm100::tc_fence_after_sync();
   cudaTriggerProgrammaticLaunchCompletion();   // the merge kernel may be set up; it reads nothing before this grid's end
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);
@@ -445,30 +492,35 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 
   if (warp == 5 || warp == 7) {
     // ---------------------------------------------------------------- loads
-    const int ring = warp == 7;                // 0: the other value half, 1: own half and the rotary columns
+    const int ring = warp == 7;                // 0: the other value half; 1: rotary columns, own value half of all keys
     const int other = half ? 0 : 4;            // first of the four column tiles of the other value half
-    uint32_t at = 0, r_at = 0, g = 0, seg = 0; // slots of ring 0 or of V (with Q), of the rotary ring, blocks, segments
-    uint32_t landed[kVSlots] = {};
+    uint32_t g = 0, seg = 0, v_at = 0, t_at = 0;               // steps, segments, slots of V and uses of T (with Q) so far
+    uint32_t v_landed[kVSlots] = {}, t_landed = 0;
     bool ok = true;
-    const uint32_t n_base = sm100::smem_u32(n_ring), r_base = sm100::smem_u32(r_ring), v_base = sm100::smem_u32(v_ring);
-    // This lane's boxes in a block (two when a box is a single row): pages and rows from the block's first row on.
-    int box_pages[2], box_rows[2], next[2], first_page = 0, first_row = 0;
+    const uint32_t n_base = sm100::smem_u32(n_ring), v_base = sm100::smem_u32(v_ring), t_base = sm100::smem_u32(t_tiles);
+    // Entries lane + 32 k of a list of pages: 64 for the own keys' boxes, 64 for the other CTA's. Where they begin,
+    // counted from the step's first row.
+    int at_pages[4], at_rows[4], next[4], first_page = 0, first_row = 0;
+    auto offset = [&](int k) {                 // in the step; -1: no such box
+      const int e = lane + 32 * k, box = (e & 63) << p.box_log2;
+      return box < kKeys ? ((e < 64) == (half == 0) ? 0 : kKeys) + box : -1;
+    };
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const unsigned off = (unsigned)(lane + 32 * k) << p.box_log2;
-      box_pages[k] = off / (unsigned)p.page_size;
-      box_rows[k] = off % (unsigned)p.page_size;
+    for (int k = 0; k < 4; ++k) {
+      const unsigned off = max(offset(k), 0);
+      at_pages[k] = off / (unsigned)p.page_size;
+      at_rows[k] = off % (unsigned)p.page_size;
     }
-    auto look = [&](const Walk& w, int j) {    // asks for the pages of block j
+    auto look = [&](const Walk& w, int j) {    // asks for the pages of step j
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int off = (lane + 32 * k) << p.box_log2;
-        const int at = first_page + box_pages[k] + (first_row + box_rows[k] >= p.page_size);
-        if (off < kKeys && j * kKeys + off < w.s.len) next[k] = load_now(p.page_table + (size_t)w.b * p.max_pages + at);
+      for (int k = 0; k < 4; ++k) {
+        if (k >= 2 && ring == 0) break;
+        const int off = offset(k), at = first_page + at_pages[k] + (first_row + at_rows[k] >= p.page_size);
+        if (off >= 0 && j * kStep + off < w.s.len) next[k] = load_now(p.page_table + (size_t)w.b * p.max_pages + at);
         else next[k] = 0;
       }
     };
-    auto step = [&]() {                        // to the next block
+    auto step = [&]() {                        // to the next step
       first_page += p.step_pages;
       first_row += p.step_rows;
       if (first_row >= p.page_size) { first_row -= p.page_size; ++first_page; }
@@ -476,173 +528,198 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     auto keep = [&](uint32_t parity) {         // one outside the pool: TMA fills with zeros
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < 4; ++k) {
+        if (k >= 2 && ring == 0) break;
         if ((unsigned)next[k] >= (unsigned)p.num_pages) {
           if (p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
           next[k] = p.num_pages;
         }
-        if (k == 0 || p.box == 1) ctl.pages[ring][parity][lane + 32 * k] = next[k];
+        if (k % 2 == 0 || p.box == 1) ctl.pages[ring][parity][k >> 1][lane + 32 * (k & 1)] = next[k];
       }
       __syncwarp();
     };
     // a slot of a ring, free again for its use number `at`
     auto room = [&](uint64_t* empty, uint32_t slots, uint32_t at) {
-      return at < slots || sm100::mbar_wait(empty + at % slots, (at / slots - 1) & 1, abort_flag, p.status, kWaitNFree);
+      return at < slots || sm100::mbar_wait(empty + at % slots, (at / slots - 1) & 1, abort_flag, p.status, kWaitFree);
+    };
+    // Rows [0, min(64, left)) of a CTA's keys, `tiles` column tiles from `from` on, in boxes that begin at row `row` of page
+    // list[0]
+    auto part = [&](uint32_t dst, uint32_t bar, int from, int tiles, int left, int row, const int* list) {
+      const int boxes = left > 0 ? (min(kKeys, left) + p.box - 1) >> p.box_log2 : 0;
+      expect_bytes(bar, tiles * boxes * p.box * 128);
+      const CUtensorMap* map = p.box < 8 || tiles == 1 ? &maps.one : tiles == 2 ? &maps.two : &maps.four;
+      if (p.box == kKeys) {
+        if (boxes > 0) tma_load_4d(dst, map, bar, 0, row, from, list[0]);
+      } else if (p.box == 8) {                 // boxes of several tiles keep the eight-row groups that swizzling wants
+        const int4 a = *reinterpret_cast<const int4*>(list), b = *reinterpret_cast<const int4*>(list + 4);
+        const int pg[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (e < boxes) tma_load_4d(dst + e * tiles * 1024, map, bar, 0, row, from, pg[e]);
+          row += 8;
+          if (row == p.page_size) row = 0;
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < tiles; ++c) {
+          int r = row;
+#pragma unroll 1
+          for (int e = 0; e < boxes; ++e) {
+            tma_load_4d(dst + c * kTile + e * p.box * 128, map, bar, 0, r, from + c, list[e]);
+            r += p.box;
+            if (r == p.page_size) r = 0;
+          }
+        }
+      }
     };
     for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
       const int nb = w.blocks();
       if (nb == 0) continue;
-      first_page = (unsigned)(w.begin() * kKeys) / (unsigned)p.page_size;
-      first_row = (unsigned)(w.begin() * kKeys) % (unsigned)p.page_size;
+      first_page = (unsigned)(w.begin() * kStep) / (unsigned)p.page_size;
+      first_row = (unsigned)(w.begin() * kStep) % (unsigned)p.page_size;
       look(w, w.begin());
       if (elect_one()) {                       // Q of this tile
         const bool many = w.t.rows > 4 * kQBox;
         const int boxes = many ? 1 : (w.t.rows + kQBox - 1) / kQBox, rows = many ? kRows : kQBox;
         const CUtensorMap* map = many ? &maps.q : &maps.q16;
-        // ring 0: its tiles of Q to where they stay. Ring 1: this half's columns through two value slots (two tiles
-        // each), the rotary ones through two slots of their ring (64 rows each)
-        if (ring == 0)
-          ok = seg == 0 || sm100::mbar_wait(&ctl.q_free, (seg - 1) & 1, abort_flag, p.status, kWaitQ);
-        else
-          ok = room(ctl.r_empty, kRSlots, r_at) && room(ctl.r_empty, kRSlots, r_at + 1) && room(ctl.v_empty, kVSlots, at) &&
-               room(ctl.v_empty, kVSlots, at + 1);
+        // ring 0: its tiles of Q to where they stay. Ring 1: two tiles through T, two through a slot of V, one through
+        // either buffer for P (free when T is, and when the other CTA has read the last P)
+        if (ring == 0) ok = seg == 0 || sm100::mbar_wait(&ctl.q_free, (seg - 1) & 1, abort_flag, p.status, kWaitQ);
+        else ok = room(ctl.v_empty, kVSlots, v_at) && room(&ctl.t_empty, 1, t_at) && room(&ctl.pv_done, 1, g);
         if (ok) {
           const uint32_t bar = sm100::smem_u32(ring == 0 ? &ctl.q_full : &ctl.q_part);
-          expect_bytes(bar, (kVTiles + ring) * boxes * rows * 128);
+          const int tiles = ring == 0 ? kQTiles : kTTiles;
+          expect_bytes(bar, tiles * boxes * rows * 128);
 #pragma unroll 1
-          for (int c = 0; c < kVTiles + ring; ++c) {
+          for (int c = 0; c < tiles; ++c) {
             uint32_t dst = sm100::smem_u32(q_smem) + c * kQChunk;
-            int col = 64 * (other + c), n = boxes, step = rows;
+            int col = 64 * (other + 1 + c);
             if (ring == 1) {
-              dst = v_base + (at + (c >> 1)) % kVSlots * kVTiles * kTile + (c & 1) * kQChunk;
-              col = 64 * (4 - other + c);
-              if (c == kVTiles) {
-                dst = r_base + r_at % kRSlots * kTile;
-                col = kDv;
-                if (many) { map = &maps.q64; n = 2; step = 64; }
-              }
+              dst = c < 2 ? t_base + c * kQChunk : c < kVTiles ? v_base + v_at % kVSlots * kVTiles * kTile + (c - 2) * kQChunk
+                                                               : sm100::smem_u32(x_tile) + (c - kVTiles) * kQChunk;
+              col = c < kVTiles ? 64 * (4 - other + c) : c == kVTiles ? kDv : 64 * other;
             }
 #pragma unroll 1
-            for (int e = 0; e < n; ++e) {
-              if (c == kVTiles && many) dst = r_base + (r_at + e) % kRSlots * kTile;
-              tma_load_2d(dst, map, bar, col, w.t.row0 + e * step);
-              dst += step * 128;
-            }
+            for (int e = 0; e < boxes; ++e) tma_load_2d(dst + e * rows * 128, map, bar, col, w.t.row0 + e * rows);
           }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       ++seg;
-      if (ring == 1) { at += 2; r_at += 2; }
+      ++v_at;
+      ++t_at;
       keep(g & 1);
-      for (int k = 0; k < nb; ++k, ++g) {
-        const int j = w.begin() + k, row0 = first_row;
-        step();
+      // own keys of step k, then (ring 1) the other CTA's of step k - 1: in the order in which their slots become free
+      for (int k = 0; k < nb + ring; ++k) {
+        const int j = w.begin() + k, len = w.s.len;
+        if (k < nb) step();
         if (k + 1 < nb) look(w, j + 1);
         if (elect_one()) {
-          const int left = w.s.len - j * kKeys;
-          const int boxes = (min(kKeys, left) + p.box - 1) >> p.box_log2, bytes = boxes * p.box * 128;
-          const int* list = ctl.pages[ring][g & 1];
-          // page and row of up to eight boxes of eight rows, or of the one box of 64
-          int pg[8], rw[8];
-          if (p.box >= 8) {
-            const int4 a = *reinterpret_cast<const int4*>(list), b = *reinterpret_cast<const int4*>(list + 4);
-            pg[0] = a.x; pg[1] = a.y; pg[2] = a.z; pg[3] = a.w; pg[4] = b.x; pg[5] = b.y; pg[6] = b.z; pg[7] = b.w;
-            rw[0] = row0;
-#pragma unroll
-            for (int e = 1; e < 8; ++e) rw[e] = rw[e - 1] + 8 == p.page_size ? 0 : rw[e - 1] + 8;
-          }
-          // two pieces: the units of ring 0, or the rotary columns and V
-          const uint32_t bar = sm100::smem_u32(&ctl.full[g % kAhead]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const bool rot = ring == 1 && u == 0, val = ring == 1 && u == 1;
-            const uint32_t use = ring == 0 ? at + u : rot ? r_at : at, slots = ring == 0 ? kNSlots : rot ? kRSlots : kVSlots;
-            ok = room(ring == 0 ? ctl.n_empty : rot ? ctl.r_empty : ctl.v_empty, slots, use);
-            if (!ok) break;
-            const int tiles = ring == 0 ? kNTiles : rot ? 1 : kVTiles;
-            const int from = ring == 0 ? other + u * kNTiles : rot ? 8 : 4 - other;
-            const uint32_t s = use % slots;
-            const uint32_t dst = ring == 0 ? n_base + s * kNTiles * kTile : rot ? r_base + s * kTile : v_base + s * kVTiles * kTile;
-            // a last block of V that the sequence does not fill goes to the clearing warp first
-            const bool last = val && left < kKeys;
-            const uint32_t on = last ? sm100::smem_u32(&ctl.v_land[s]) : bar;
-#pragma unroll
-            for (int e = 0; e < kVSlots; ++e) landed[e] += last && s == e;
-            if (ring == 1 || u == 0) expect_bytes(on, (ring == 0 ? kQTiles : tiles) * bytes);
-            const CUtensorMap* map = p.box < 8 || tiles == 1 ? &maps.one : tiles == 2 ? &maps.two : &maps.four;
-            if (p.box == kKeys) {
-              tma_load_4d(dst, map, on, 0, rw[0], from, pg[0]);
-            } else if (p.box == 8) {           // boxes of several tiles keep the eight-row groups that swizzling wants
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (e < boxes) tma_load_4d(dst + e * tiles * 1024, map, on, 0, rw[e], from, pg[e]);
-            } else {
-#pragma unroll 1
-              for (int c = 0; c < tiles; ++c) {
-                int row = row0;
-#pragma unroll 1
-                for (int e = 0; e < boxes; ++e) {
-                  tma_load_4d(dst + c * kTile + e * p.box * 128, map, on, 0, row, from + c, list[e]);
-                  row += p.box;
-                  if (row == p.page_size) row = 0;
-                }
+          // of a CTA's keys in step `at`: how many rows are left from its first one on, and that one's row in its page
+          auto left_of = [&](int at, int rank) { return len - at * kStep - rank * kKeys; };
+          auto row_of = [&](int at, int rank) { return (unsigned)(at * kStep + rank * kKeys) % (unsigned)p.page_size; };
+          if (k < nb) {
+            const int left = left_of(j, half), row = row_of(j, half);
+            const int* list = ctl.pages[ring][g & 1][0];
+            const uint32_t full = sm100::smem_u32(&ctl.n_full);
+            if (ring == 0) {
+              for (int u = 0; u < kNUnits && ok; ++u) {
+                ok = room(&ctl.n_empty[u], 1, g);
+                if (!ok) break;
+                const uint32_t dst = n_base + u * kNTiles * kTile;
+                part(dst, full, other + u * kNTiles, kNTiles, left, row, list);
               }
+            } else {
+              ok = room(&ctl.r_empty, 1, g);
+              if (ok) {
+                part(sm100::smem_u32(r_tile), full, 8, 1, left, row, list);
+                ok = room(ctl.v_empty, kVSlots, v_at);
+              }
+              if (ok) {                        // rows behind the sequence's end: to the clearing warp first
+                const uint32_t s = v_at % kVSlots;
+                const bool tail = left < kKeys;
+#pragma unroll
+                for (int e = 0; e < kVSlots; ++e) v_landed[e] += tail && s == e;
+                part(v_base + s * kVTiles * kTile, sm100::smem_u32(tail ? &ctl.v_land[s] : &ctl.v_full[g & 1]), 4 - other, kVTiles,
+                     left, row, list);
+              }
+            }
+          }
+          if (ring == 1 && ok && k > 0) {
+            const int left = left_of(j - 1, half ^ 1), row = row_of(j - 1, half ^ 1);
+            ok = room(&ctl.t_empty, 1, t_at);
+            if (ok) {
+              const bool tail = left < kKeys;
+              t_landed += tail;
+              part(t_base, sm100::smem_u32(tail ? &ctl.t_land : &ctl.t_full), 4 - other, kVTiles, left, row,
+                   ctl.pages[ring][(g - 1) & 1][1]);
             }
           }
         }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        at += ring == 0 ? kNUnits : 1;
-        r_at += ring;
-        if (k + 1 < nb) keep((g + 1) & 1);
+        if (k > 0) ++t_at;
+        if (k < nb) { ++g; ++v_at; }
+        if (k + 1 < nb) keep(g & 1);
       }
     }
     // Giving up: nothing that is on its way may land after the CTA has ended. The last use of every slot is waited
     // for, with a limit.
-    if (!ok && elect_one()) {                  // counted: what was asked for, and up to a block more
+    if (!ok && elect_one()) {                  // counted: what was asked for, and up to a step more
       int never = 0;
-      // the last `slots` uses before `end` of a ring
-      auto drain = [&](uint64_t* bars, uint32_t slots, uint32_t end) {
-        for (uint32_t i = end > slots ? end - slots : 0; i < end; ++i)
-          sm100::mbar_wait_limited(bars + i % slots, (i / slots) & 1, &never, nullptr, kWaitQ, 20000000LL);
+      auto drain = [&](uint64_t* bar, uint32_t uses) {
+        if (uses > 0) sm100::mbar_wait_limited(bar, (uses - 1) & 1, &never, nullptr, kWaitQ, 20000000LL);
       };
-      drain(ctl.full, kAhead, g + 1);
+      drain(&ctl.n_full, g);
+      drain(&ctl.n_full, g + 1);
       if (ring == 0) {
-        if (seg > 0) drain(&ctl.q_full, 1, seg);
+        drain(&ctl.q_full, seg);
       } else {
-        if (seg > 0) drain(&ctl.q_part, 1, seg);
+        drain(&ctl.q_part, seg);
+        drain(&ctl.t_full, g);
+        drain(&ctl.t_land, t_landed);
+        for (int e = 0; e < 2; ++e) drain(&ctl.v_full[e], (g + 2 - e) / 2);
 #pragma unroll
-        for (int e = 0; e < kVSlots; ++e)
-          if (landed[e]) drain(&ctl.v_land[e], 1, landed[e]);
+        for (int e = 0; e < kVSlots; ++e) drain(&ctl.v_land[e], v_landed[e]);
       }
     }
     __syncwarp();
   } else if (warp == 6) {
     // ---------------------------------------------------------------- rows behind a sequence's end
     // They may hold anything, also NaN, which a weight of zero would keep.
-    uint32_t v_at = 0, g = 0, cleared[kVSlots] = {};
+    uint32_t v_at = 0, g = 0, v_cleared[kVSlots] = {}, t_cleared = 0;
     bool ok = true;
+    const uint32_t group = p.tile_bytes == 1024 ? kVTiles * 1024 : 1024;
+    auto clear = [&](uint8_t* v, int valid) {
+      for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)     // 16 bytes each, 64 to eight rows
+#pragma unroll
+        for (int c = 0; c < kVTiles; ++c)
+          *reinterpret_cast<uint4*>(v + c * p.tile_bytes + (e >> 6) * group + (e & 63) * 16) = make_uint4(0, 0, 0, 0);
+      sm100::fence_proxy_async();
+      __syncwarp();
+    };
     for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
-      if (w.blocks() > 0) v_at += 2;           // Q
-      const int nb = w.blocks(), valid = nb ? w.s.len - (w.begin() + nb - 1) * kKeys : kKeys;
-      if (valid < kKeys) {                     // only a segment's last block can be the sequence's last
+      const int nb = w.blocks();
+      if (nb == 0) continue;
+      ++v_at;                                  // Q
+      // only a segment's last step can be the sequence's last
+      const int left = w.s.len - (w.begin() + nb - 1) * kStep;
+      const int mine = left - half * kKeys, theirs = left - (half ^ 1) * kKeys;
+      if (mine < kKeys) {
         const uint32_t s = (v_at + nb - 1) % kVSlots;
         uint32_t uses = 0;
 #pragma unroll
         for (int e = 0; e < kVSlots; ++e)
-          if (s == e) uses = cleared[e]++;
+          if (s == e) uses = v_cleared[e]++;
         if (!warp_wait(&ctl.v_land[s], uses & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
-        uint8_t* v = v_ring + s * kVTiles * kTile;
-        const uint32_t group = p.tile_bytes == 1024 ? kVTiles * 1024 : 1024;
-        for (int e = valid * 8 + lane; e < kKeys * 8; e += 32)   // 16 bytes each, 64 to eight rows
-#pragma unroll
-          for (int c = 0; c < kVTiles; ++c)
-            *reinterpret_cast<uint4*>(v + c * p.tile_bytes + (e >> 6) * group + (e & 63) * 16) = make_uint4(0, 0, 0, 0);
-        sm100::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&ctl.full[(g + nb - 1) % kAhead]);
+        clear(v_ring + s * kVTiles * kTile, max(mine, 0));
+        if (lane == 0) sm100::mbar_arrive(&ctl.v_full[(g + nb - 1) & 1]);
+      }
+      if (theirs < kKeys) {
+        if (!warp_wait(&ctl.t_land, t_cleared++ & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
+        clear(t_tiles, max(theirs, 0));
+        if (lane == 0) sm100::mbar_arrive(&ctl.t_full);
       }
       v_at += nb;
       g += nb;
@@ -653,15 +730,17 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     if (elect_one()) {
       constexpr uint32_t idesc_qk = sm100::umma_idesc(kFmt, kRows, kKeys);
       constexpr uint32_t idesc_pv = sm100::umma_idesc(kFmt, kRows, kHalf) | (1u << 16);   // V: keys down, columns along
-      // parts of a block, by what the boxes left: tiles of 8 KB, or the tiles of eight rows after one another
+      // rows of a step, by what the boxes left: tiles of 8 KB, or the tiles of eight rows after one another
       const bool by_rows = p.tile_bytes == 1024;
       const uint64_t q_desc = desc_sw128(sm100::smem_u32(q_smem), 16, 1024);
       const uint64_t n_desc = desc_sw128(sm100::smem_u32(n_ring), 16, by_rows ? kNTiles * 1024 : 1024);
-      const uint64_t r_desc = desc_sw128(sm100::smem_u32(r_ring), 16, 1024);
+      const uint64_t r_desc = desc_sw128(sm100::smem_u32(r_tile), 16, 1024);
       const uint32_t v_group = by_rows ? kVTiles * 1024 : 1024, tile = p.tile_bytes >> 4;
       const uint64_t vk_desc = desc_sw128(sm100::smem_u32(v_ring), 16, v_group);
       const uint64_t vn_desc = desc_sw128(sm100::smem_u32(v_ring), p.tile_bytes, v_group);
-      uint32_t n_at = 0, r_at = 0, v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
+      const uint64_t tn_desc = desc_sw128(sm100::smem_u32(t_tiles), p.tile_bytes, v_group);
+      const uint64_t x_desc = desc_sw128(sm100::smem_u32(x_tile), 16, 1024), p_desc = desc_sw128(sm100::smem_u32(p_tile), 16, 1024);
+      uint32_t v_qk = 0, v_pv = 0, g_qk = 0, g_pv = 0, seg = 0;
       bool ok = true;
       for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
         const int nb = w.blocks();
@@ -670,36 +749,38 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             !sm100::mbar_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ))
           break;
         ++seg;
-        for (int h = 0; h < 2; ++h, ++v_qk, ++v_pv, ++r_at) {    // the slots that Q came through were read
-          sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);
-          sm100::mbar_arrive(&ctl.r_empty[r_at % kRSlots]);
-        }
+        sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);        // where Q came through was read
+        sm100::mbar_arrive(&ctl.t_empty);
+        sm100::mbar_arrive_cluster_relaxed(sm100::cluster_map(sm100::smem_u32(&ctl.x_first), half ^ 1));
+        ++v_qk;
+        ++v_pv;
         sm100::tc_fence_after_sync();
+        const uint32_t x_bytes = (w.t.rows + 31) / 32 * 32 * 128;                // what the other CTA's warps send in a step
         for (int k = 0; k <= nb; ++k) {
-          if (k < nb) {                        // S = Q . K^T of block k
-            if (!sm100::mbar_wait(&ctl.full[g_qk % kAhead], (g_qk / kAhead) & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
+          if (k < nb) {                        // S = Q . K^T of step k, own keys
+            if (!sm100::mbar_wait(&ctl.n_full, g_qk & 1, abort_flag, p.status, kWaitN)) { ok = false; break; }
             if (g_qk > 0 && !sm100::mbar_wait(&ctl.s_read, (g_qk - 1) & 1, abort_flag, p.status, kWaitRead)) { ok = false; break; }
             sm100::tc_fence_after_sync();
             const uint32_t d = tmem + kColS;
 #pragma unroll
-            for (int u = 0; u < kNUnits; ++u, ++n_at) {
-              const uint32_t s = n_at % kNSlots;
-              const uint64_t b = n_desc + s * kNTiles * (kTile >> 4);
+            for (int u = 0; u < kNUnits; ++u) {
+              const uint64_t b = n_desc + u * kNTiles * (kTile >> 4);
 #pragma unroll
               for (int c = 0; c < kNTiles; ++c)
 #pragma unroll
-                for (int k4 = 0; k4 < 4; ++k4)
-                  sm100::umma_f16(d, q_desc + (u * kNTiles + c) * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk,
-                                  (u > 0 || c > 0 || k4 > 0) ? 1u : 0u);
-              sm100::umma_commit(&ctl.n_empty[s]);
+                for (int k4 = 0; k4 < 4; ++k4) {
+                  const int t = u * kNTiles + c;
+                  if (t == 0) umma_ts(d, tmem + kColQ + (kTTiles - 1) * 32 + k4 * 8, b + 2 * k4, idesc_qk, k4 > 0 ? 1u : 0u);
+                  else sm100::umma_f16(d, q_desc + (t - 1) * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk, 1u);
+                }
+              sm100::umma_commit(&ctl.n_empty[u]);
             }
-            const uint32_t sr = r_at % kRSlots;
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4)
-              umma_ts(d, tmem + kColQ + kVTiles * 32 + k4 * 8, r_desc + sr * (kTile >> 4) + 2 * k4, idesc_qk, 1u);
-            sm100::umma_commit(&ctl.r_empty[sr]);
-            ++r_at;
+              umma_ts(d, tmem + kColQ + kVTiles * 32 + k4 * 8, r_desc + 2 * k4, idesc_qk, 1u);
+            sm100::umma_commit(&ctl.r_empty);
             const uint32_t s = v_qk % kVSlots;
+            if (!sm100::mbar_wait(&ctl.v_full[g_qk & 1], (g_qk >> 1) & 1, abort_flag, p.status, kWaitV)) { ok = false; break; }
 #pragma unroll
             for (int c = 0; c < kVTiles; ++c) {
               const uint64_t b = vk_desc + s * kVTiles * (kTile >> 4) + c * tile;
@@ -711,16 +792,24 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             ++g_qk;
             ++v_qk;
           }
-          if (k > 0) {                         // O += P . V of block k - 1
+          if (k > 0) {                         // O += P . V of step k - 1: own keys, then the other CTA's
             const uint32_t s = v_pv % kVSlots;
+            expect_bytes(sm100::smem_u32(&ctl.x_full), x_bytes);                   // the last one was waited for
             if (!sm100::mbar_wait(&ctl.p_full, g_pv & 1, abort_flag, p.status, kWaitP)) { ok = false; break; }
             sm100::tc_fence_after_sync();
             const uint64_t b = vn_desc + s * kVTiles * (kTile >> 4);
 #pragma unroll
             for (int k4 = 0; k4 < kKeys / 16; ++k4)
-              umma_ts(tmem + kColO, tmem + kColP + k4 * 8, b + k4 * (v_group >> 3), idesc_pv, (k > 1 || k4 > 0) ? 1u : 0u);
+              sm100::umma_f16(tmem + kColO, p_desc + 2 * k4, b + k4 * (v_group >> 3), idesc_pv, (k > 1 || k4 > 0) ? 1u : 0u);
             sm100::umma_commit(&ctl.v_empty[s]);
-            sm100::umma_commit(&ctl.pv_done);
+            if (!sm100::mbar_wait(&ctl.t_full, g_pv & 1, abort_flag, p.status, kWaitV) ||
+                !sm100::mbar_wait_cluster(&ctl.x_full, g_pv & 1, abort_flag, p.status, kWaitPeer)) { ok = false; break; }
+            sm100::tc_fence_after_sync();
+#pragma unroll
+            for (int k4 = 0; k4 < kKeys / 16; ++k4)
+              sm100::umma_f16(tmem + kColO, x_desc + 2 * k4, tn_desc + k4 * (v_group >> 3), idesc_pv, 1u);
+            sm100::umma_commit(&ctl.t_empty);
+            umma_commit_both(&ctl.pv_done);
             ++g_pv;
             ++v_pv;
           }
@@ -730,30 +819,37 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, one row per thread
+    // weights up to 2^kJump before m moves; it moves to kBias below the maximum (fp16: small weights stay normal numbers)
+    constexpr float kJump = std::is_same_v<T, __half> ? 15.f : 64.f, kBias = std::is_same_v<T, __half> ? 6.f : 0.f;
     const int row = threadIdx.x;
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    uint32_t g = 0, v_at = 0, r_at = 0, seg = 0;   // blocks, value slots, rotary slots and tiles with blocks so far
+    const uint32_t peer = half ^ 1;
+    auto there = [&](const void* mine) { return sm100::cluster_map(sm100::smem_u32(mine), peer); };
+    const uint32_t x_there = there(x_tile) + warp * 32 * 128, x_full_there = there(&ctl.x_full);
+    const uint32_t flag_there = there(&ctl.flag[0][warp]), flag_full_there = there(&ctl.flag_full[0][warp]);
+    const uint32_t max_there = there(&ctl.row_max[row]), max_full_there = there(&ctl.max_full[warp]);
+    const uint32_t sum_there = there(&ctl.row_sum[row]), sum_full_there = there(&ctl.sum_full[warp]);
+    uint32_t g = 0, v_at = 0, seg = 0;         // steps, slots of V and tiles with steps so far
+    uint32_t flags = 0, moves = 0, sums = 0;   // exchanges of this warp so far
     bool ok = true;
     const int own = half * kHalf;
-    // Columns of Q to tensor memory, a row per thread: this half's from two slots of the value ring (two tiles of 64
-    // columns, 128 rows each), the rotary ones from two slots of their ring (64 rows each).
-    auto take_tile = [&](const uint8_t* src, int r, int c) {
-      uint32_t u[32];
-#pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        const uint4 x = *reinterpret_cast<const uint4*>(src + r * 128 + ((v ^ (r & 7)) << 4));
-        u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
-      }
-      tmem_st_32x32(lanes + kColQ + c * 32, u);
-    };
+    // Columns of Q to tensor memory, a row per thread: two tiles of 64 columns from T, two from a slot of V, one from
+    // either buffer for P.
     auto take_q = [&]() {
       if (!warp_wait(&ctl.q_part, seg & 1, abort_flag, p.status, kWaitQ)) { ok = false; return; }
+      const uint8_t* slot = v_ring + v_at % kVSlots * kVTiles * kTile;
 #pragma unroll 1
-      for (int c = 0; c < kVTiles; ++c)
-        take_tile(v_ring + (v_at + (c >> 1)) % kVSlots * kVTiles * kTile + (c & 1) * kQChunk, row, c);
-      take_tile(r_ring + (r_at + (warp >> 1)) % kRSlots * kTile, row & 63, kVTiles);
-      v_at += 2;
-      r_at += 2;
+      for (int c = 0; c < kTTiles; ++c) {
+        const uint8_t* src = (c < 2 ? t_tiles + c * kQChunk : c < kVTiles ? slot + (c - 2) * kQChunk : x_tile + (c - kVTiles) * kQChunk) + row * 128;
+        uint32_t u[32];
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + ((v ^ (row & 7)) << 4));
+          u[4 * v] = x.x; u[4 * v + 1] = x.y; u[4 * v + 2] = x.z; u[4 * v + 3] = x.w;
+        }
+        tmem_st_32x32(lanes + kColQ + c * 32, u);
+      }
+      ++v_at;
       ++seg;
       tmem_st_wait();
       sm100::tc_fence_before_sync();
@@ -771,12 +867,12 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       int hi = p.causal ? min(w.s.len, w.s.pos + tok + 1) : w.s.len;
       const int lo = p.window > 0 ? (int)max(0LL, (long long)w.s.pos + tok + 1 - p.window) : 0;
       if (!live) hi = 0;
-      const bool warp_live = warp * 32 < w.t.rows;
+      const bool warp_live = warp * 32 < w.t.rows;             // the same in both CTAs
       float m_ref = -INFINITY, l_sum = 0.f;
       for (int k = 0; k < nb; ++k, ++g) {
         if (!warp_wait(&ctl.s_full, g & 1, abort_flag, p.status, kWaitS)) { ok = false; break; }
         sm100::tc_fence_after_sync();
-        uint32_t u0[32], u1[32];
+        uint32_t u0[32], u1[32], pk[32];
         if (warp_live) {
           sm100::tmem_ld_32x32(lanes + kColS, u0);
           sm100::tmem_ld_32x32(lanes + kColS + 32, u1);
@@ -784,11 +880,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         }
         sm100::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&ctl.s_read);        // the next block's scores may overwrite them
-        uint32_t pk[32];
+        if (lane == 0) sm100::mbar_arrive(&ctl.s_read);        // the next step's scores may overwrite them
+        bool moved = false;
         float factor = 1.f;
         if (warp_live) {
-          const int key0 = (w.begin() + k) * kKeys;
+          const int key0 = (w.begin() + k) * kStep + half * kKeys;
           if (!__all_sync(0xffffffffu, lo <= key0 && key0 + kKeys <= hi)) {
             const unsigned a = (unsigned)(key0 - lo), span = hi > lo ? (unsigned)(hi - lo) : 0u;
 #pragma unroll
@@ -803,38 +899,63 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             m0 = fmaxf(m0, __uint_as_float(u0[i]));
             m1 = fmaxf(m1, __uint_as_float(u1[i]));
           }
-          const float m_blk = fmaxf(m0, m1) * p.scale_log2;      // scale > 0: the maximum commutes with it
-          if (m_blk > -INFINITY) {
-            if (m_ref == -INFINITY) {
-              m_ref = m_blk;                   // O is zero or not begun: nothing to rescale
-            } else if (m_blk > m_ref + kRescale) {
-              factor = exp2_approx(m_ref - m_blk);
-              m_ref = m_blk;
-            }
+          const float m_own = fmaxf(m0, m1) * p.scale_log2;      // scale > 0: the maximum commutes with it
+          // m has to move if a score exceeds it by too much (any score, as long as there is none)
+          const int jump = __any_sync(0xffffffffu, m_own > m_ref + kJump);
+          if (lane == 0) {
+            expect_bytes(sm100::smem_u32(&ctl.flag_full[flags & 1][warp]), 4);
+            send_word(flag_there + (flags & 1) * 16, flag_full_there + (flags & 1) * 32, jump);
           }
-          const float neg = m_ref == -INFINITY ? 0.f : -m_ref;   // masked scores: exp2(-inf) = 0
-          float s0 = 0.f, s1 = 0.f;
+          float sum;
+          auto weigh = [&]() {
+            const float neg = m_ref == -INFINITY ? 0.f : -m_ref;   // masked scores: exp2(-inf) = 0
+            float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float a = exp2_approx(fmaf(__uint_as_float(u0[i]), p.scale_log2, neg));
-            const float b = exp2_approx(fmaf(__uint_as_float(u0[i + 1]), p.scale_log2, neg));
-            const float c = exp2_approx(fmaf(__uint_as_float(u1[i]), p.scale_log2, neg));
-            const float d = exp2_approx(fmaf(__uint_as_float(u1[i + 1]), p.scale_log2, neg));
-            s0 += a + b;
-            s1 += c + d;
-            // P is rounded to the cache's 16-bit type, the only form the tensor core takes beside it: half a
-            // step of 2^-8 (bf16) or 2^-11 (fp16) per weight, as much as the rounding of the result itself
-            pk[i >> 1] = pack2<T>(a, b);
-            pk[16 + (i >> 1)] = pack2<T>(c, d);
+            for (int i = 0; i < 32; i += 2) {
+              const float a = exp2_approx(fmaf(__uint_as_float(u0[i]), p.scale_log2, neg));
+              const float b = exp2_approx(fmaf(__uint_as_float(u0[i + 1]), p.scale_log2, neg));
+              const float c = exp2_approx(fmaf(__uint_as_float(u1[i]), p.scale_log2, neg));
+              const float d = exp2_approx(fmaf(__uint_as_float(u1[i + 1]), p.scale_log2, neg));
+              s0 += a + b;
+              s1 += c + d;
+              // P is rounded to the cache's 16-bit type, the only form the tensor core takes beside it: half a
+              // step of 2^-8 (bf16) or 2^-11 (fp16) per weight, as much as the rounding of the result itself
+              pk[i >> 1] = pack2<T>(a, b);
+              pk[16 + (i >> 1)] = pack2<T>(c, d);
+            }
+            sum = s0 + s1;
+          };
+          if (!jump) weigh();
+          // two barriers in turn: the other CTA may be a step ahead, not two
+          int jump_there = 0, got = 1;
+          if (lane == 0) {
+            got = sm100::mbar_wait_cluster(&ctl.flag_full[flags & 1][warp], (flags >> 1) & 1, abort_flag, p.status, kWaitPeer);
+            jump_there = *reinterpret_cast<volatile int*>(&ctl.flag[flags & 1][warp]);
           }
-          l_sum = l_sum * factor + (s0 + s1);
+          jump_there = __shfl_sync(0xffffffffu, got ? jump_there : -1, 0);
+          if (jump_there < 0) { ok = false; break; }
+          ++flags;
+          if (jump | jump_there) {             // both CTAs' warps of these rows come here together
+            send_word(max_there, max_full_there, __float_as_uint(m_own));
+            if (!warp_wait_peer(&ctl.max_full[warp], moves & 1, 128, abort_flag, p.status)) { ok = false; break; }
+            ++moves;
+            const float top = fmaxf(m_own, *reinterpret_cast<volatile float*>(&ctl.row_max[row]));
+            if (top > m_ref + kBias) {
+              const float m_new = ceilf(top) - kBias;
+              factor = m_ref == -INFINITY ? 1.f : exp2_approx(m_ref - m_new);     // O is zero or not begun: nothing to rescale
+              m_ref = m_new;
+            }
+            moved = __any_sync(0xffffffffu, factor != 1.f);
+            weigh();
+          }
+          l_sum = l_sum * factor + sum;
         }
-        // P of the block before, and O, are free when its P.V is done (which it mostly is: it follows the scores). Warps
-        // without rows wait as well: an arrival on p_full must not come before the last one was taken.
+        // O and both buffers for P are free when the P.V of the step before is done, here and there (a tile's last one was
+        // waited for). Warps without rows wait as well: an arrival on p_full must not come before the last one was taken.
         if (k > 0 && !warp_wait(&ctl.pv_done, (g - 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
         if (warp_live) {
-          sm100::tc_fence_after_sync();
-          if (__any_sync(0xffffffffu, factor != 1.f)) {        // only from the second block of a segment on
+          if (moved && k > 0) {
+            sm100::tc_fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < kHalf; c += 32) {
               uint32_t o[32];
@@ -844,23 +965,37 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
               tmem_st_32x32(lanes + kColO + c, o);
             }
+            tmem_st_wait();
+            sm100::tc_fence_before_sync();
           }
-          tmem_st_32x32(lanes + kColP, pk);
-          tmem_st_wait();
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(p_tile + row * 128 + ((c ^ (row & 7)) << 4)) =
+                make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+          sm100::fence_proxy_async();
         }
-        sm100::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&ctl.p_full);
+        // the same to the other CTA; in a tile's first step not before Q has come through the buffer there
+        if (k == 0 && !warp_wait_peer(&ctl.x_first, (seg - 1) & 1, 0, abort_flag, p.status)) { ok = false; break; }
+        if (lane == 0 && warp_live) bulk_copy_to(x_there, p_tile + warp * 32 * 128, 32 * 128, x_full_there);
+        __syncwarp();
       }
       if (!ok) break;
       // Q of the next tile may go in as soon as the last scores are out
       Walk nx = w;
       nx.next(p);
       v_at += nb;
-      r_at += nb;
+      if (nb > 0 && warp_live) send_word(sum_there, sum_full_there, __float_as_uint(l_sum));
       if (nx.live() && nx.blocks() > 0) take_q();
       if (!ok) break;
       if (nb > 0) {
+        if (warp_live) {
+          if (!warp_wait_peer(&ctl.sum_full[warp], sums & 1, 128, abort_flag, p.status)) { ok = false; break; }
+          const float theirs = *reinterpret_cast<volatile float*>(&ctl.row_sum[row]);
+          ++sums;
+          l_sum = half == 0 ? l_sum + theirs : theirs + l_sum;
+        }
         if (!warp_wait(&ctl.pv_done, (g - 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
         sm100::tc_fence_after_sync();
       }
@@ -893,7 +1028,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 #pragma unroll 1
           for (int c = 0; c < kHalf; c += 32) {
             uint32_t o[32];
-            sm100::tmem_ld_32x32(lanes + kColO + c, o);          // a cut tile has at least one block in each part
+            sm100::tmem_ld_32x32(lanes + kColO + c, o);          // a cut tile has at least one step in each part
             sm100::tmem_ld_wait();
             if (live) {
 #pragma unroll
@@ -919,12 +1054,15 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     }
   }
 
+  if (ctl.abort_flag) __nanosleep(50000);      // what is on its way to the other CTA lands
   sm100::tc_fence_before_sync();
   __syncthreads();
   if (warp == 4) {
     sm100::tc_fence_after_sync();
     sm100::tmem_dealloc(tmem, kTmemCols);
   }
+  __syncwarp();
+  sm100::cluster_sync_all();                   // nobody writes to a CTA that has ended
 }
 
 // Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own maximum m_k. 128
@@ -1055,7 +1193,7 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.box = box;
   p.box_log2 = 0;
   while ((1 << p.box_log2) < box) ++p.box_log2;
-  p.step_pages = kKeys / batch->page_size; p.step_rows = kKeys % batch->page_size;
+  p.step_pages = kStep / batch->page_size; p.step_rows = kStep % batch->page_size;
   p.tile_bytes = box == 8 ? 1024 : kTile;
   p.causal = causal != 0;
   p.window = window < (long long)batch->max_pages * batch->page_size ? window : 0;   // wider than any history: none
@@ -1086,7 +1224,6 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   };
   if (!make(&maps.one, 1) || !make(&maps.two, 2) || !make(&maps.four, 4)) return CAB_ERR_BAD_ARGUMENT;
   if (!sm100::make_tmap_2d_sw128(&maps.q, q, type, 2, (uint64_t)T * H, kD, kRows, 64) ||
-      !sm100::make_tmap_2d_sw128(&maps.q64, q, type, 2, (uint64_t)T * H, kD, 64, 64) ||
       !sm100::make_tmap_2d_sw128(&maps.q16, q, type, 2, (uint64_t)T * H, kD, kQBox, 64))
     return CAB_ERR_BAD_ARGUMENT;
   if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
