@@ -857,8 +857,13 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       if (lane == 0) sm100::mbar_arrive(&ctl.q_ready);
     };
 
+    // Q of the next tile with steps, if there is one: it goes in as soon as the last scores are out.
+    auto next_q = [&](Walk n) {
+      while (n.live() && n.blocks() == 0) n.next(p);
+      if (n.live()) take_q();
+    };
     Walk w(p, ctl);
-    if (w.live() && w.blocks() > 0) take_q();
+    next_q(w);
     while (w.live() && ok) {
       const int nb = w.blocks();
       // what this row sees: cache rows [lo, hi)
@@ -906,38 +911,43 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             expect_bytes(sm100::smem_u32(&ctl.flag_full[flags & 1][warp]), 4);
             send_word(flag_there + (flags & 1) * 16, flag_full_there + (flags & 1) * 32, jump);
           }
-          float sum;
-          auto weigh = [&]() {
-            const float neg = m_ref == -INFINITY ? 0.f : -m_ref;   // masked scores: exp2(-inf) = 0
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float a = exp2_approx(fmaf(__uint_as_float(u0[i]), p.scale_log2, neg));
-              const float b = exp2_approx(fmaf(__uint_as_float(u0[i + 1]), p.scale_log2, neg));
-              const float c = exp2_approx(fmaf(__uint_as_float(u1[i]), p.scale_log2, neg));
-              const float d = exp2_approx(fmaf(__uint_as_float(u1[i + 1]), p.scale_log2, neg));
-              s0 += a + b;
-              s1 += c + d;
-              // P is rounded to the cache's 16-bit type, the only form the tensor core takes beside it: half a
-              // step of 2^-8 (bf16) or 2^-11 (fp16) per weight, as much as the rounding of the result itself
-              pk[i >> 1] = pack2<T>(a, b);
-              pk[16 + (i >> 1)] = pack2<T>(c, d);
+          float sum = 0.f;
+          // twice at most; a loop, so that its code is there once: the first step waits for code as much as for data
+#pragma unroll 1
+          for (int pass = 0;; ++pass) {
+            if (pass > 0 || !jump) {
+              const float neg = m_ref == -INFINITY ? 0.f : -m_ref;   // masked scores: exp2(-inf) = 0
+              float s0 = 0.f, s1 = 0.f;
+  #pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float a = exp2_approx(fmaf(__uint_as_float(u0[i]), p.scale_log2, neg));
+                const float b = exp2_approx(fmaf(__uint_as_float(u0[i + 1]), p.scale_log2, neg));
+                const float c = exp2_approx(fmaf(__uint_as_float(u1[i]), p.scale_log2, neg));
+                const float d = exp2_approx(fmaf(__uint_as_float(u1[i + 1]), p.scale_log2, neg));
+                s0 += a + b;
+                s1 += c + d;
+                // P is rounded to the cache's 16-bit type, the only form the tensor core takes beside it: half a
+                // step of 2^-8 (bf16) or 2^-11 (fp16) per weight, as much as the rounding of the result itself
+                pk[i >> 1] = pack2<T>(a, b);
+                pk[16 + (i >> 1)] = pack2<T>(c, d);
+              }
+              sum = s0 + s1;
+              if (pass > 0) break;
             }
-            sum = s0 + s1;
-          };
-          if (!jump) weigh();
-          // two barriers in turn: the other CTA may be a step ahead, not two
-          int jump_there = 0, got = 1;
-          if (lane == 0) {
-            got = sm100::mbar_wait_cluster(&ctl.flag_full[flags & 1][warp], (flags >> 1) & 1, abort_flag, p.status, kWaitPeer);
-            jump_there = *reinterpret_cast<volatile int*>(&ctl.flag[flags & 1][warp]);
-          }
-          jump_there = __shfl_sync(0xffffffffu, got ? jump_there : -1, 0);
-          if (jump_there < 0) { ok = false; break; }
-          ++flags;
-          if (jump | jump_there) {             // both CTAs' warps of these rows come here together
+            // two barriers in turn: the other CTA may be a step ahead, not two
+            int jump_there = 0, got = 1;
+            if (lane == 0) {
+              got = sm100::mbar_wait_cluster(&ctl.flag_full[flags & 1][warp], (flags >> 1) & 1, abort_flag, p.status, kWaitPeer);
+              jump_there = *reinterpret_cast<volatile int*>(&ctl.flag[flags & 1][warp]);
+            }
+            jump_there = __shfl_sync(0xffffffffu, got ? jump_there : -1, 0);
+            ok = jump_there >= 0;
+            ++flags;
+            if (!ok || !(jump | jump_there)) break;
+            // both CTAs' warps of these rows come here together
             send_word(max_there, max_full_there, __float_as_uint(m_own));
-            if (!warp_wait_peer(&ctl.max_full[warp], moves & 1, 128, abort_flag, p.status)) { ok = false; break; }
+            ok = warp_wait_peer(&ctl.max_full[warp], moves & 1, 128, abort_flag, p.status);
+            if (!ok) break;
             ++moves;
             const float top = fmaxf(m_own, *reinterpret_cast<volatile float*>(&ctl.row_max[row]));
             if (top > m_ref + kBias) {
@@ -946,8 +956,8 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
               m_ref = m_new;
             }
             moved = __any_sync(0xffffffffu, factor != 1.f);
-            weigh();
           }
+          if (!ok) break;
           l_sum = l_sum * factor + sum;
         }
         // O and both buffers for P are free when the P.V of the step before is done, here and there (a tile's last one was
@@ -982,13 +992,10 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         __syncwarp();
       }
       if (!ok) break;
-      // Q of the next tile may go in as soon as the last scores are out
-      Walk nx = w;
-      nx.next(p);
       v_at += nb;
       if (nb > 0 && warp_live) send_word(sum_there, sum_full_there, __float_as_uint(l_sum));
-      if (nx.live() && nx.blocks() > 0) take_q();
-      if (!ok) break;
+      Walk nx = w;
+      nx.next(p);
       if (nb > 0) {
         if (warp_live) {
           if (!warp_wait_peer(&ctl.sum_full[warp], sums & 1, 128, abort_flag, p.status)) { ok = false; break; }
@@ -999,47 +1006,39 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         if (!warp_wait(&ctl.pv_done, (g - 1) & 1, abort_flag, p.status, kWaitPv)) { ok = false; break; }
         sm100::tc_fence_after_sync();
       }
-      if (warp_live) {
-        const bool any = nb > 0;
-        if (w.whole()) {
-          const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;    // NaN stays NaN
-          const bool zero = l_sum == 0.f;
-          T* dst = static_cast<T*>(p.out) + (size_t)(w.t.row0 + row) * kDv + own;
+      const bool whole = w.whole(), zero = l_sum == 0.f;
+      const float inv = zero ? 0.f : 1.f / l_sum;              // NaN stays NaN
+      const size_t slot = ((size_t)pair * 2 + (w.u0 == 0 ? 1 : 0)) * p.rows_cap + row;
+      T* dst = static_cast<T*>(p.out) + (size_t)(w.t.row0 + row) * kDv + own;
+      float* part = p.part_o + slot * kDv + own;
 #pragma unroll 1
-          for (int c = 0; c < kHalf; c += 32) {
-            uint32_t o[32];
-            if (any) { sm100::tmem_ld_32x32(lanes + kColO + c, o); sm100::tmem_ld_wait(); }
-            if (live) {
+      for (int c = 0; c < kHalf; c += 32) {
+        if (c == kHalf / 2 && nb > 0) next_q(nx);              // by now it is there, and has its tensor cores busy meanwhile
+        if (!ok) break;
+        if (!warp_live) continue;
+        uint32_t o[32];
+        if (nb > 0) { sm100::tmem_ld_32x32(lanes + kColO + c, o); sm100::tmem_ld_wait(); }
+        if (!live) continue;
+        if (whole) {
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t x[4];
+          for (int v = 0; v < 4; ++v) {
+            uint32_t x[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  x[k] = zero ? 0u : pack2<T>(__uint_as_float(o[8 * v + 2 * k]) * inv, __uint_as_float(o[8 * v + 2 * k + 1]) * inv);
-                *reinterpret_cast<uint4*>(dst + c + 8 * v) = make_uint4(x[0], x[1], x[2], x[3]);
-              }
-            }
+            for (int k = 0; k < 4; ++k)
+              x[k] = zero ? 0u : pack2<T>(__uint_as_float(o[8 * v + 2 * k]) * inv, __uint_as_float(o[8 * v + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + c + 8 * v) = make_uint4(x[0], x[1], x[2], x[3]);
           }
-          if (live && half == 0 && p.lse)
-            p.lse[w.t.row0 + row] = zero ? -INFINITY : m_ref * 0.6931471805599453f + logf(l_sum);
-        } else {
-          const size_t slot = (size_t)pair * 2 + (w.u0 == 0 ? 1 : 0);
-          float* dst = p.part_o + (slot * p.rows_cap + row) * kDv + own;
-#pragma unroll 1
-          for (int c = 0; c < kHalf; c += 32) {
-            uint32_t o[32];
-            sm100::tmem_ld_32x32(lanes + kColO + c, o);          // a cut tile has at least one step in each part
-            sm100::tmem_ld_wait();
-            if (live) {
+        } else {                               // a cut tile has at least one step in each part
 #pragma unroll
-              for (int v = 0; v < 8; ++v)
-                *reinterpret_cast<uint4*>(dst + c + 4 * v) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-            }
-          }
-          if (live)
-            *reinterpret_cast<float2*>(p.part_ml + ((slot * 2 + half) * p.rows_cap + row) * 2) = make_float2(m_ref, l_sum);
+          for (int v = 0; v < 8; ++v)
+            *reinterpret_cast<uint4*>(part + c + 4 * v) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
         }
       }
+      if (!ok) break;
+      if (live && whole && half == 0 && p.lse)
+        p.lse[w.t.row0 + row] = zero ? -INFINITY : m_ref * 0.6931471805599453f + logf(l_sum);
+      if (live && !whole)
+        *reinterpret_cast<float2*>(p.part_ml + (((slot - row) * 2 + (size_t)half * p.rows_cap) + row) * 2) = make_float2(m_ref, l_sum);
       sm100::tc_fence_before_sync();           // O was read: the next tile's first P.V comes after these threads' next p_full
       w = nx;
     }
