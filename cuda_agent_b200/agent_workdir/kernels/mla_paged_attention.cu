@@ -119,10 +119,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c1, int c2, int c3, int c4) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
 __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
@@ -204,8 +204,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Cache rows as (64 columns, row in the page, column tile, page): boxes of 1, 2 and 4 tiles; Q: boxes of 128
-// and 16 rows.
+// Cache rows as (64 columns, row of eight, column tile, eight of the page, page), in pages of less than eight rows or
+// an uneven number (64 columns, row, column tile, 1, page): boxes of 1, 2 and 4 tiles; Q: boxes of 128 and 16 rows.
 struct Maps { CUtensorMap one, two, four, q, q16; };
 
 __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
@@ -548,27 +548,16 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       const int boxes = left > 0 ? (min(kKeys, left) + p.box - 1) >> p.box_log2 : 0;
       expect_bytes(bar, tiles * boxes * p.box * 128);
       const CUtensorMap* map = p.box < 8 || tiles == 1 ? &maps.one : tiles == 2 ? &maps.two : &maps.four;
-      if (p.box == kKeys) {
-        if (boxes > 0) tma_load_4d(dst, map, bar, 0, row, from, list[0]);
-      } else if (p.box == 8) {                 // boxes of several tiles keep the eight-row groups that swizzling wants
-        const int4 a = *reinterpret_cast<const int4*>(list), b = *reinterpret_cast<const int4*>(list + 4);
-        const int pg[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e < boxes) tma_load_4d(dst + e * tiles * 1024, map, bar, 0, row, from, pg[e]);
-          row += 8;
-          if (row == p.page_size) row = 0;
-        }
-      } else {
+      // one copy of the instruction, in loops: unrolled over eight boxes it took 1500 clk a part, for two boxes as for eight
+      const int rounds = p.box < 8 ? tiles : 1, bytes = (p.box < 8 ? 1 : tiles) * p.box * 128;
 #pragma unroll 1
-        for (int c = 0; c < tiles; ++c) {
-          int r = row;
+      for (int c = 0; c < rounds; ++c) {
+        int r = row;
 #pragma unroll 1
-          for (int e = 0; e < boxes; ++e) {
-            tma_load_4d(dst + c * kTile + e * p.box * 128, map, bar, 0, r, from + c, list[e]);
-            r += p.box;
-            if (r == p.page_size) r = 0;
-          }
+        for (int e = 0; e < boxes; ++e) {
+          tma_load_5d(dst + c * kTile + e * bytes, map, bar, p.box < 8 ? r : 0, from + c, p.box < 8 ? 0 : r >> 3, list[e]);
+          r += p.box;
+          if (r == p.page_size) r = 0;
         }
       }
     };
@@ -577,6 +566,12 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       if (nb == 0) continue;
       first_page = (unsigned)(w.begin() * kStep) / (unsigned)p.page_size;
       first_row = (unsigned)(w.begin() * kStep) % (unsigned)p.page_size;
+      int own_row = (unsigned)(first_row + half * kKeys) % (unsigned)p.page_size;
+      int their_row = (unsigned)(first_row + (half ^ 1) * kKeys) % (unsigned)p.page_size;
+      auto further = [&](int row) {
+        row += p.step_rows;
+        return row >= p.page_size ? row - p.page_size : row;
+      };
       look(w, w.begin());
       if (elect_one()) {                       // Q of this tile
         const bool many = w.t.rows > 4 * kQBox;
@@ -616,24 +611,20 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         if (k < nb) step();
         if (k + 1 < nb) look(w, j + 1);
         if (elect_one()) {
-          // of a CTA's keys in step `at`: how many rows are left from its first one on, and that one's row in its page
-          auto left_of = [&](int at, int rank) { return len - at * kStep - rank * kKeys; };
-          auto row_of = [&](int at, int rank) { return (unsigned)(at * kStep + rank * kKeys) % (unsigned)p.page_size; };
           if (k < nb) {
-            const int left = left_of(j, half), row = row_of(j, half);
+            const int left = len - j * kStep - half * kKeys;
             const int* list = ctl.pages[ring][g & 1][0];
             const uint32_t full = sm100::smem_u32(&ctl.n_full);
             if (ring == 0) {
-              for (int u = 0; u < kNUnits && ok; ++u) {
-                ok = room(&ctl.n_empty[u], 1, g);
-                if (!ok) break;
-                const uint32_t dst = n_base + u * kNTiles * kTile;
-                part(dst, full, other + u * kNTiles, kNTiles, left, row, list);
+#pragma unroll
+              for (int u = 0; u < kNUnits; ++u) {
+                ok = ok && room(&ctl.n_empty[u], 1, g);
+                if (ok) part(n_base + u * kNTiles * kTile, full, other + u * kNTiles, kNTiles, left, own_row, list);
               }
             } else {
               ok = room(&ctl.r_empty, 1, g);
               if (ok) {
-                part(sm100::smem_u32(r_tile), full, 8, 1, left, row, list);
+                part(sm100::smem_u32(r_tile), full, 8, 1, left, own_row, list);
                 ok = room(ctl.v_empty, kVSlots, v_at);
               }
               if (ok) {                        // rows behind the sequence's end: to the clearing warp first
@@ -642,24 +633,25 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 #pragma unroll
                 for (int e = 0; e < kVSlots; ++e) v_landed[e] += tail && s == e;
                 part(v_base + s * kVTiles * kTile, sm100::smem_u32(tail ? &ctl.v_land[s] : &ctl.v_full[g & 1]), 4 - other, kVTiles,
-                     left, row, list);
+                     left, own_row, list);
               }
             }
           }
           if (ring == 1 && ok && k > 0) {
-            const int left = left_of(j - 1, half ^ 1), row = row_of(j - 1, half ^ 1);
+            const int left = len - (j - 1) * kStep - (half ^ 1) * kKeys;
             ok = room(&ctl.t_empty, 1, t_at);
             if (ok) {
               const bool tail = left < kKeys;
               t_landed += tail;
-              part(t_base, sm100::smem_u32(tail ? &ctl.t_land : &ctl.t_full), 4 - other, kVTiles, left, row,
+              part(t_base, sm100::smem_u32(tail ? &ctl.t_land : &ctl.t_full), 4 - other, kVTiles, left, their_row,
                    ctl.pages[ring][(g - 1) & 1][1]);
             }
           }
         }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (k > 0) ++t_at;
+        own_row = further(own_row);            // of step k + 1, and the other CTA's of step k
+        if (k > 0) { ++t_at; their_row = further(their_row); }
         if (k < nb) { ++g; ++v_at; }
         if (k + 1 < nb) keep(g & 1);
       }
@@ -1183,17 +1175,15 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.page_table = batch->page_table; p.q_start = batch->q_start; p.kv_len = batch->kv_len;
   p.T = T; p.H = H; p.batch = batch->batch; p.tail = tail;
   p.max_pages = batch->max_pages; p.num_pages = batch->num_pages; p.page_size = batch->page_size;
-  // Rows that are sure to lie in one page. 64: a box takes several tiles, each 8 KB. 8: several tiles too, and the
-  // tiles of eight rows lie after one another (eight is what the swizzle repeats after, so 16 and 32 go as 8: fewer
-  // instructions than a box per tile). Below: a box per tile.
+  // Rows that are sure to lie in one page, 64 at most. From eight on (the rows after which swizzling repeats) a box takes
+  // all tiles of a part, and the tiles of eight rows lie after one another; below it is a box per tile.
   int box = 1;
   while (box < kKeys && batch->page_size % (2 * box) == 0) box *= 2;
-  if (box > 8 && box < kKeys) box = 8;
   p.box = box;
   p.box_log2 = 0;
   while ((1 << p.box_log2) < box) ++p.box_log2;
   p.step_pages = kStep / batch->page_size; p.step_rows = kStep % batch->page_size;
-  p.tile_bytes = box == 8 ? 1024 : kTile;
+  p.tile_bytes = box >= 8 ? 1024 : kTile;
   p.causal = causal != 0;
   p.window = window < (long long)batch->max_pages * batch->page_size ? window : 0;   // wider than any history: none
   p.rows_cap = rows_cap_of(T, H);
@@ -1213,12 +1203,15 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   if (!encode) return CAB_ERR_LAUNCH;
   const CUtensorMapDataType type =
       batch->dtype == CAB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const cuuint64_t dims[4] = {64, (cuuint64_t)batch->page_size, kD / 64, (cuuint64_t)batch->num_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)batch->token_stride * 2, 128, (cuuint64_t)batch->page_stride * 2};
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const bool eights = box >= 8;
+  const cuuint64_t dims[5] = {64, (cuuint64_t)(eights ? 8 : batch->page_size), kD / 64, (cuuint64_t)(eights ? batch->page_size / 8 : 1),
+                              (cuuint64_t)batch->num_pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)batch->token_stride * 2, 128, (cuuint64_t)batch->token_stride * 16,
+                                 (cuuint64_t)batch->page_stride * 2};
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
   auto make = [&](CUtensorMap* map, int tiles) {
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, (cuuint32_t)tiles, 1};
-    return encode(map, type, 4, batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint32_t boxes[5] = {64, (cuuint32_t)(eights ? 8 : box), (cuuint32_t)tiles, (cuuint32_t)(eights ? box / 8 : 1), 1};
+    return encode(map, type, 5, batch->rows, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   if (!make(&maps.one, 1) || !make(&maps.two, 2) || !make(&maps.four, 4)) return CAB_ERR_BAD_ARGUMENT;
