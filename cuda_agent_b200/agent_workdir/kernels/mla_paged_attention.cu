@@ -107,8 +107,8 @@ struct Params {
   int tail;                                    // write the tokens behind the last sequence as such that see nothing
   int causal, window, rows_cap, pairs;
   float scale_log2;
-  float* part_o;                               // [pair][2][rows_cap][512]
-  float* part_ml;                              // [pair][2][half][rows_cap][2]
+  float4* part_o;                              // [pair][2][512 / 4 columns][rows_cap]: a warp writes, and the merge reads, whole lines
+  float2* part_ml;                             // [pair][2][rows_cap]
   Meta* meta;                                  // [pair]
   int* status;
 };
@@ -1002,7 +1002,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       const float inv = zero ? 0.f : 1.f / l_sum;              // NaN stays NaN
       const size_t slot = ((size_t)pair * 2 + (w.u0 == 0 ? 1 : 0)) * p.rows_cap + row;
       T* dst = static_cast<T*>(p.out) + (size_t)(w.t.row0 + row) * kDv + own;
-      float* part = p.part_o + slot * kDv + own;
+      float4* part = p.part_o + ((slot - row) * (kDv / 4) + (size_t)(own / 4) * p.rows_cap + row);
 #pragma unroll 1
       for (int c = 0; c < kHalf; c += 32) {
         if (c == kHalf / 2 && nb > 0) next_q(nx);              // by now it is there, and has its tensor cores busy meanwhile
@@ -1023,14 +1023,14 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
         } else {                               // a cut tile has at least one step in each part
 #pragma unroll
           for (int v = 0; v < 8; ++v)
-            *reinterpret_cast<uint4*>(part + c + 4 * v) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            part[(size_t)(c / 4 + v) * p.rows_cap] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                                                                 __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
         }
       }
       if (!ok) break;
       if (live && whole && half == 0 && p.lse)
         p.lse[w.t.row0 + row] = zero ? -INFINITY : m_ref * 0.6931471805599453f + logf(l_sum);
-      if (live && !whole)
-        *reinterpret_cast<float2*>(p.part_ml + (((slot - row) * 2 + (size_t)half * p.rows_cap) + row) * 2) = make_float2(m_ref, l_sum);
+      if (live && !whole && half == 0) p.part_ml[slot] = make_float2(m_ref, l_sum);
       sm100::tc_fence_before_sync();           // O was read: the next tile's first P.V comes after these threads' next p_full
       w = nx;
     }
@@ -1056,45 +1056,45 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   sm100::cluster_sync_all();                   // nobody writes to a CTA that has ended
 }
 
-// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own maximum m_k. 128
-// threads per row, four columns each; the parts' maxima and sums are read side by side, their columns eight at a
-// time, and added in the order of the pairs.
-constexpr int kMergeRows = 4;
+// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own reference m_k. Eight rows
+// and 128 columns a block, four columns a thread; the parts' references and sums are read side by side, their columns
+// eight parts at a time, and added in the order of the pairs.
+constexpr int kMergeRows = 8, kMergeCols = 128;
 template <typename T>
-__global__ void __launch_bounds__(128 * kMergeRows) mla_paged_merge_kernel(const Params p) {
-  __shared__ float2 s_ml[kMergeRows][2][cab::kNumSMs / 2];
+__global__ void __launch_bounds__(kMergeRows * kMergeCols / 4) mla_paged_merge_kernel(const Params p) {
+  __shared__ float2 s_ml[cab::kNumSMs / 2][kMergeRows];
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
-  const int pair = blockIdx.x, sub = threadIdx.x >> 7, tid = threadIdx.x & 127;
+  const int pair = blockIdx.x, sub = threadIdx.x % kMergeRows;
   const Meta m = p.meta[pair];
-  if ((int)blockIdx.y * kMergeRows >= m.rows) return;
-  const int row = blockIdx.y * kMergeRows + sub, parts = pair - m.first + 1;
-  const bool live = row < m.rows;
+  const int row0 = blockIdx.y * kMergeRows, row = row0 + sub, parts = pair - m.first + 1;
+  if (row0 >= m.rows) return;
   auto slot_of = [&](int k) { return (size_t)(m.first + k) * 2 + (k == 0 ? 1 : 0); };
-  if (live)
-    for (int e = tid; e < 2 * parts; e += 128)
-      s_ml[sub][e & 1][e >> 1] = *reinterpret_cast<const float2*>(p.part_ml + ((slot_of(e >> 1) * 2 + (e & 1)) * p.rows_cap + row) * 2);
+  for (int e = threadIdx.x; e < kMergeRows * parts; e += blockDim.x) {
+    const int k = e / kMergeRows, r = row0 + e % kMergeRows;
+    if (r < m.rows) s_ml[k][e % kMergeRows] = p.part_ml[slot_of(k) * p.rows_cap + r];
+  }
   __syncthreads();
-  if (!live) return;
-  const int col = tid * 4, half = col >= kHalf;
-  const float2* ml = s_ml[sub][half];
+  if (row >= m.rows) return;
+  const int col = blockIdx.z * kMergeCols + threadIdx.x / kMergeRows * 4;
   float top = -INFINITY;
   for (int k = 0; k < parts; ++k)
-    if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
+    if (s_ml[k][sub].y != 0.f) top = fmaxf(top, s_ml[k][sub].x);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
   for (int k0 = 0; k0 < parts; k0 += 8) {
     float4 o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (k0 + e < parts) o[e] = __ldcs(reinterpret_cast<const float4*>(p.part_o + (slot_of(k0 + e) * p.rows_cap + row) * kDv + col));
+      if (k0 + e < parts) o[e] = __ldcs(p.part_o + (slot_of(k0 + e) * (kDv / 4) + col / 4) * p.rows_cap + row);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (k0 + e >= parts) break;
-      const float f = ml[k0 + e].y != 0.f ? exp2_approx(ml[k0 + e].x - top) : 0.f;
+      const float2 ml = s_ml[k0 + e][sub];
+      const float f = ml.y != 0.f ? exp2_approx(ml.x - top) : 0.f;
       if (f != 0.f) {                          // also true for NaN
         acc.x += f * o[e].x; acc.y += f * o[e].y; acc.z += f * o[e].z; acc.w += f * o[e].w;
-        l += f * ml[k0 + e].y;
+        l += f * ml.y;
       }
     }
   }
@@ -1104,7 +1104,7 @@ __global__ void __launch_bounds__(128 * kMergeRows) mla_paged_merge_kernel(const
   r.x = zero ? 0u : pack2<T>(acc.x * inv, acc.y * inv);
   r.y = zero ? 0u : pack2<T>(acc.z * inv, acc.w * inv);
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)(m.row0 + row) * kDv + col) = r;
-  if (tid == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
+  if (col == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
 }
 
 constexpr int kPairs = cab::kNumSMs / 2;       // the workspace is sized for this many, a smaller device runs fewer
@@ -1130,8 +1130,8 @@ int launch(Params& p, const Maps& maps, cudaStream_t stream) {
   if (cudaLaunchKernelEx(&cfg, mla_paged_attention_kernel<T>, static_cast<const Params>(p), maps) != cudaSuccess)
     return CAB_ERR_LAUNCH;
   if (p.pairs > 1) {
-    cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows);
-    cfg.blockDim = dim3(128 * kMergeRows);
+    cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows, kDv / kMergeCols);
+    cfg.blockDim = dim3(kMergeRows * kMergeCols / 4);
     cfg.dynamicSmemBytes = 0;
     if (cudaLaunchKernelEx(&cfg, mla_paged_merge_kernel<T>, static_cast<const Params>(p)) != cudaSuccess) return CAB_ERR_LAUNCH;
   }
@@ -1143,7 +1143,7 @@ int launch(Params& p, const Maps& maps, cudaStream_t stream) {
 extern "C" size_t mla_paged_attention_workspace_bytes(int T, int H) {
   if (T <= 0 || H <= 0) return 0;
   const size_t rows = (size_t)kPairs * 2 * rows_cap_of(T, H);
-  return align256(rows * kDv * 4) + align256(rows * 2 * 2 * 4) + align256(kPairs * sizeof(Meta));
+  return align256(rows * kDv * 4) + align256(rows * sizeof(float2)) + align256(kPairs * sizeof(Meta));
 }
 
 extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q, const cab_mla_paged_batch* batch, int T,
@@ -1193,9 +1193,9 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.pairs = sms / 2 < kPairs ? sms / 2 : kPairs;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const size_t rows = (size_t)kPairs * 2 * p.rows_cap;
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float*>(ws + align256(rows * kDv * 4));
-  p.meta = reinterpret_cast<Meta*>(ws + align256(rows * kDv * 4) + align256(rows * 2 * 2 * 4));
+  p.part_o = reinterpret_cast<float4*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + align256(rows * kDv * 4));
+  p.meta = reinterpret_cast<Meta*>(ws + align256(rows * kDv * 4) + align256(rows * sizeof(float2)));
   p.status = status;
 
   Maps maps;
