@@ -485,7 +485,6 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   __syncthreads();
   sm100::cluster_sync_all();                   // both CTAs' barriers exist before anything arrives on them
   sm100::tc_fence_after_sync();
-  cudaTriggerProgrammaticLaunchCompletion();   // the merge kernel may be set up; it reads nothing before this grid's end
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);
   volatile int* abort_flag = &ctl.abort_flag;
   constexpr uint32_t kFmt = std::is_same_v<T, __half> ? 0 : 1;
@@ -897,9 +896,9 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             m1 = fmaxf(m1, __uint_as_float(u1[i]));
           }
           const float m_own = fmaxf(m0, m1) * p.scale_log2;      // scale > 0: the maximum commutes with it
-          // m has to move if a score exceeds it by too much (any score, as long as there is none)
-          const int jump = __any_sync(0xffffffffu, m_own > m_ref + kJump);
-          if (lane == 0) {
+          // m has to move if a score exceeds it by too much, and in the first step, which needs no flag
+          const int jump = k == 0 || __any_sync(0xffffffffu, m_own > m_ref + kJump);
+          if (k > 0 && lane == 0) {
             expect_bytes(sm100::smem_u32(&ctl.flag_full[flags & 1][warp]), 4);
             send_word(flag_there + (flags & 1) * 16, flag_full_there + (flags & 1) * 32, jump);
           }
@@ -926,16 +925,17 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
               sum = s0 + s1;
               if (pass > 0) break;
             }
-            // two barriers in turn: the other CTA may be a step ahead, not two
-            int jump_there = 0, got = 1;
-            if (lane == 0) {
-              got = sm100::mbar_wait_cluster(&ctl.flag_full[flags & 1][warp], (flags >> 1) & 1, abort_flag, p.status, kWaitPeer);
-              jump_there = *reinterpret_cast<volatile int*>(&ctl.flag[flags & 1][warp]);
+            if (k > 0) {                       // two barriers in turn: the other CTA may be a step ahead, not two
+              int jump_there = 0, got = 1;
+              if (lane == 0) {
+                got = sm100::mbar_wait_cluster(&ctl.flag_full[flags & 1][warp], (flags >> 1) & 1, abort_flag, p.status, kWaitPeer);
+                jump_there = *reinterpret_cast<volatile int*>(&ctl.flag[flags & 1][warp]);
+              }
+              jump_there = __shfl_sync(0xffffffffu, got ? jump_there : -1, 0);
+              ok = jump_there >= 0;
+              ++flags;
+              if (!ok || !(jump | jump_there)) break;
             }
-            jump_there = __shfl_sync(0xffffffffu, got ? jump_there : -1, 0);
-            ok = jump_there >= 0;
-            ++flags;
-            if (!ok || !(jump | jump_there)) break;
             // both CTAs' warps of these rows come here together
             send_word(max_there, max_full_there, __float_as_uint(m_own));
             ok = warp_wait_peer(&ctl.max_full[warp], moves & 1, 128, abort_flag, p.status);
@@ -1056,55 +1056,82 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   sm100::cluster_sync_all();                   // nobody writes to a CTA that has ended
 }
 
-// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own reference m_k. Eight rows
-// and 128 columns a block, four columns a thread; the parts' references and sums are read side by side, their columns
-// eight parts at a time, and added in the order of the pairs.
-constexpr int kMergeRows = 8, kMergeCols = 128;
-template <typename T>
-__global__ void __launch_bounds__(kMergeRows * kMergeCols / 4) mla_paged_merge_kernel(const Params p) {
-  __shared__ float2 s_ml[cab::kNumSMs / 2][kMergeRows];
-  cudaTriggerProgrammaticLaunchCompletion();
-  cudaGridDependencySynchronize();
-  const int pair = blockIdx.x, sub = threadIdx.x % kMergeRows;
-  const Meta m = p.meta[pair];
-  const int row0 = blockIdx.y * kMergeRows, row = row0 + sub, parts = pair - m.first + 1;
-  if (row0 >= m.rows) return;
+// Joins the parts of the tile that pair blockIdx.x ends: part k has weights relative to its own reference m_k. A block has
+// eight rows, a thread of it four columns of each of its chunks of 128: all four chunks, or one where the grid has them as z.
+// The parts are added in the order of the pairs. What costs is latency: eight loads are under way before the references
+// and sums are waited for, kParts parts of 8 / kParts chunks.
+constexpr int kMergeRows = 8, kMergeCols = 128, kMergeChunks = kDv / kMergeCols;
+template <typename T, int kParts>
+__device__ __forceinline__ void merge_parts(const Params& p, const Meta& m, float2 (&s_ml)[cab::kNumSMs / 2][kMergeRows]) {
+  constexpr int kChunks = 8 / kParts;
+  const int pair = blockIdx.x, sub = threadIdx.x % kMergeRows, row0 = blockIdx.y * kMergeRows, row = row0 + sub;
+  const int parts = pair - m.first + 1, group = threadIdx.x / kMergeRows;
+  const bool live = row < m.rows;
   auto slot_of = [&](int k) { return (size_t)(m.first + k) * 2 + (k == 0 ? 1 : 0); };
-  for (int e = threadIdx.x; e < kMergeRows * parts; e += blockDim.x) {
-    const int k = e / kMergeRows, r = row0 + e % kMergeRows;
-    if (r < m.rows) s_ml[k][e % kMergeRows] = p.part_ml[slot_of(k) * p.rows_cap + r];
-  }
+  float2 mine = make_float2(0.f, 0.f);         // at most one a thread in the first round, more parts follow below
+  const int e0 = threadIdx.x / kMergeRows;
+  if (e0 < parts && live) mine = p.part_ml[slot_of(e0) * p.rows_cap + row];
+  float4 o[kChunks][kParts];
+  auto load = [&](int c0, int k0) {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+      for (int e = 0; e < kParts; ++e)
+        if (live && k0 + e < parts && c0 + c < kMergeChunks)
+          o[c][e] = __ldcs(p.part_o + (slot_of(k0 + e) * (kDv / 4) + (c0 + c) * (kMergeCols / 4) + group) * p.rows_cap + row);
+  };
+  load(blockIdx.z, 0);
+  if (e0 < parts && live) s_ml[e0][sub] = mine;
+  for (int k = e0 + kMergeCols / 4; k < parts; k += kMergeCols / 4)
+    if (live) s_ml[k][sub] = p.part_ml[slot_of(k) * p.rows_cap + row];
   __syncthreads();
-  if (row >= m.rows) return;
-  const int col = blockIdx.z * kMergeCols + threadIdx.x / kMergeRows * 4;
+  if (!live) return;
   float top = -INFINITY;
   for (int k = 0; k < parts; ++k)
     if (s_ml[k][sub].y != 0.f) top = fmaxf(top, s_ml[k][sub].x);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int k0 = 0; k0 < parts; k0 += 8) {
-    float4 o[8];
+  for (int c0 = blockIdx.z; c0 < kMergeChunks; c0 += gridDim.z * kChunks) {
+    float4 acc[kChunks] = {};
+    float l = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += kParts) {
+      if (c0 != (int)blockIdx.z || k0 > 0) load(c0, k0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k0 + e < parts) o[e] = __ldcs(p.part_o + (slot_of(k0 + e) * (kDv / 4) + col / 4) * p.rows_cap + row);
+      for (int e = 0; e < kParts; ++e) {
+        if (k0 + e >= parts) break;
+        const float2 ml = s_ml[k0 + e][sub];
+        const float f = ml.y != 0.f ? exp2_approx(ml.x - top) : 0.f;
+        if (f != 0.f) {                        // also true for NaN
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (k0 + e >= parts) break;
-      const float2 ml = s_ml[k0 + e][sub];
-      const float f = ml.y != 0.f ? exp2_approx(ml.x - top) : 0.f;
-      if (f != 0.f) {                          // also true for NaN
-        acc.x += f * o[e].x; acc.y += f * o[e].y; acc.z += f * o[e].z; acc.w += f * o[e].w;
-        l += f * ml.y;
+          for (int c = 0; c < kChunks; ++c) {
+            acc[c].x += f * o[c][e].x; acc[c].y += f * o[c][e].y; acc[c].z += f * o[c][e].z; acc[c].w += f * o[c][e].w;
+          }
+          l += f * ml.y;
+        }
       }
     }
+    const bool zero = l == 0.f;
+    const float inv = zero ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (c0 + c >= kMergeChunks) break;
+      uint2 r;
+      r.x = zero ? 0u : pack2<T>(acc[c].x * inv, acc[c].y * inv);
+      r.y = zero ? 0u : pack2<T>(acc[c].z * inv, acc[c].w * inv);
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)(m.row0 + row) * kDv + (c0 + c) * kMergeCols + group * 4) = r;
+    }
+    if (c0 == 0 && group == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  const bool zero = l == 0.f;
-  uint2 r;
-  r.x = zero ? 0u : pack2<T>(acc.x * inv, acc.y * inv);
-  r.y = zero ? 0u : pack2<T>(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)(m.row0 + row) * kDv + col) = r;
-  if (col == 0 && p.lse) p.lse[m.row0 + row] = zero ? -INFINITY : top * 0.6931471805599453f + logf(l);
+}
+template <typename T>
+__global__ void __launch_bounds__(kMergeRows * kMergeCols / 4, 4) mla_paged_merge_kernel(const Params p) {
+  __shared__ float2 s_ml[cab::kNumSMs / 2][kMergeRows];
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
+  const Meta m = p.meta[blockIdx.x];
+  if ((int)blockIdx.y * kMergeRows >= m.rows) return;
+  const int parts = blockIdx.x - m.first + 1;
+  if (gridDim.z > 1 || parts > 4) merge_parts<T, 8>(p, m, s_ml);
+  else if (parts > 2) merge_parts<T, 4>(p, m, s_ml);
+  else merge_parts<T, 2>(p, m, s_ml);
 }
 
 constexpr int kPairs = cab::kNumSMs / 2;       // the workspace is sized for this many, a smaller device runs fewer
@@ -1113,7 +1140,7 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 int rows_cap_of(int T, int H) { return (int)((long long)T * H < kRows ? (long long)T * H : kRows); }
 
 template <typename T>
-int launch(Params& p, const Maps& maps, cudaStream_t stream) {
+int launch(Params& p, const Maps& maps, int sms, cudaStream_t stream) {
   if (!cab::ensure_dynamic_smem<&mla_paged_attention_kernel<T>>(kSmemBytes)) return CAB_ERR_LAUNCH;
   // Either kernel is set up while the one before it ends, and waits for that end itself before it reads or writes
   // anything (cudaGridDependencySynchronize): some 2 us less for a decode step.
@@ -1130,7 +1157,9 @@ int launch(Params& p, const Maps& maps, cudaStream_t stream) {
   if (cudaLaunchKernelEx(&cfg, mla_paged_attention_kernel<T>, static_cast<const Params>(p), maps) != cudaSuccess)
     return CAB_ERR_LAUNCH;
   if (p.pairs > 1) {
-    cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows, kDv / kMergeCols);
+    // A chunk a block where there are so few rows that all their blocks run at once.
+    const long long blocks = ((long long)p.T * p.H + kMergeRows - 1) / kMergeRows;
+    cfg.gridDim = dim3(p.pairs, (p.rows_cap + kMergeRows - 1) / kMergeRows, blocks <= sms ? kMergeChunks : 1);
     cfg.blockDim = dim3(kMergeRows * kMergeCols / 4);
     cfg.dynamicSmemBytes = 0;
     if (cudaLaunchKernelEx(&cfg, mla_paged_merge_kernel<T>, static_cast<const Params>(p)) != cudaSuccess) return CAB_ERR_LAUNCH;
@@ -1219,5 +1248,5 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
       !sm100::make_tmap_2d_sw128(&maps.q16, q, type, 2, (uint64_t)T * H, kD, kQBox, 64))
     return CAB_ERR_BAD_ARGUMENT;
   if (status && cudaMemsetAsync(status, 0, sizeof(int), stream) != cudaSuccess) return CAB_ERR_LAUNCH;
-  return batch->dtype == CAB_F16 ? launch<__half>(p, maps, stream) : launch<__nv_bfloat16>(p, maps, stream);
+  return batch->dtype == CAB_F16 ? launch<__half>(p, maps, sms, stream) : launch<__nv_bfloat16>(p, maps, sms, stream);
 }
