@@ -273,6 +273,26 @@ def test_attention_score_ranges(ext, cuda_device, spread):
     check_attention(ext, (q, cache, table, start, kv))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [1e3, 1e5, 1e7, 1e30])
+def test_attention_scores_beyond_whole_numbers(ext, cuda_device, scale, dtype):
+    """Scores so large that fp32 holds them to whole units or worse: the key that each query repeats wins alone (another
+    key's score is smaller by some 400 of 576, so far more than any rounding; 1e30 times 2^10 stays finite). From 1e5 on
+    its score in powers of two, 8e7 and more, is a whole number, as is the reference: the weight is a power of two and the
+    values come back as they are. At 1e3 it is 8e5 with a fraction f: the weight 2^-f is rounded to the 16-bit type on its
+    way into the product, half a step, and not in the sum that it is divided by, and the result is rounded once more:
+    two half steps, and the fp32 product and quotient (2^-22 is ample)."""
+    q, cache, table, start, kv = make_batch([(7, 300), (2, 150)], 16, 16, dtype, cuda_device, seed=5)
+    picked = torch.randint(0, 140, (9, 16), generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    b = (torch.arange(9, device=cuda_device) >= 7).long()
+    rows = cache[table[b[:, None], picked // 16].long(), picked % 16]
+    out, _ = ext.mla_paged_attention_forward(rows, cache, table, start, kv, scale, check=True)
+    if scale >= 1e5:
+        assert torch.equal(out, rows[..., :512])
+    want = rows[..., :512].double()
+    assert ((out.double() - want).abs() <= want.abs() * ((1 + torch.finfo(dtype).eps / 2) ** 2 - 1 + 2.0 ** -22)).all()
+
+
 def test_attention_nan_and_inf_in_a_query_stay_in_its_row(ext, cuda_device):
     args = make_batch([(6, 200), (1, 150)], 16, 16, torch.bfloat16, cuda_device)
     clean, _ = ext.mla_paged_attention_forward(*args, SCALE)
