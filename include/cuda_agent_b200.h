@@ -381,7 +381,7 @@ int mla_gather_rows_launcher(cab_bf16* rows, const cab_bf16* kv, const int* seq_
 enum cab_dtype { CAB_BF16 = 0, CAB_F16 = 1, CAB_F32 = 2 };
 
 /* Codes that the launchers below leave in *status (device int, may be NULL; it is  */
-/* cleared first). 211 .. 219: a bounded wait gave up.                               */
+/* cleared first). 211 .. 219: a bounded wait gave up. */
 enum cab_paged_status {
   CAB_PAGED_BAD_PAGE = 401,      /* a table entry that is needed lies outside [0, num_pages), or the table row is too short */
   CAB_PAGED_BAD_INDEX = 402,     /* a page or sequence number of a list lies outside its range, or stands there twice */
@@ -389,11 +389,10 @@ enum cab_paged_status {
   CAB_PAGED_NOT_EMPTY = 404      /* a fork's child is in use already: nothing was changed */
 };
 
-/* The new tokens of a batch and the cache they belong to. Sequence b has the new tokens     */
-/* [q_start[b], q_start[b+1]) of the T that a call gets, at positions kv_len[b] - n .. kv_len[b] - 1: */
-/* kv_len counts the new tokens too. Element (page, token, column) of the cache is at          */
-/* rows + page * page_stride + token * token_stride + column (strides in elements, multiples of 8;   */
-/* rows 16-byte aligned).                                                                               */
+/* The new tokens of a batch and the cache they belong to. Sequence b has the new tokens [q_start[b], */
+/* q_start[b+1]) of the T that a call gets, at positions kv_len[b] - n .. kv_len[b] - 1: kv_len counts the */
+/* new tokens too. Element (page, token, column) of the cache is at rows + page * page_stride + token * */
+/* token_stride + column (strides in elements, multiples of 8; rows 16-byte aligned). */
 typedef struct cab_mla_paged_batch {
   void* rows;
   long long page_stride, token_stride;
@@ -405,67 +404,70 @@ typedef struct cab_mla_paged_batch {
   int dtype;                       /* CAB_BF16 or CAB_F16 */
 } cab_mla_paged_batch;
 
-/* Rotary positions on the R columns of each head of x [T, H, R]: with a = positions[t] * freq[i]  */
-/* (radians; turned into a fraction of a turn in 64 bits, so far positions keep their angle),        */
-/*   (x0, x1) -> mscale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a)                                   */
-/* for the pairs (2i, 2i+1) if interleaved, else (i, i + R/2). inverse != 0 turns by -a: that is also    */
-/* the gradient (times the same mscale). A part of a head is a view: strides in elements, the columns     */
-/* contiguous. out may be x itself (same strides); otherwise they must not overlap. R even, <= 2048.       */
-/* dtype: CAB_BF16, CAB_F16 or CAB_F32 for x and out.                                                       */
+/* Rotary positions on the R columns of each head of x [T, H, R]: with a = positions[t] * freq[i] (radians; */
+/* turned into a fraction of a turn in 64 bits, so far positions keep their angle), */
+/*   (x0, x1) -> mscale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a) */
+/* for the pairs (2i, 2i+1) if interleaved, else (i, i + R/2). inverse != 0 turns by -a: that is also the */
+/* gradient (times the same mscale). A part of a head is a view: strides in elements, the columns contiguous. */
+/* out may be x itself (same strides); otherwise they must not overlap. R even, <= 2048. dtype: CAB_BF16, */
+/* CAB_F16 or CAB_F32 for x and out. */
 int mla_rope_launcher(void* out, const void* x, const int* positions, const double* freq, int T, int H, int R,
                       long long x_stride_t, long long x_stride_h, long long out_stride_t, long long out_stride_h,
                       int dtype, int interleaved, int inverse, float mscale, int config, cab_stream_t stream);
 
-/* The new rows of a batch: rotates q_pe [T, H, 64] into q_out (strides as above) and k_pe [T, 64] as     */
-/* mla_rope does (freq [32]), and writes c_kv [T, 512] | rotated k_pe into the page rows of the tokens'     */
-/* positions. Tokens at and after q_start[batch] are left alone. A row whose page is invalid is not         */
-/* written (status CAB_PAGED_BAD_PAGE). H == 0: only the cache is written.                                   */
+/* The new rows of a batch: rotates q_pe [T, H, 64] into q_out (strides as above) and k_pe [T, 64] as */
+/* mla_rope does (freq [32]), and writes c_kv [T, 512] | rotated k_pe into the page rows of the tokens' */
+/* positions. Tokens at and after q_start[batch] are left alone. A row whose page is invalid is not written */
+/* (status CAB_PAGED_BAD_PAGE). H == 0: only the cache is written. */
 int mla_rope_append_launcher(void* q_out, const void* q_pe, const void* c_kv, const void* k_pe,
                              const cab_mla_paged_batch* batch, const double* freq, int T, int H,
                              long long q_out_stride_t, long long q_out_stride_h, long long q_stride_t,
                              long long q_stride_h, long long c_stride_t, long long k_stride_t, int interleaved,
                              float mscale, int* status, int config, cab_stream_t stream);
 
-/* Attention of the new tokens over their sequences' cached rows (their own among them, written before):     */
-/*   out[t,h] = softmax_j(softmax_scale * q[t,h] . row_j) . row_j[:512], lse[t,h] = log of the softmax's sum    */
-/* over the rows j < kv_len[b] with j <= p if causal and j > p - window if window > 0, p the token's position.  */
-/* q [T, H, 576], out [T, H, 512] in the cache's type, lse fp32 [T, H] or NULL. Nothing visible: zeros and       */
-/* -infinity. Rows of the cache at and after kv_len are never used, whatever they hold; an invalid page reads      */
-/* as zeros (status CAB_PAGED_BAD_PAGE), a length beyond max_pages * page_size as that product. One new token per sequence is the decode step. workspace:                  */
-/* mla_paged_attention_workspace_bytes(T, H) bytes, 16-byte aligned, contents irrelevant, not shared by calls that    */
-/* can overlap. softmax_scale > 0. T * H < 2^31, batch <= 16384. Tokens at and after q_start[batch] are left alone;    */
-/* config 256 writes them as tokens that see nothing.                                                                   */
+/* Attention of the new tokens over their sequences' cached rows (their own among them, written before): */
+/*   out[t,h] = softmax_j(softmax_scale * q[t,h] . row_j) . row_j[:512], lse[t,h] = log of the softmax's sum */
+/* over the rows j < kv_len[b] with j <= p if causal and j > p - window if window > 0, p the token's */
+/* position. q [T, H, 576], out [T, H, 512] in the cache's type, lse fp32 [T, H] or NULL. Nothing visible: */
+/* zeros and -infinity. Rows of the cache at and after kv_len are never used, whatever they hold; rows before */
+/* it that a token does not see have weight zero and must be finite; an invalid page reads as zeros (status */
+/* CAB_PAGED_BAD_PAGE), a length beyond max_pages * page_size as that product. One new token per sequence is */
+/* the decode step. workspace: mla_paged_attention_workspace_bytes(T, H) bytes, 16-byte aligned, contents */
+/* irrelevant, not shared by calls that can overlap. softmax_scale > 0. T * H < 2^31, batch <= 16384. Tokens */
+/* at and after q_start[batch] are left alone; config 256 writes them as tokens that see nothing. */
 size_t mla_paged_attention_workspace_bytes(int T, int H);
 int mla_paged_attention_launcher(void* out, float* lse, const void* q, const cab_mla_paged_batch* batch, int T, int H,
                                  float softmax_scale, int causal, int window, void* workspace,
                                  size_t workspace_bytes, int* status, int config, cab_stream_t stream);
 
-/* Page management. `pages` holds num_pages pages of page_bytes in each of `layers` layers, layer l at             */
-/* pages + l * layer_stride (bytes). refcount[num_pages]: how many sequences hold a page; 0 = free. A sequence       */
-/* slot s has length[s] rows, in the first ceil(length / page_size) entries of page_table[s, max_pages]; the           */
-/* entries after them are -1. Free pages are taken lowest number first, in the order of the list and of the              */
-/* positions. extend and fork change everything or nothing. scratch: mla_pages_scratch_bytes(num_pages, n) bytes,           */
-/* 16-byte aligned, contents irrelevant.                                                                                     */
+/* Page management. `pages` holds num_pages pages of page_bytes in each of `layers` layers, layer l at pages */
+/* + l * layer_stride (bytes). refcount[num_pages]: how many sequences hold a page; 0 = free. A sequence slot */
+/* s has length[s] rows, in the first ceil(length / page_size) entries of page_table[s, max_pages]; the */
+/* entries after them are -1. Free pages are taken lowest number first, in the order of the list and of the */
+/* positions. extend and fork change everything or nothing. scratch: mla_pages_scratch_bytes(num_pages, n) */
+/* bytes, 16-byte aligned, contents irrelevant. */
 size_t mla_pages_scratch_bytes(int num_pages, int n);
-/* pages[:, dst[i]] = pages[:, src[i]]. src[i] < 0 or dst[i] < 0 skips the pair. A number beyond the pool, a dst that    */
-/* stands there twice and a dst that is another pair's src skip every pair concerned and raise CAB_PAGED_BAD_INDEX.        */
+/* pages[:, dst[i]] = pages[:, src[i]]. src[i] < 0 or dst[i] < 0 skips the pair. A number beyond the pool, a */
+/* dst that stands there twice and a dst that is another pair's src skip every pair concerned and raise */
+/* CAB_PAGED_BAD_INDEX. */
 int mla_pages_copy_launcher(void* pages, long long layer_stride, int layers, int num_pages, long long page_bytes,
                             const int* src, const int* dst, int n, void* scratch, int* status, int config,
                             cab_stream_t stream);
-/* length[seqs[i]] = new_length[i] with pages for it; a new length below the present one changes nothing.              */
+/* length[seqs[i]] = new_length[i] with pages for it; a new length below the present one changes nothing. */
 int mla_pages_extend_launcher(int* page_table, int* length, int* refcount, int slots, int max_pages, int num_pages,
                               int page_size, const int* seqs, const int* new_length, int n, void* scratch, int* status,
                               int config, cab_stream_t stream);
-/* Sequence dst[i], empty before, becomes a copy of src[i]: full pages are shared, a partly filled last one is copied.  */
+/* Sequence dst[i], empty before, becomes a copy of src[i]: full pages are shared, a partly filled last one */
+/* is copied. */
 int mla_pages_fork_launcher(void* pages, long long layer_stride, int layers, long long page_bytes, int* page_table,
                             int* length, int* refcount, int slots, int max_pages, int num_pages, int page_size,
                             const int* src, const int* dst, int n, void* scratch, int* status, int config,
                             cab_stream_t stream);
-/* Gives back the pages of seqs[i]; a sequence listed twice is freed once.                                               */
+/* Gives back the pages of seqs[i]; a sequence listed twice is freed once. */
 int mla_pages_free_launcher(int* page_table, int* length, int* refcount, int slots, int max_pages, int num_pages,
                             int page_size, const int* seqs, int n, int* status, int config, cab_stream_t stream);
-/* With U pages in use: those numbered U and above move, in ascending order, to the free ones below U; tables and        */
-/* reference counts follow.                                                                                                */
+/* With U pages in use: those numbered U and above move, in ascending order, to the free ones below U; tables */
+/* and reference counts follow. */
 int mla_pages_compact_launcher(void* pages, long long layer_stride, int layers, long long page_bytes, int* page_table,
                                const int* length, int* refcount, int slots, int max_pages, int num_pages, int page_size,
                                void* scratch, int* status, int config, cab_stream_t stream);
