@@ -56,18 +56,23 @@ void check_rows_apart(const torch::Tensor& t, const char* name) {
   TORCH_CHECK(t.numel() == 0 || outer || inner, name, ": rows of the output overlap");
 }
 
+// From the first byte of a view to behind its last: two tensors may share a program's one buffer, but not its bytes.
+std::pair<const char*, const char*> span_of(const torch::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const char* p = static_cast<const char*>(t.data_ptr());
+  return {p, p + (last + 1) * t.element_size()};
+}
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  if (!a.numel() || !b.numel()) return false;
+  const auto x = span_of(a), y = span_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+
 // An output is its input itself, or lies elsewhere.
 void check_apart(const torch::Tensor& out, const torch::Tensor& in, const char* what) {
-  if (!out.numel() || !in.numel() || !out.is_alias_of(in)) return;
+  if (!overlap(out, in)) return;
   if (out.data_ptr() == in.data_ptr() && out.sizes() == in.sizes() && out.strides() == in.strides()) return;
-  auto span = [](const torch::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    const char* p = static_cast<const char*>(t.data_ptr());
-    return std::pair<const char*, const char*>(p, p + (last + 1) * t.element_size());
-  };
-  const auto a = span(out), b = span(in);
-  if (a.second <= b.first || b.second <= a.first) return;
   // two column ranges of the same rows
   bool same = out.dim() == in.dim();
   for (int64_t d = 0; same && d + 1 < out.dim(); ++d) same = out.size(d) <= 1 || in.size(d) <= 1 || out.stride(d) == in.stride(d);
@@ -190,7 +195,7 @@ torch::Tensor mla_rope_append_forward(torch::Tensor q_pe, torch::Tensor c_kv, to
     check_apart(out, q_pe, "q_pe and q_out");
   }
   for (const torch::Tensor* t : {&q_pe, &c_kv, &k_pe, &out})
-    TORCH_CHECK(!t->numel() || !t->is_alias_of(cache), "the new rows and q_out must not lie in the cache's storage");
+    TORCH_CHECK(!overlap(*t, cache), "the new rows and q_out must not overlap the cache");
   torch::Tensor status;
   if (check) status = torch::empty({1}, q_start.options());
   check_status(mla_rope_append_launcher(out.data_ptr(), q_pe.data_ptr(), c_kv.data_ptr(), k_pe.data_ptr(), &batch,
@@ -221,7 +226,8 @@ std::tuple<torch::Tensor, torch::Tensor> mla_paged_attention_forward(
     check_cuda_contig(out, "out", q.scalar_type());
     TORCH_CHECK(out.dim() == 3 && out.size(0) == T && out.size(1) == H && out.size(2) == 512, "out must be [T, H, 512]");
     check_same_device(cache, out, "cache", "out");
-    TORCH_CHECK(!out.numel() || (!out.is_alias_of(q) && !out.is_alias_of(cache)), "out must not share storage with q or the cache");
+    for (const torch::Tensor* t : {&q, &cache, &page_table, &q_start, &kv_len})
+      TORCH_CHECK(!overlap(out, *t), "out must not overlap an input");
   } else {
     out = fresh({T, H, 512}, q, q.scalar_type());
     config |= 256;                             // tokens behind the last sequence: zeros in a fresh output
@@ -232,6 +238,8 @@ std::tuple<torch::Tensor, torch::Tensor> mla_paged_attention_forward(
     TORCH_CHECK(lse.dim() == 2 && lse.size(0) == T && lse.size(1) == H, "lse must be [T, H]");
     check_same_device(cache, lse, "cache", "lse");
     TORCH_CHECK(out_arg.has_value(), "lse is given together with out");
+    for (const torch::Tensor* t : {&q, &cache, &page_table, &q_start, &kv_len, &out})
+      TORCH_CHECK(!overlap(lse, *t), "lse must not overlap out or an input");
   } else {
     lse = out_arg.has_value() ? torch::full({T, H}, -INFINITY, q.options().dtype(torch::kFloat32))
                               : fresh({T, H}, q, torch::kFloat32);
@@ -284,12 +292,18 @@ PoolArgs pool_of(const torch::Tensor& page_table, const torch::Tensor& length, c
   TORCH_CHECK(refcount.dim() == 1 && refcount.numel() > 0, "refcount must be [pages]");
   check_same_device(page_table, length, "page_table", "length");
   check_same_device(page_table, refcount, "page_table", "refcount");
+  TORCH_CHECK(!overlap(page_table, length) && !overlap(page_table, refcount) && !overlap(length, refcount),
+              "page_table, length and refcount must not overlap");
   return {to_int(page_table.size(0), "slots"), to_int(page_table.size(1), "max_pages"), to_int(refcount.size(0), "pages")};
 }
-int list_of(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+// A list is read again after the pool changed, so it must lie outside it.
+int list_of(const torch::Tensor& t, const char* name, std::initializer_list<const torch::Tensor*> pool) {
   check_cuda_contig(t, name, torch::kInt32);
   TORCH_CHECK(t.dim() == 1, name, " must be a list");
-  check_same_device(t, like, name, "the pool");
+  for (const torch::Tensor* part : pool) {
+    check_same_device(t, *part, name, "the pool");
+    TORCH_CHECK(!overlap(t, *part), name, " must not overlap the pool");
+  }
   return to_int(t.size(0), name);
 }
 // On the current device and stream.
@@ -301,8 +315,8 @@ int* status_ptr(const torch::Tensor& t) { return t.defined() ? ptr<int>(t) : nul
 
 torch::Tensor mla_pages_copy(torch::Tensor pages, torch::Tensor src, torch::Tensor dst, bool check) {
   const Pages p = pages_of(pages);
-  const int n = list_of(src, "src", pages);
-  TORCH_CHECK(list_of(dst, "dst", pages) == n, "src and dst must be equally long");
+  const int n = list_of(src, "src", {&pages});
+  TORCH_CHECK(list_of(dst, "dst", {&pages}) == n, "src and dst must be equally long");
   c10::cuda::CUDAGuard guard(pages.device());
   const auto scratch = scratch_for(p.num_pages, n);
   const auto status = status_if(check, pages);
@@ -316,9 +330,8 @@ torch::Tensor mla_pages_copy(torch::Tensor pages, torch::Tensor src, torch::Tens
 void mla_pages_extend(torch::Tensor page_table, torch::Tensor length, torch::Tensor refcount, torch::Tensor seqs,
                       torch::Tensor new_length, int64_t page_size, bool check) {
   const PoolArgs q = pool_of(page_table, length, refcount);
-  const int n = list_of(seqs, "seqs", length);
-  TORCH_CHECK(list_of(new_length, "new_length", length) == n, "seqs and new_length must be equally long");
-  TORCH_CHECK(!new_length.is_alias_of(length), "new_length must not be length itself");
+  const int n = list_of(seqs, "seqs", {&page_table, &length, &refcount});
+  TORCH_CHECK(list_of(new_length, "new_length", {&page_table, &length, &refcount}) == n, "seqs and new_length must be equally long");
   c10::cuda::CUDAGuard guard(length.device());
   const auto scratch = scratch_for(q.num_pages, n);
   const auto status = status_if(check, length);
@@ -336,8 +349,8 @@ void mla_pages_fork(torch::Tensor pages, torch::Tensor page_table, torch::Tensor
   const PoolArgs q = pool_of(page_table, length, refcount);
   TORCH_CHECK(q.num_pages == p.num_pages, "refcount must have an entry for each page");
   check_same_device(pages, length, "pages", "length");
-  const int n = list_of(src, "src", length);
-  TORCH_CHECK(list_of(dst, "dst", length) == n, "src and dst must be equally long");
+  const int n = list_of(src, "src", {&page_table, &length, &refcount, &pages});
+  TORCH_CHECK(list_of(dst, "dst", {&page_table, &length, &refcount, &pages}) == n, "src and dst must be equally long");
   c10::cuda::CUDAGuard guard(length.device());
   const auto scratch = scratch_for(q.num_pages, n);
   const auto status = status_if(check, length);
@@ -352,7 +365,7 @@ void mla_pages_fork(torch::Tensor pages, torch::Tensor page_table, torch::Tensor
 void mla_pages_free(torch::Tensor page_table, torch::Tensor length, torch::Tensor refcount, torch::Tensor seqs,
                     int64_t page_size, bool check) {
   const PoolArgs q = pool_of(page_table, length, refcount);
-  const int n = list_of(seqs, "seqs", length);
+  const int n = list_of(seqs, "seqs", {&page_table, &length, &refcount});
   c10::cuda::CUDAGuard guard(length.device());
   auto status = status_if(check, length);
   check_status(mla_pages_free_launcher(ptr<int>(page_table), ptr<int>(length), ptr<int>(refcount), q.slots, q.max_pages,

@@ -448,3 +448,25 @@ def test_attention_and_append_refusals(ext, cuda_device):
                 lambda: a(q_pe, cache[0, :2, :512], k_pe, cache, table, start, kv, freq)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_attention_outputs_in_one_buffer_with_the_inputs(ext, cuda_device):
+    """Views of one buffer are fine as long as no byte is shared; out or lse over an input, or over each other, is refused."""
+    args = make_batch([(3, 40)], 4, 16, torch.bfloat16, cuda_device)
+    q, T, H = args[0], 3, 4
+    store = torch.zeros(T * H * (576 + 512 + 2), dtype=torch.bfloat16, device=cuda_device)
+    q2 = store[:T * H * 576].view(T, H, 576)
+    out = store[T * H * 576:T * H * 1088].view(T, H, 512)
+    lse = store[T * H * 1088:].view(torch.float32).view(T, H)
+    q2.copy_(q)
+    want, want_lse = ext.mla_paged_attention_forward(*args, SCALE)
+    ext.mla_paged_attention_forward(q2, *args[1:], SCALE, out=out, lse=lse, check=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(q2, q)
+    half = T * H * 512
+    for bad in (dict(out=store[:half].view(T, H, 512)), dict(out=store[T * H * 576 - 8:][:half].view(T, H, 512)),
+                dict(out=args[1].reshape(-1)[:half].view(T, H, 512)),
+                dict(out=out, lse=store[:2 * T * H].view(torch.float32).view(T, H)),
+                dict(out=out, lse=out.view(-1)[:2 * T * H].view(torch.float32).view(T, H))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ext.mla_paged_attention_forward(q2, *args[1:], SCALE, **bad)
+    assert torch.equal(out, want) and torch.equal(q2, q)

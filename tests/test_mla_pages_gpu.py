@@ -280,3 +280,28 @@ def test_pages_refusals(ext, cuda_device):
         with pytest.raises(RuntimeError):
             bad()
     s.check()
+
+
+def test_lists_inside_the_pool_are_refused_and_one_buffer_is_not(ext, cuda_device):
+    """A list that is read again after the table or the lengths changed would no longer say what was checked."""
+    store = torch.zeros(16 + 4 + 12 + 8, dtype=torch.int32, device=cuda_device)
+    table, length, refcount, lists = store[:16].view(4, 4), store[16:20], store[20:32], store[32:]
+    table.fill_(-1)
+    pages = torch.zeros(2, 12, 4, 8, dtype=torch.int32, device=cuda_device)
+    one = ints([0], cuda_device)
+    inside = pages[0, 0, 0]
+    for bad in (lambda: ext.mla_pages_extend(table, length, refcount, length, ints([1, 1, 1, 1], cuda_device), 4),
+                lambda: ext.mla_pages_extend(table, length, refcount, refcount[:1], one, 4),
+                lambda: ext.mla_pages_extend(table, length, refcount, one, table[3, 3:], 4),
+                lambda: ext.mla_pages_extend(table, store[15:19], refcount, one, one, 4),
+                lambda: ext.mla_pages_extend(table, length, store[19:31], one, one, 4),
+                lambda: ext.mla_pages_fork(pages, table, length, refcount, length[:1], one),
+                lambda: ext.mla_pages_fork(pages, table, length, refcount, one, inside[:1]),
+                lambda: ext.mla_pages_copy(pages, one, inside[:1]),
+                lambda: ext.mla_pages_free(table, length, refcount, table[0], 4)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            bad()
+    assert (table == -1).all() and not length.any() and not refcount.any()
+    lists[:2] = ints([2, 7], cuda_device)
+    ext.mla_pages_extend(table, length, refcount, lists[:1], lists[1:2], 4, True)
+    assert table[2].tolist() == [0, 1, -1, -1] and length.tolist() == [0, 0, 7, 0] and refcount[:3].tolist() == [1, 1, 0]
