@@ -274,6 +274,22 @@ def test_attention_score_ranges(ext, cuda_device, spread):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("blocks", ["even", "odd", "any"])
+def test_attention_maxima_that_rise_in_some_blocks(ext, cuda_device, blocks, dtype):
+    """Runs of 64 rows with keys up to 40 times as long: a row's maximum rises far in the keys of one CTA of a pair or of
+    the other, in some lane quadrants and not in others, early and late in a run."""
+    q, cache, table, start, kv = make_batch([(3, 3000), (50, 1500), (1, 130)], 50, 32, dtype, cuda_device, seed=9)
+    g = torch.Generator().manual_seed(3)
+    for b in range(3):
+        for i in range(0, kv[b].item(), 64):
+            long_one = torch.rand((), generator=g).item() < 0.3 and (blocks == "any" or (i // 64) % 2 == (blocks == "odd"))
+            if long_one:
+                for page in table[b, i // 32:min(i // 32 + 2, -(-kv[b].item() // 32))].tolist():
+                    cache[page] *= 1 + 39 * torch.rand((), generator=g).item()
+    check_attention(ext, (q, cache, table, start, kv), scale=SCALE / 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("scale", [1e3, 1e5, 1e7, 1e30])
 def test_attention_scores_beyond_whole_numbers(ext, cuda_device, scale, dtype):
     """Scores so large that fp32 holds them to whole units or worse: the key that each query repeats wins alone (another
