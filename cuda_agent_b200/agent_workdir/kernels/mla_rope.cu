@@ -8,10 +8,10 @@
 // Columns move in 16-byte pieces where pointers, strides and R allow it, else pair by pair. A thread keeps one place
 // in the row and steps through the rows of its CTA, so nothing is divided in the loop; its first rows are asked
 // for before the sines and cosines are made.
-// Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 26.6 us (5.0 TB/s of the 134 MB read and
-// written; a copy of the same strided view 24.7 us); 64 of 128 fp32 columns of 2047 tokens x 16 heads, inverse, 4.2 us; the
-// append of 4096 tokens with 128 heads 36 us (144 MB, 4.0 TB/s: the rows' 128-byte pieces of q and the cache rows at
-// once), of 32 tokens 4.2 us.
+// Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 24.6 us (5.5 TB/s of the 134 MB read and
+// written; a copy of the same strided view takes 24.7 us); 64 of 128 fp32 columns of 2047 tokens x 16 heads, inverse,
+// 4.2 us; the append of 4096 tokens with 128 heads 33 us (144 MB, 4.3 TB/s: the heads' 128-byte pieces of q and the cache
+// rows at once), of 32 tokens 4.2 us.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -313,11 +313,13 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   w.rest(cs);
 }
 
-// Tokens and heads per CTA: about 1024 units (four a thread), fewer where the call is too small to fill the device.
+// Tokens and heads per CTA: about 4096 units (sixteen a thread), fewer where the call is too small to fill the device. (With
+// four a thread the angles, and an append's look into the tables, are waited for too often: 26.7 and 36.9 us for the two
+// large calls above instead of 24.6 and 33.4.)
 void split(RopeParams& p, int units_per_head, dim3& grid) {
   const int half = p.R / 2;
   const long long per_token = (long long)(p.H > 0 ? p.H : 1) * units_per_head;
-  long long tokens = 4 * kThreads / per_token;
+  long long tokens = 16 * kThreads / per_token;
   const long long most = kAngles / half < 1 ? 1 : kAngles / half;
   if (tokens > most) tokens = most;
   const long long fill = ((long long)p.T + 4 * cab::kNumSMs - 1) / (4 * cab::kNumSMs);
