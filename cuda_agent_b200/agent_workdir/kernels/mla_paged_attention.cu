@@ -189,6 +189,8 @@ __device__ __forceinline__ void bulk_copy_to(uint32_t cluster_dst, const void* s
                ::"r"(cluster_dst), "r"(sm100::smem_u32(src)), "r"(bytes), "r"(cluster_bar)
                : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // One lane of a converged warp, always the same one.
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
@@ -224,6 +226,7 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   s.pos = s.len - s.n;
   return s;
 }
+__device__ __forceinline__ bool descends(const Params& p, int b) { return __ldg(p.q_start + b) > __ldg(p.q_start + b + 1); }
 __device__ __forceinline__ int tiles_of(const Params& p, int n) {
   return (int)(((unsigned)n * (unsigned)p.H + kRows - 1) / kRows);    // T * H < 2^31
 }
@@ -353,7 +356,8 @@ __device__ __forceinline__ void found(const Params& p, Control& ctl, const Run& 
 
 // Where pair `pair` begins: thread-parallel over the sequences, then over the tiles. `pre`: batch + 1 ints of
 // shared memory that nothing else uses yet. A decode step of up to 32 sequences (no more than eight tiles each) is
-// settled by one warp without barriers, 1000 clk sooner.
+// settled by one warp without barriers, 1000 clk sooner. Starts that descend would give the same tokens to several
+// sequences, without end: nothing is done then.
 __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
   const int tid = threadIdx.x;
   if (p.batch <= 32) {
@@ -361,7 +365,9 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
     if (tid < 32) {
       Seq s{0, 0, 0, 0};
       if (tid < p.batch) s = seq_of(p, tid);
-      const int tiles = tiles_of(p, s.n);
+      const bool bad = __any_sync(0xffffffffu, tid < p.batch && descends(p, tid));
+      if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_INDEX);
+      const int tiles = bad ? 0 : tiles_of(p, s.n);
       done = __all_sync(0xffffffffu, tiles <= 8);
       if (done) {
         int sum = 0;
@@ -394,8 +400,14 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
   {
     const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
     long long sum = 0;
-    for (int b = b0; b < b1; ++b) sum += tiles_of(p, seq_of(p, b).n);
-    long long at = block_scan(ctl, sum);
+    bool bad = false;
+    for (int b = b0; b < b1; ++b) {
+      bad |= descends(p, b);
+      sum += tiles_of(p, seq_of(p, b).n);
+    }
+    bad = __syncthreads_or(bad);
+    if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_INDEX);
+    long long at = block_scan(ctl, bad ? 0 : sum);
     for (int b = b0; b < b1; ++b) {
       pre[b] = (int)min(at, (long long)0x7fffffff);
       at += tiles_of(p, seq_of(p, b).n);
@@ -489,7 +501,8 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
   sm100::fence_proxy_async();                  // the rings were used as scratch
   sm100::tc_fence_before_sync();
   __syncthreads();
-  sm100::cluster_sync_all();                   // both CTAs' barriers exist before anything arrives on them
+  cluster_arrive();                            // both CTAs' barriers exist before anything of the other's arrives on them
+  if (warp <= 4) cluster_wait();
   sm100::tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);
   volatile int* abort_flag = &ctl.abort_flag;
@@ -1074,6 +1087,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     sm100::tmem_dealloc(tmem, kTmemCols);
   }
   __syncwarp();
+  if (warp > 4) cluster_wait();
   sm100::cluster_sync_all();                   // nobody writes to a CTA that has ended
 }
 

@@ -384,7 +384,8 @@ enum cab_dtype { CAB_BF16 = 0, CAB_F16 = 1, CAB_F32 = 2 };
 /* cleared first). 211 .. 219: a bounded wait gave up. */
 enum cab_paged_status {
   CAB_PAGED_BAD_PAGE = 401,      /* a table entry that is needed lies outside [0, num_pages), or the table row is too short */
-  CAB_PAGED_BAD_INDEX = 402,     /* a page or sequence number of a list lies outside its range, or stands there twice */
+  CAB_PAGED_BAD_INDEX = 402,     /* a page or sequence number of a list lies outside its range, or stands there twice; */
+                                 /* attention: q_start descends, nothing was computed                                  */
   CAB_PAGED_NO_ROOM = 403,       /* too few free pages, or a sequence longer than a table row: nothing was changed */
   CAB_PAGED_NOT_EMPTY = 404      /* a fork's child is in use already: nothing was changed */
 };

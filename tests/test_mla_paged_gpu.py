@@ -486,3 +486,18 @@ def test_attention_outputs_in_one_buffer_with_the_inputs(ext, cuda_device):
         with pytest.raises(RuntimeError, match="overlap"):
             ext.mla_paged_attention_forward(q2, *args[1:], SCALE, **bad)
     assert torch.equal(out, want) and torch.equal(q2, q)
+
+
+@pytest.mark.parametrize("batch", [3, 32, 40, 500])
+def test_attention_with_starts_that_descend_does_nothing(ext, cuda_device, batch):
+    """They would give tokens to several sequences at once. The outputs stay as they were, and the next call is sound."""
+    args = make_batch([(2, 40)] * batch, 4, 16, torch.bfloat16, cuda_device)
+    q, cache, table, start, kv = args
+    wrong = start.clone()
+    wrong[batch // 2] = 2 * batch
+    out = torch.full((2 * batch, 4, 512), 7.0, dtype=q.dtype, device=cuda_device)
+    lse = torch.full((2 * batch, 4), 7.0, device=cuda_device)
+    with pytest.raises(RuntimeError, match="q_start descends"):
+        ext.mla_paged_attention_forward(q, cache, table, wrong, kv, SCALE, out=out, lse=lse, check=True)
+    assert (out == 7).all() and (lse == 7).all()
+    check_attention(ext, args)
