@@ -56,7 +56,7 @@ constexpr int kStep = 2 * kKeys;               // and of both
 constexpr int kTile = kKeys * 128;             // 64 cache rows x 64 columns, 128-byte swizzle
 // 64-column tiles: units of the other value half, own value half
 constexpr int kNTiles = 2, kNUnits = 2, kVTiles = 4;
-// of Q: in shared memory (all of the other value half but its first), in tensor memory (own value half, rotary, that first)
+// of Q: in shared memory (all of the other value half but its last), in tensor memory (own value half, rotary, that last)
 constexpr int kQTiles = kNTiles * kNUnits - 1, kTTiles = kVTiles + 2;
 constexpr int kVSlots = 2;
 constexpr int kQChunk = kRows * 128;
@@ -606,11 +606,11 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
 #pragma unroll 1
           for (int c = 0; c < tiles; ++c) {
             uint32_t dst = sm100::smem_u32(q_smem) + c * kQChunk;
-            int col = 64 * (other + 1 + c);
+            int col = 64 * (other + c);
             if (ring == 1) {
               dst = c < 2 ? t_base + c * kQChunk : c < kVTiles ? v_base + v_at % kVSlots * kVTiles * kTile + (c - 2) * kQChunk
                                                                : sm100::smem_u32(x_tile) + (c - kVTiles) * kQChunk;
-              col = c < kVTiles ? 64 * (4 - other + c) : c == kVTiles ? kDv : 64 * other;
+              col = c < kVTiles ? 64 * (4 - other + c) : c == kVTiles ? kDv : 64 * (other + kQTiles);
             }
 #pragma unroll 1
             for (int e = 0; e < boxes; ++e) tma_load_2d(dst + e * rows * 128, map, bar, col, w.t.row0 + e * rows);
@@ -755,16 +755,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       for (Walk w(p, ctl); w.live() && ok; w.next(p)) {
         const int nb = w.blocks();
         if (nb == 0) continue;
-        if (!sm100::mbar_wait(&ctl.q_full, seg & 1, abort_flag, p.status, kWaitQ) ||
-            !sm100::mbar_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ))
-          break;
-        ++seg;
-        sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);        // where Q came through was read
-        sm100::mbar_arrive(&ctl.t_empty);
-        sm100::mbar_arrive_cluster_relaxed(sm100::cluster_map(sm100::smem_u32(&ctl.x_first), half ^ 1));
-        ++v_qk;
-        ++v_pv;
-        sm100::tc_fence_after_sync();
+        if (!sm100::mbar_wait(&ctl.q_full, seg & 1, abort_flag, p.status, kWaitQ)) break;
         const uint32_t x_bytes = (w.t.rows + 31) / 32 * 32 * 128;                // what the other CTA's warps send in a step
         for (int k = 0; k <= nb; ++k) {
           if (k < nb) {                        // S = Q . K^T of step k, own keys
@@ -776,15 +767,31 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
             for (int u = 0; u < kNUnits; ++u) {
               const uint64_t b = n_desc + u * kNTiles * (kTile >> 4);
 #pragma unroll
-              for (int c = 0; c < kNTiles; ++c)
+              for (int c = 0; c < kNTiles; ++c) {
+                if (u * kNTiles + c == kQTiles && k == 0) {        // the rest of Q: the parts before it did not need it
+                  ok = sm100::mbar_wait(&ctl.q_ready, seg & 1, abort_flag, p.status, kWaitQ);
+                  if (!ok) break;
+                  ++seg;
+                  sm100::mbar_arrive(&ctl.v_empty[v_qk % kVSlots]);        // where Q came through was read
+                  sm100::mbar_arrive(&ctl.t_empty);
+                  sm100::mbar_arrive_cluster_relaxed(sm100::cluster_map(sm100::smem_u32(&ctl.x_first), half ^ 1));
+                  ++v_qk;
+                  ++v_pv;
+                  sm100::tc_fence_after_sync();
+                }
 #pragma unroll
                 for (int k4 = 0; k4 < 4; ++k4) {
                   const int t = u * kNTiles + c;
-                  if (t == 0) umma_ts(d, tmem + kColQ + (kTTiles - 1) * 32 + k4 * 8, b + 2 * k4, idesc_qk, k4 > 0 ? 1u : 0u);
-                  else sm100::umma_f16(d, q_desc + (t - 1) * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk, 1u);
+                  if (t < kQTiles)
+                    sm100::umma_f16(d, q_desc + t * (kQChunk >> 4) + 2 * k4, b + c * tile + 2 * k4, idesc_qk, t > 0 || k4 > 0 ? 1u : 0u);
+                  else
+                    umma_ts(d, tmem + kColQ + (kTTiles - 1) * 32 + k4 * 8, b + c * tile + 2 * k4, idesc_qk, 1u);
                 }
+              }
+              if (!ok) break;
               sm100::umma_commit(&ctl.n_empty[u]);
             }
+            if (!ok) break;
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4)
               umma_ts(d, tmem + kColQ + kVTiles * 32 + k4 * 8, r_desc + 2 * k4, idesc_qk, 1u);
