@@ -14,11 +14,14 @@
 //   shared memory  the other 192 columns of Q (48 KB); of the own keys the other value half in two units of 128
 //                  columns (16 KB each), the rotary columns (8 KB) and the own value half (32 KB, two slots); of the
 //                  other CTA's keys the own value half (32 KB); P of either CTA's keys (16 KB each)
-//   tensor core    Q.K^T of step j+1, P.V of step j with the own keys, P.V with the other CTA's: 2900 clk together. So
-//                  the softmax of step j has the time of a Q.K^T, and every slot is asked for again 1500 clk or more
-//                  before it is read: a row comes from either die's L2, 1000 to 1500 clk away
+//   tensor core    Q.K^T of step j+1, P.V of step j with the own keys, P.V with the other CTA's. So the softmax of
+//                  step j has the time of a Q.K^T, and every slot is asked for again 1500 clk or more before it is
+//                  read: a row comes from either die's L2, 1000 to 1500 clk away
+// What bounds a step is shared memory: operands 216 KB, loads 104 KB, P 48 KB are 2940 clk at 128 bytes a clk, of 3150;
+// the tensor core alone would take 2050.
 // P goes to shared memory, where the tensor core reads it and a bulk copy takes it to the other CTA. (Written there by
 // the threads it arrived 2000 clk later: stores to another CTA of 16 bytes a row are slow, and so are the fences.)
+// A tile's first scores begin with the columns of Q in shared memory, while the others are on their way to tensor memory.
 // Both CTAs must weigh a row's keys against one reference m, or their parts of O would not add up. m is a whole
 // number (log2 units) that moves only in a tile's first step and when a score exceeds it by more than kJump, so P is
 // computed against the m of the step before while a flag from either CTA travels: only if one says so do the two
@@ -37,8 +40,8 @@
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
 // Every wait is bounded.
 // Measured, 128 heads, bf16, pages of 64: 1024 tokens after 7168 rows 1.78 ms (1235 TFLOP/s; 1.92 ms at the power limit,
-// 1.6 GHz); 64 sequences of 8192 rows and less, one token each, 123 us (3.0 TB/s of the cache: a step waits for its rows,
-// the merge is 13 us of it). 32 sequences of 4096 rows and less, 5 tokens with 24 heads, pages of 16: 49 us. One token
+// 1.6 GHz); 64 sequences of 8192 rows and less, one token each, 119 to 129 us on different boxes (3 TB/s of the cache: a
+// step waits for its rows, the merge is 13 us of it). 32 sequences of 4096 rows and less, 5 tokens with 24 heads, pages of 16: 49 us. One token
 // with 16 heads and 1000 rows: 15 us, set-up and latency.
 #include <cuda_fp16.h>
 

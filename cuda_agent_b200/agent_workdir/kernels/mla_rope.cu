@@ -8,9 +8,9 @@
 // Columns move in 16-byte pieces where pointers, strides and R allow it, else pair by pair. A thread keeps one place
 // in the row and steps through the rows of its CTA, so nothing is divided in the loop; its first rows are asked
 // for before the sines and cosines are made.
-// Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 24.6 us (5.5 TB/s of the 134 MB read and
+// Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 26.6 us (5.0 TB/s of the 134 MB read and
 // written; a copy of the same strided view takes 24.7 us); 64 of 128 fp32 columns of 2047 tokens x 16 heads, inverse,
-// 4.2 us; the append of 4096 tokens with 128 heads 33 us (144 MB, 4.3 TB/s: the heads' 128-byte pieces of q and the cache
+// 4.2 us; the append of 4096 tokens with 128 heads 32.9 us (144 MB, 4.4 TB/s: the heads' 128-byte pieces of q and the cache
 // rows at once), of 32 tokens 4.2 us.
 #include <cuda_fp16.h>
 
@@ -313,13 +313,14 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   w.rest(cs);
 }
 
-// Tokens and heads per CTA: about 4096 units (sixteen a thread), fewer where the call is too small to fill the device. (With
-// four a thread the angles, and an append's look into the tables, are waited for too often: 26.7 and 36.9 us for the two
-// large calls above instead of 24.6 and 33.4.)
-void split(RopeParams& p, int units_per_head, dim3& grid) {
+// Tokens and heads per CTA: about `each` units a thread, fewer where the call is too small to fill the device. An append takes
+// eight, so that its look into the tables is waited for less often (the large call above takes 32.9 us, with four 36.9, with
+// sixteen 33.5). The rotation alone takes four: on rows that another kernel or call just touched 26.6 us, with eight
+// 27.4, with sixteen 28.5 (on rows that are nowhere near, 34.4, 33.6 and 31.4).
+void split(RopeParams& p, int units_per_head, int each, dim3& grid) {
   const int half = p.R / 2;
   const long long per_token = (long long)(p.H > 0 ? p.H : 1) * units_per_head;
-  long long tokens = 16 * kThreads / per_token;
+  long long tokens = each * kThreads / per_token;
   const long long most = kAngles / half < 1 ? 1 : kAngles / half;
   if (tokens > most) tokens = most;
   const long long fill = ((long long)p.T + 4 * cab::kNumSMs - 1) / (4 * cab::kNumSMs);
@@ -345,7 +346,7 @@ void split(RopeParams& p, int units_per_head, dim3& grid) {
 template <typename T, int N, bool kInterleaved>
 int launch_rope(RopeParams& p, cudaStream_t stream) {
   dim3 grid;
-  split(p, (kInterleaved ? p.R : p.R / 2) / N, grid);
+  split(p, (kInterleaved ? p.R : p.R / 2) / N, 4, grid);
   if (grid.y > 65535) return CAB_ERR_TOO_LARGE;
   mla_rope_kernel<T, N, kInterleaved><<<grid, kThreads, 0, stream>>>(p);
   return cab::launch_status();
@@ -367,7 +368,7 @@ int run_append(AppendParams& p, bool interleaved, cudaStream_t stream) {
                    (p.r.H == 0 || (vec16(p.r.x, p.r.xt, p.r.xh) && vec16(p.r.out, p.r.ot, p.r.oh)));
   const int n = vec ? 8 : (interleaved ? 2 : 1);
   dim3 grid;
-  split(p.r, (interleaved ? kRot : kRot / 2) / n, grid);
+  split(p.r, (interleaved ? kRot : kRot / 2) / n, 8, grid);
   if (grid.y > 65535) return CAB_ERR_TOO_LARGE;
   if (interleaved) {
     if (vec) mla_rope_append_kernel<T, true, true><<<grid, kThreads, 0, stream>>>(p);
