@@ -23,6 +23,29 @@ __host__ __device__ inline bool aligned_to(const void* p, size_t bytes) {
 // without synchronising the stream.
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? CAB_OK : CAB_ERR_LAUNCH; }
 
+// For small kernels that follow one another: the launch lets the kernel be set up while the one before it in the stream ends, and
+// the kernel's first statement waits for that end, with all that was written by then: 1 to 2 us less between two of
+// them. What the kernel reads goes through ordinary loads (no __ldg), as it may be there before it is written.
+template <typename... P, typename... A>
+inline int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) != cudaSuccess) return CAB_ERR_LAUNCH;
+  return launch_status();
+}
+__device__ __forceinline__ void after_predecessor() {
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
+}
+
 // Threads for a CTA that walks `chunks` equal pieces of a row, one piece per thread and pass: the largest
 // multiple of 32 up to 256 that leaves no thread idle in the last pass (7168 bf16 columns in 16-byte pieces:
 // 896 = 4 x 224), else 256.

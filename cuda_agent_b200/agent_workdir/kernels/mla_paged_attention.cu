@@ -40,7 +40,7 @@
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
 // Every wait is bounded.
 // Measured, 128 heads, bf16, pages of 64: 1024 tokens after 7168 rows 1.78 ms (1235 TFLOP/s; 1.92 ms at the power limit,
-// 1.6 GHz); 64 sequences of 8192 rows and less, one token each, 119 to 129 us on different boxes (3 TB/s of the cache: a
+// 1.6 GHz); 64 sequences of 8192 rows and less, one token each, 119 to 129 us from one B200 to another (3 TB/s of the cache: a
 // step waits for its rows, the merge is 13 us of it). 32 sequences of 4096 rows and less, 5 tokens with 24 heads, pages of 16: 49 us. One token
 // with 16 heads and 1000 rows: 15 us, set-up and latency.
 #include <cuda_fp16.h>
@@ -138,9 +138,11 @@ __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // Issued where it stands, so that the load is under way while other work is done.
+// (An ordinary load, as all of them here: the read-only path is for data that nobody writes while the kernel is there, and
+// this one is there before its predecessor has ended.)
 __device__ __forceinline__ int load_now(const int* p) {
   int v;
-  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -221,15 +223,15 @@ struct Maps { CUtensorMap one, two, four, q, q16; };
 
 __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   Seq s;
-  const int a = min(max(__ldg(p.q_start + b), 0), p.T);
-  const int e = min(max(__ldg(p.q_start + b + 1), a), p.T);
+  const int a = min(max(p.q_start[b], 0), p.T);
+  const int e = min(max(p.q_start[b + 1], a), p.T);
   s.tok = a;
   s.n = e - a;
-  s.len = (int)min((long long)max(__ldg(p.kv_len + b), 0), (long long)p.max_pages * p.page_size);
+  s.len = (int)min((long long)max(p.kv_len[b], 0), (long long)p.max_pages * p.page_size);
   s.pos = s.len - s.n;
   return s;
 }
-__device__ __forceinline__ bool descends(const Params& p, int b) { return __ldg(p.q_start + b) > __ldg(p.q_start + b + 1); }
+__device__ __forceinline__ bool descends(const Params& p, int b) { return p.q_start[b] > p.q_start[b + 1]; }
 __device__ __forceinline__ int tiles_of(const Params& p, int n) {
   return (int)(((unsigned)n * (unsigned)p.H + kRows - 1) / kRows);    // T * H < 2^31
 }
@@ -1080,7 +1082,7 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
     }
     if (p.tail && ok) {                        // a warp per row; outside the division of work, so that padding does not move its cuts
       const long long end = (long long)p.T * p.H;
-      for (long long r = (long long)min(max(__ldg(p.q_start + p.batch), 0), p.T) * p.H + blockIdx.x * 4 + warp; r < end;
+      for (long long r = (long long)min(max(p.q_start[p.batch], 0), p.T) * p.H + blockIdx.x * 4 + warp; r < end;
            r += gridDim.x * 4) {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * kDv);
         dst[lane] = dst[lane + 32] = make_uint4(0, 0, 0, 0);

@@ -103,6 +103,7 @@ __device__ bool lowest_free(const int* refcount, int num_pages, int want, int* l
 // anything on entry.
 __global__ void __launch_bounds__(kPlan) mla_pages_check_copy_kernel(const int* src, const int* dst, int n, int num_pages,
                                                                      Scratch s, int* status) {
+  cab::after_predecessor();
   constexpr int kSrc = 1, kDst = 2, kTwice = 4;
   if (threadIdx.x == 0 && status) *status = 0;
   if (threadIdx.x == 0) s.head[0] = n;
@@ -141,7 +142,7 @@ __device__ __forceinline__ void copy_pages(uint8_t* pages, long long layer_strid
     const int piece = (int)(e % pieces);
     const long long rest = e / pieces;
     const int layer = (int)(rest % layers), i = (int)(rest / layers);
-    const int a = __ldg(src + i), b = __ldg(dst + i);
+    const int a = src[i], b = dst[i];
     if (a < 0 || b < 0) continue;
     const Unit* from = reinterpret_cast<const Unit*>(pages + layer * layer_stride + a * page_bytes);
     Unit* to = reinterpret_cast<Unit*>(pages + layer * layer_stride + b * page_bytes);
@@ -160,6 +161,7 @@ template <typename Unit>
 __global__ void __launch_bounds__(kCopy) mla_pages_copy_kernel(uint8_t* pages, long long layer_stride, int layers,
                                                                long long page_bytes, const int* count, const int* src,
                                                                const int* dst) {
+  cab::after_predecessor();
   copy_pages<Unit>(pages, layer_stride, layers, page_bytes, *count, src, dst);
 }
 
@@ -168,6 +170,7 @@ __global__ void __launch_bounds__(kCopy) mla_pages_copy_kernel(uint8_t* pages, l
 // exchanged for the mark that finds a sequence listed twice.
 __global__ void __launch_bounds__(kPlan) mla_pages_extend_kernel(Pool q, const int* seqs, const int* new_length, int n,
                                                                  Scratch s, int* status) {
+  cab::after_predecessor();
   __shared__ int bad;
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -219,6 +222,7 @@ __global__ void __launch_bounds__(kPlan) mla_pages_extend_kernel(Pool q, const i
 // n_a: length of the parent, n_b: the fresh page of child i (-1: none), n_c: its mark was set.
 __global__ void __launch_bounds__(kPlan) mla_pages_plan_fork_kernel(Pool q, const int* src, const int* dst, int n, Scratch s,
                                                                     int* status) {
+  cab::after_predecessor();
   __shared__ int bad;
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -285,6 +289,7 @@ template <typename Unit>
 __global__ void __launch_bounds__(kCopy) mla_pages_fork_kernel(Pool q, const int* src, const int* dst, int n, Scratch s,
                                                                uint8_t* pages, long long layer_stride, int layers,
                                                                long long page_bytes, int* status) {
+  cab::after_predecessor();
   if (!s.head[1]) return;
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
     const int full = s.n_a[i] / q.page_size;
@@ -303,6 +308,7 @@ __global__ void __launch_bounds__(kCopy) mla_pages_fork_kernel(Pool q, const int
 // ------------------------------------------------------------------------------------------------ free
 // One CTA per listed sequence; whoever takes the length out of the array gives its pages back.
 __global__ void __launch_bounds__(256) mla_pages_free_kernel(Pool q, const int* seqs, int n, int* status) {
+  cab::after_predecessor();
   __shared__ int taken;
   const int seq = seqs[blockIdx.x];
   if ((unsigned)seq >= (unsigned)q.slots) {
@@ -327,6 +333,7 @@ __global__ void __launch_bounds__(256) mla_pages_free_kernel(Pool q, const int* 
 // ------------------------------------------------------------------------------------------------ compact
 // list_b -> list_a: the moves; map[p] for p >= U: where page p went, -1 if it was free.
 __global__ void __launch_bounds__(kPlan) mla_pages_plan_compact_kernel(int* refcount, int num_pages, Scratch s, int* status) {
+  cab::after_predecessor();
   if (threadIdx.x == 0 && status) *status = 0;
   int used = 0;
   for (int base = 0; base < num_pages; base += kPlan * kScan) {
@@ -379,6 +386,7 @@ __global__ void __launch_bounds__(kPlan) mla_pages_plan_compact_kernel(int* refc
 template <typename Unit>
 __global__ void __launch_bounds__(kCopy) mla_pages_compact_kernel(Pool q, Scratch s, uint8_t* pages, long long layer_stride,
                                                                   int layers, long long page_bytes, int* status) {
+  cab::after_predecessor();
   const int used = s.head[2];
   for (int seq = blockIdx.x; seq < q.slots; seq += gridDim.x) {
     const int need = min(pages_for(max(q.length[seq], 0), q.page_size), q.max_pages);
@@ -446,17 +454,15 @@ extern "C" int mla_pages_copy_launcher(void* pages, long long layer_stride, int 
   if (n > kMaxList || num_pages > kMaxPages) return CAB_ERR_TOO_LARGE;
   if (!cab::aligned_to(scratch, 16)) return CAB_ERR_MISALIGNED;
   const Scratch s = carve(scratch, num_pages, n);
-  mla_pages_check_copy_kernel<<<1, kPlan, 0, stream>>>(src, dst, n, num_pages, s, status);
-  int rc = cab::launch_status();
+  const int rc = cab::launch_behind(&mla_pages_check_copy_kernel, dim3(1), dim3(kPlan), 0, stream, src, dst, n, num_pages, s, status);
   if (rc != CAB_OK) return rc;
   const int unit = unit_of(pages, layers > 1 ? layer_stride : 0, page_bytes);
   const unsigned grid = grid_of(n, layers, page_bytes, unit, 0);
-#define CAB_LAUNCH(U)                                                                                                    \
-  mla_pages_copy_kernel<U><<<grid, kCopy, 0, stream>>>(static_cast<uint8_t*>(pages), layer_stride, layers, page_bytes, \
-                                                       s.head, s.n_a, s.n_b)
+#define CAB_LAUNCH(U)                                                                                             \
+  return cab::launch_behind(&mla_pages_copy_kernel<U>, dim3(grid), dim3(kCopy), 0, stream, static_cast<uint8_t*>(pages), \
+                            layer_stride, layers, page_bytes, s.head, s.n_a, s.n_b)
   CAB_BY_UNIT(unit, CAB_LAUNCH);
 #undef CAB_LAUNCH
-  return cab::launch_status();
 }
 
 extern "C" int mla_pages_extend_launcher(int* page_table, int* length, int* refcount, int slots, int max_pages, int num_pages,
@@ -472,8 +478,8 @@ extern "C" int mla_pages_extend_launcher(int* page_table, int* length, int* refc
   if (n > kMaxList || num_pages > kMaxPages) return CAB_ERR_TOO_LARGE;
   if (!cab::aligned_to(scratch, 16)) return CAB_ERR_MISALIGNED;
   const Pool q{page_table, length, refcount, slots, max_pages, num_pages, page_size};
-  mla_pages_extend_kernel<<<1, kPlan, 0, stream>>>(q, seqs, new_length, n, carve(scratch, num_pages, n), status);
-  return cab::launch_status();
+  return cab::launch_behind(&mla_pages_extend_kernel, dim3(1), dim3(kPlan), 0, stream, q, seqs, new_length, n,
+                            carve(scratch, num_pages, n), status);
 }
 
 extern "C" int mla_pages_fork_launcher(void* pages, long long layer_stride, int layers, long long page_bytes, int* page_table,
@@ -493,18 +499,16 @@ extern "C" int mla_pages_fork_launcher(void* pages, long long layer_stride, int 
   if (!cab::aligned_to(scratch, 16)) return CAB_ERR_MISALIGNED;
   const Pool q{page_table, length, refcount, slots, max_pages, num_pages, page_size};
   const Scratch s = carve(scratch, num_pages, n);
-  mla_pages_plan_fork_kernel<<<1, kPlan, 0, stream>>>(q, src, dst, n, s, status);
-  int rc = cab::launch_status();
+  const int rc = cab::launch_behind(&mla_pages_plan_fork_kernel, dim3(1), dim3(kPlan), 0, stream, q, src, dst, n, s, status);
   if (rc != CAB_OK) return rc;
   if (layers == 0) page_bytes = 0;
   const int unit = unit_of(pages, layers > 1 ? layer_stride : 0, page_bytes);
   const unsigned grid = grid_of(n, layers, page_bytes, unit, n);
-#define CAB_LAUNCH(U)                                                                                                 \
-  mla_pages_fork_kernel<U><<<grid, kCopy, 0, stream>>>(q, src, dst, n, s, static_cast<uint8_t*>(pages), layer_stride, \
-                                                       layers, page_bytes, status)
+#define CAB_LAUNCH(U)                                                                                                  \
+  return cab::launch_behind(&mla_pages_fork_kernel<U>, dim3(grid), dim3(kCopy), 0, stream, q, src, dst, n, s,             \
+                            static_cast<uint8_t*>(pages), layer_stride, layers, page_bytes, status)
   CAB_BY_UNIT(unit, CAB_LAUNCH);
 #undef CAB_LAUNCH
-  return cab::launch_status();
 }
 
 extern "C" int mla_pages_free_launcher(int* page_table, int* length, int* refcount, int slots, int max_pages, int num_pages,
@@ -516,8 +520,7 @@ extern "C" int mla_pages_free_launcher(int* page_table, int* length, int* refcou
   if (!seqs) return CAB_ERR_BAD_ARGUMENT;
   if (n > kMaxList || num_pages > kMaxPages) return CAB_ERR_TOO_LARGE;
   const Pool q{page_table, length, refcount, slots, max_pages, num_pages, page_size};
-  mla_pages_free_kernel<<<n, 256, 0, stream>>>(q, seqs, n, status);
-  return cab::launch_status();
+  return cab::launch_behind(&mla_pages_free_kernel, dim3(n), dim3(256), 0, stream, q, seqs, n, status);
 }
 
 extern "C" int mla_pages_compact_launcher(void* pages, long long layer_stride, int layers, long long page_bytes, int* page_table,
@@ -531,16 +534,14 @@ extern "C" int mla_pages_compact_launcher(void* pages, long long layer_stride, i
   if (!cab::aligned_to(scratch, 16)) return CAB_ERR_MISALIGNED;
   const Pool q{page_table, const_cast<int*>(length), refcount, slots, max_pages, num_pages, page_size};
   const Scratch s = carve(scratch, num_pages, 0);
-  mla_pages_plan_compact_kernel<<<1, kPlan, 0, stream>>>(refcount, num_pages, s, status);
-  int rc = cab::launch_status();
+  const int rc = cab::launch_behind(&mla_pages_plan_compact_kernel, dim3(1), dim3(kPlan), 0, stream, refcount, num_pages, s, status);
   if (rc != CAB_OK) return rc;
   if (layers == 0) page_bytes = 0;
   const int unit = unit_of(pages, layers > 1 ? layer_stride : 0, page_bytes);
   const unsigned grid = grid_of(num_pages / 2 + 1, layers, page_bytes, unit, slots);
-#define CAB_LAUNCH(U)                                                                                                       \
-  mla_pages_compact_kernel<U><<<grid, kCopy, 0, stream>>>(q, s, static_cast<uint8_t*>(pages), layer_stride, layers, page_bytes, \
-                                                          status)
+#define CAB_LAUNCH(U)                                                                                           \
+  return cab::launch_behind(&mla_pages_compact_kernel<U>, dim3(grid), dim3(kCopy), 0, stream, q, s,                \
+                            static_cast<uint8_t*>(pages), layer_stride, layers, page_bytes, status)
   CAB_BY_UNIT(unit, CAB_LAUNCH);
 #undef CAB_LAUNCH
-  return cab::launch_status();
 }

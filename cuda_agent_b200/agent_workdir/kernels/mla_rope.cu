@@ -8,10 +8,10 @@
 // Columns move in 16-byte pieces where pointers, strides and R allow it, else pair by pair. A thread keeps one place
 // in the row and steps through the rows of its CTA, so nothing is divided in the loop; its first rows are asked
 // for before the sines and cosines are made.
-// Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 26.6 us (5.0 TB/s of the 134 MB read and
-// written; a copy of the same strided view takes 24.7 us); 64 of 128 fp32 columns of 2047 tokens x 16 heads, inverse,
-// 4.2 us; the append of 4096 tokens with 128 heads 32.9 us (144 MB, 4.4 TB/s: the heads' 128-byte pieces of q and the cache
-// rows at once), of 32 tokens 4.2 us.
+// Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 24.9 us (5.4 TB/s of the 134 MB read and
+// written; a library copy of the same strided view takes 24.7 us); 64 of 128 fp32 columns of 2047 tokens x 16 heads, inverse,
+// 3.8 us; the append of 4096 tokens with 128 heads 31.2 us (144 MB, 4.6 TB/s: the heads' 128-byte pieces of q and the cache
+// rows at once), of 32 tokens 5.9 us. (Per call, calls one behind the other.)
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -213,6 +213,7 @@ struct RowWalk {
 template <typename T, int N, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads, 4) mla_rope_kernel(const RopeParams p) {
   __shared__ __align__(16) float2 cs[kAngles];
+  cab::after_predecessor();
   const int t0 = blockIdx.x * p.tokens, tokens = min(p.tokens, p.T - t0), half = p.R / 2;
   const int h0 = blockIdx.y * p.heads, h1 = min(p.H, h0 + p.heads);
   T* out = static_cast<T*>(p.out) + t0 * p.ot + h0 * p.oh;
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_kernel(const RopeParams 
   RowWalk<T, N, kInterleaved> w(out, x, tokens, h1 - h0, p.R, p.xt, p.xh, p.ot, p.oh);
   w.load();
   for (int e = threadIdx.x; e < tokens * half; e += kThreads)
-    cs[e] = turn_of(__ldg(p.positions + t0 + e / half), __ldg(p.freq + e % half), p.mscale, p.inverse != 0);
+    cs[e] = turn_of(p.positions[t0 + e / half], p.freq[e % half], p.mscale, p.inverse != 0);
   __syncthreads();
   w.rest(cs);
   // rows of more units than threads have: the others
@@ -254,8 +255,9 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   __shared__ __align__(16) float2 cs[kAngles];
   __shared__ int s_pos[kAngles / half];
   __shared__ long long s_row[kAngles / half];  // where the cache row begins, -1: nowhere
+  cab::after_predecessor();
   const int t0 = blockIdx.x * p.r.tokens;
-  const int end = min(max(__ldg(p.q_start + p.batch), 0), p.r.T);     // tokens behind the last sequence stay as they are
+  const int end = min(max(p.q_start[p.batch], 0), p.r.T);     // tokens behind the last sequence stay as they are
   const int tokens = min(p.r.tokens, end - t0);
   if (tokens <= 0) return;
   // what does not depend on the tables is asked for before they are read
@@ -276,11 +278,11 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
     int lo = 0, hi = p.batch;                  // last b with q_start[b] <= t
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(p.q_start + mid) <= t) lo = mid; else hi = mid;
+      if (p.q_start[mid] <= t) lo = mid; else hi = mid;
     }
-    const int pos = __ldg(p.kv_len + lo) - __ldg(p.q_start + lo + 1) + t;
+    const int pos = p.kv_len[lo] - p.q_start[lo + 1] + t;
     const int at = pos / p.page_size;
-    const int page = pos >= 0 && at < p.max_pages ? __ldg(p.page_table + (long long)lo * p.max_pages + at) : -1;
+    const int page = pos >= 0 && at < p.max_pages ? p.page_table[(long long)lo * p.max_pages + at] : -1;
     const bool ok = (unsigned)page < (unsigned)p.num_pages;
     s_pos[threadIdx.x] = pos;
     s_row[threadIdx.x] = ok ? page * p.page_stride + (pos - at * p.page_size) * p.token_stride : -1;
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   }
   __syncthreads();
   for (int e = threadIdx.x; e < tokens * half; e += kThreads)
-    cs[e] = turn_of(s_pos[e / half], __ldg(p.r.freq + e % half), p.r.mscale, false);
+    cs[e] = turn_of(s_pos[e / half], p.r.freq[e % half], p.r.mscale, false);
   if (copies) {                                // the latent part of the rows: a copy
     T* rows = static_cast<T*>(p.rows);
     for (int e = threadIdx.x; e < tokens * (kLatent / C); e += kThreads) {
@@ -314,9 +316,9 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
 }
 
 // Tokens and heads per CTA: about `each` units a thread, fewer where the call is too small to fill the device. An append takes
-// eight, so that its look into the tables is waited for less often (the large call above takes 32.9 us, with four 36.9, with
+// eight, so that its look into the tables is waited for less often (the large call above took 32.9 us, with four 36.9, with
 // sixteen 33.5). The rotation alone takes four: on rows that another kernel or call just touched 26.6 us, with eight
-// 27.4, with sixteen 28.5 (on rows that are nowhere near, 34.4, 33.6 and 31.4).
+// 27.4, with sixteen 28.5 (on rows that are nowhere near, 34.4, 33.6 and 31.4). These before launch_behind, 1.7 us each.
 void split(RopeParams& p, int units_per_head, int each, dim3& grid) {
   const int half = p.R / 2;
   const long long per_token = (long long)(p.H > 0 ? p.H : 1) * units_per_head;
@@ -348,8 +350,7 @@ int launch_rope(RopeParams& p, cudaStream_t stream) {
   dim3 grid;
   split(p, (kInterleaved ? p.R : p.R / 2) / N, 4, grid);
   if (grid.y > 65535) return CAB_ERR_TOO_LARGE;
-  mla_rope_kernel<T, N, kInterleaved><<<grid, kThreads, 0, stream>>>(p);
-  return cab::launch_status();
+  return cab::launch_behind(&mla_rope_kernel<T, N, kInterleaved>, grid, dim3(kThreads), 0, stream, p);
 }
 
 template <typename T>
@@ -370,14 +371,11 @@ int run_append(AppendParams& p, bool interleaved, cudaStream_t stream) {
   dim3 grid;
   split(p.r, (interleaved ? kRot : kRot / 2) / n, 8, grid);
   if (grid.y > 65535) return CAB_ERR_TOO_LARGE;
-  if (interleaved) {
-    if (vec) mla_rope_append_kernel<T, true, true><<<grid, kThreads, 0, stream>>>(p);
-    else mla_rope_append_kernel<T, true, false><<<grid, kThreads, 0, stream>>>(p);
-  } else {
-    if (vec) mla_rope_append_kernel<T, false, true><<<grid, kThreads, 0, stream>>>(p);
-    else mla_rope_append_kernel<T, false, false><<<grid, kThreads, 0, stream>>>(p);
-  }
-  return cab::launch_status();
+  if (interleaved)
+    return vec ? cab::launch_behind(&mla_rope_append_kernel<T, true, true>, grid, dim3(kThreads), 0, stream, p)
+               : cab::launch_behind(&mla_rope_append_kernel<T, true, false>, grid, dim3(kThreads), 0, stream, p);
+  return vec ? cab::launch_behind(&mla_rope_append_kernel<T, false, true>, grid, dim3(kThreads), 0, stream, p)
+             : cab::launch_behind(&mla_rope_append_kernel<T, false, false>, grid, dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
