@@ -84,6 +84,13 @@ inline int sm_count() {
   return n;
 }
 
+// The starts of a paged batch's sequences run from 0, never descend, and stay within the T tokens of the call. Whether entry b
+// (of `batch`) and the one after it break that.
+__device__ __forceinline__ bool wrong_start(const int* q_start, int b, int batch, int T) {
+  const int a = q_start[b], e = q_start[b + 1];
+  return a > e || (b == 0 && a != 0) || (b == batch - 1 && e > T);
+}
+
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);

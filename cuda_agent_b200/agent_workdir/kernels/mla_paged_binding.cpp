@@ -97,7 +97,8 @@ int to_int(int64_t v, const char* name) {
 void raise_status(const torch::Tensor& status, const char* op) {
   const int code = status.item<int>();
   const char* text = code == CAB_PAGED_BAD_PAGE      ? "a needed page table entry lies outside the pool"
-                     : code == CAB_PAGED_BAD_INDEX   ? "a listed page or sequence is out of range or listed twice, or q_start descends"
+                     : code == CAB_PAGED_BAD_INDEX   ? "a listed page or sequence is out of range or listed twice, or q_start descends, does not begin "
+                                                       "at 0 or passes the tokens"
                      : code == CAB_PAGED_NO_ROOM     ? "not enough free pages, or a sequence longer than its table row"
                      : code == CAB_PAGED_NOT_EMPTY   ? "a fork's child is in use"
                                                      : "a bounded wait gave up";

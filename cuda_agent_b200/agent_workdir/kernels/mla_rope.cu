@@ -259,7 +259,13 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   const int t0 = blockIdx.x * p.r.tokens;
   const int end = min(max(p.q_start[p.batch], 0), p.r.T);     // tokens behind the last sequence stay as they are
   const int tokens = min(p.r.tokens, end - t0);
-  if (tokens <= 0) return;
+  const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+  if (tokens <= 0 && !first) return;           // the first one stays, to say whether the starts are sound
+  // Wrong starts would put tokens on rows that are there already. Every CTA looks at all of them, so all agree to write nothing
+  // (no difference up to 4096 sequences, their loads hide behind those of the rows; 16384 of one token with 128 heads 129 -> 169 us).
+  bool wrong = false, lost = false;
+#pragma unroll 4
+  for (int b = threadIdx.x; b < p.batch; b += kThreads) wrong |= cab::wrong_start(p.q_start, b, p.batch, p.r.T);
   // what does not depend on the tables is asked for before they are read
   const int h0 = blockIdx.y * p.r.heads, h1 = min(p.r.H, h0 + p.r.heads);
   RowWalk<T, N, kInterleaved> w(static_cast<T*>(p.r.out) + t0 * p.r.ot + h0 * p.r.oh,
@@ -286,9 +292,13 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
     const bool ok = (unsigned)page < (unsigned)p.num_pages;
     s_pos[threadIdx.x] = pos;
     s_row[threadIdx.x] = ok ? page * p.page_stride + (pos - at * p.page_size) * p.token_stride : -1;
-    if (!ok && blockIdx.y == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
+    lost = !ok && blockIdx.y == 0;
   }
-  __syncthreads();
+  if (__syncthreads_or(wrong)) {
+    if (first && threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_INDEX);
+    return;
+  }
+  if (lost && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_PAGE);
   for (int e = threadIdx.x; e < tokens * half; e += kThreads)
     cs[e] = turn_of(s_pos[e / half], p.r.freq[e % half], p.r.mscale, false);
   if (copies) {                                // the latent part of the rows: a copy

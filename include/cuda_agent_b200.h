@@ -385,6 +385,7 @@ enum cab_dtype { CAB_BF16 = 0, CAB_F16 = 1, CAB_F32 = 2 };
 enum cab_paged_status {
   CAB_PAGED_BAD_PAGE = 401,      /* a table entry that is needed lies outside [0, num_pages), or the table row is too short */
   CAB_PAGED_BAD_INDEX = 402,     /* a page or sequence number of a list lies outside its range, or stands there twice; */
+                                 /* append: q_start does not begin at 0, descends or ends beyond T, nothing was written; */
                                  /* attention: q_start descends, nothing was computed                                  */
   CAB_PAGED_NO_ROOM = 403,       /* too few free pages, or a sequence longer than a table row: nothing was changed */
   CAB_PAGED_NOT_EMPTY = 404      /* a fork's child is in use already: nothing was changed */
@@ -399,7 +400,7 @@ typedef struct cab_mla_paged_batch {
   long long page_stride, token_stride;
   int num_pages, page_size;
   const int* page_table;           /* [batch, max_pages] */
-  const int* q_start;              /* [batch + 1], ascending, from 0 */
+  const int* q_start;              /* [batch + 1], from 0, never descending, at most T */
   const int* kv_len;               /* [batch] */
   int batch, max_pages;
   int dtype;                       /* CAB_BF16 or CAB_F16 */

@@ -501,3 +501,37 @@ def test_attention_with_starts_that_descend_does_nothing(ext, cuda_device, batch
         ext.mla_paged_attention_forward(q, cache, table, wrong, kv, SCALE, out=out, lse=lse, check=True)
     assert (out == 7).all() and (lse == 7).all()
     check_attention(ext, args)
+
+
+WRONG_STARTS = {"begin_late": (0, 1), "begin_below": (0, -1), "descend": (1, 10 ** 6), "end_low": (-1, -3), "end_early": (-1, 1),
+                "end_late": (-1, 10 ** 6)}
+
+
+def wrong_starts(start, kind):
+    at, value = WRONG_STARTS[kind]
+    wrong = start.clone()
+    wrong[at] = min(value, start[-1].item() + 1)
+    return wrong
+
+
+@pytest.mark.parametrize("batch", [2, 32, 300])
+@pytest.mark.parametrize("kind", list(WRONG_STARTS))
+def test_append_with_wrong_starts_writes_nothing(ext, cuda_device, kind, batch):
+    """Starts that do not begin at 0, descend or pass the tokens: rows of earlier tokens and of other sequences stay, as do the
+    queries; a call with the right ones goes through after it."""
+    _, cache, table, start, kv = make_batch([(2, 40)] * batch, 1, 16, torch.bfloat16, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    T, heads = 2 * batch, 3
+    joint = torch.randn(T, 576, generator=g, device=cuda_device).to(torch.bfloat16)
+    q_pe = torch.randn(T, heads, 64, generator=g, device=cuda_device).to(torch.bfloat16)
+    freq = 10000.0 ** (-torch.arange(32, dtype=torch.float64, device=cuda_device) / 32)
+    q = torch.full((T, heads, 64), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    before, wrong = cache.clone(), wrong_starts(start, kind)
+    with pytest.raises(RuntimeError, match="q_start"):
+        ext.mla_rope_append_forward(q_pe, joint[:, :512], joint[:, 512:], cache, table, wrong, kv, freq, q, check=True)
+    assert torch.equal(cache, before) and (q == 7).all()
+    fresh = ext.mla_rope_append_forward(q_pe, joint[:, :512], joint[:, 512:], cache, table, wrong, kv, freq)
+    assert torch.equal(cache, before) and (fresh == 0).all()
+    ext.mla_rope_append_forward(q_pe, joint[:, :512], joint[:, 512:], cache, table, start, kv, freq, q, check=True)
+    at = table[:, 2].long()
+    assert torch.equal(cache[at, 6:8, :512].reshape(T, 512), joint[:, :512]) and not (q == 7).all()
