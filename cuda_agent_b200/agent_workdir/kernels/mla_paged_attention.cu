@@ -92,7 +92,7 @@ struct __align__(16) Control {
   Item first_item;
   alignas(16) int pages[2][2][2][kKeys];       // [producer][step parity][own / other keys]: the pages of the boxes
   uint32_t tmem_base;
-  int abort_flag, settled;
+  int abort_flag, settled, wrong;              // wrong: the starts are not sound, nothing is computed
 };
 constexpr int kRingBytes = (kNUnits * kNTiles + 1 + (kVSlots + 1) * kVTiles) * kTile;
 constexpr int kPBytes = kRows * 128;           // P of a CTA: 128 rows x 64 keys
@@ -231,7 +231,6 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   s.pos = s.len - s.n;
   return s;
 }
-__device__ __forceinline__ bool descends(const Params& p, int b) { return p.q_start[b] > p.q_start[b + 1]; }
 __device__ __forceinline__ int tiles_of(const Params& p, int n) {
   return (int)(((unsigned)n * (unsigned)p.H + kRows - 1) / kRows);    // T * H < 2^31
 }
@@ -362,7 +361,8 @@ __device__ __forceinline__ void found(const Params& p, Control& ctl, const Run& 
 // Where pair `pair` begins: thread-parallel over the sequences, then over the tiles. `pre`: batch + 1 ints of
 // shared memory that nothing else uses yet. A decode step of up to 32 sequences (no more than eight tiles each) is
 // settled by one warp without barriers, 1000 clk sooner. Starts that descend would give the same tokens to several
-// sequences, without end: nothing is done then.
+// sequences, without end, and the append writes nothing at such, at starts that begin late or that pass the tokens:
+// nothing is done then.
 __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
   const int tid = threadIdx.x;
   if (p.batch <= 32) {
@@ -370,7 +370,7 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
     if (tid < 32) {
       Seq s{0, 0, 0, 0};
       if (tid < p.batch) s = seq_of(p, tid);
-      const bool bad = __any_sync(0xffffffffu, tid < p.batch && descends(p, tid));
+      const bool bad = __any_sync(0xffffffffu, tid < p.batch && cab::wrong_start(p.q_start, tid, p.batch, p.T));
       if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_INDEX);
       const int tiles = bad ? 0 : tiles_of(p, s.n);
       done = __all_sync(0xffffffffu, tiles <= 8);
@@ -397,7 +397,10 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
           if ((blockIdx.x & 1) == 0) p.meta[pair] = Meta{0, 0, 0};
         }
       }
-      if (tid == 0) ctl.settled = done;
+      if (tid == 0) {
+        ctl.settled = done;
+        ctl.wrong = bad;
+      }
     }
     __syncthreads();
     if (ctl.settled) return;
@@ -407,11 +410,12 @@ __device__ void find_run(const Params& p, Control& ctl, int* pre, int pair) {
     long long sum = 0;
     bool bad = false;
     for (int b = b0; b < b1; ++b) {
-      bad |= descends(p, b);
+      bad |= cab::wrong_start(p.q_start, b, p.batch, p.T);
       sum += tiles_of(p, seq_of(p, b).n);
     }
     bad = __syncthreads_or(bad);
     if (bad && tid == 0 && p.status) atomicCAS(p.status, 0, (int)CAB_PAGED_BAD_INDEX);
+    if (tid == 0) ctl.wrong = bad;
     long long at = block_scan(ctl, bad ? 0 : sum);
     for (int b = b0; b < b1; ++b) {
       pre[b] = (int)min(at, (long long)0x7fffffff);
@@ -1081,9 +1085,9 @@ mla_paged_attention_kernel(const Params p, const __grid_constant__ Maps maps) {
       w = nx;
     }
     if (p.tail && ok) {                        // a warp per row; outside the division of work, so that padding does not move its cuts
-      const long long end = (long long)p.T * p.H;
-      for (long long r = (long long)min(max(p.q_start[p.batch], 0), p.T) * p.H + blockIdx.x * 4 + warp; r < end;
-           r += gridDim.x * 4) {
+      // (with wrong starts all rows are such; without sequences there is nothing before the tail)
+      const long long end = (long long)p.T * p.H, begin = ctl.wrong || p.batch == 0 ? 0 : (long long)p.q_start[p.batch] * p.H;
+      for (long long r = begin + blockIdx.x * 4 + warp; r < end; r += gridDim.x * 4) {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * kDv);
         dst[lane] = dst[lane + 32] = make_uint4(0, 0, 0, 0);
         if (lane == 0 && p.lse) p.lse[r] = -INFINITY;

@@ -385,8 +385,8 @@ enum cab_dtype { CAB_BF16 = 0, CAB_F16 = 1, CAB_F32 = 2 };
 enum cab_paged_status {
   CAB_PAGED_BAD_PAGE = 401,      /* a table entry that is needed lies outside [0, num_pages), or the table row is too short */
   CAB_PAGED_BAD_INDEX = 402,     /* a page or sequence number of a list lies outside its range, or stands there twice; */
-                                 /* append: q_start does not begin at 0, descends or ends beyond T, nothing was written; */
-                                 /* attention: q_start descends, nothing was computed                                  */
+                                 /* append, attention: q_start does not begin at 0, descends or ends beyond T, nothing  */
+                                 /* was written (attention with config 256: all tokens see nothing)                    */
   CAB_PAGED_NO_ROOM = 403,       /* too few free pages, or a sequence longer than a table row: nothing was changed */
   CAB_PAGED_NOT_EMPTY = 404      /* a fork's child is in use already: nothing was changed */
 };
@@ -436,7 +436,8 @@ int mla_rope_append_launcher(void* q_out, const void* q_pe, const void* c_kv, co
 /* CAB_PAGED_BAD_PAGE), a length beyond max_pages * page_size as that product. One new token per sequence is */
 /* the decode step. workspace: mla_paged_attention_workspace_bytes(T, H) bytes, 16-byte aligned, contents */
 /* irrelevant, not shared by calls that can overlap. softmax_scale > 0. T * H < 2^31, batch <= 16384. Tokens */
-/* at and after q_start[batch] are left alone; config 256 writes them as tokens that see nothing. */
+/* at and after q_start[batch] are left alone; config 256 writes them as tokens that see nothing, and all */
+/* tokens where q_start is wrong (CAB_PAGED_BAD_INDEX). */
 size_t mla_paged_attention_workspace_bytes(int T, int H);
 int mla_paged_attention_launcher(void* out, float* lse, const void* q, const cab_mla_paged_batch* batch, int T, int H,
                                  float softmax_scale, int causal, int window, void* workspace,

@@ -535,3 +535,28 @@ def test_append_with_wrong_starts_writes_nothing(ext, cuda_device, kind, batch):
     ext.mla_rope_append_forward(q_pe, joint[:, :512], joint[:, 512:], cache, table, start, kv, freq, q, check=True)
     at = table[:, 2].long()
     assert torch.equal(cache[at, 6:8, :512].reshape(T, 512), joint[:, :512]) and not (q == 7).all()
+
+
+@pytest.mark.parametrize("batch", [2, 32, 300])
+@pytest.mark.parametrize("kind", list(WRONG_STARTS))
+def test_attention_with_wrong_starts_returns_no_old_memory(ext, cuda_device, kind, batch):
+    """Fresh outputs come from memory that held something else: zeros and -infinity, also where nobody asks for the status.
+    Outputs that are given stay as they were."""
+    args = make_batch([(2, 40)] * batch, 4, 16, torch.bfloat16, cuda_device)
+    q, cache, table, start, kv = args
+    wrong = wrong_starts(start, kind)
+    for check in (False, True):
+        poison = [torch.full((2 * batch, 4, 512), 7.0, dtype=q.dtype, device=cuda_device) for _ in range(4)]
+        poison += [torch.full((2 * batch, 4), 7.0, device=cuda_device) for _ in range(4)]
+        del poison
+        if check:
+            with pytest.raises(RuntimeError, match="q_start"):
+                ext.mla_paged_attention_forward(q, cache, table, wrong, kv, SCALE, check=True)
+        else:
+            out, lse = ext.mla_paged_attention_forward(q, cache, table, wrong, kv, SCALE)
+            assert (out == 0).all() and (lse == -math.inf).all()
+    out = torch.full((2 * batch, 4, 512), 7.0, dtype=q.dtype, device=cuda_device)
+    lse = torch.full((2 * batch, 4), 7.0, device=cuda_device)
+    ext.mla_paged_attention_forward(q, cache, table, wrong, kv, SCALE, out=out, lse=lse)
+    assert (out == 7).all() and (lse == 7).all()
+    check_attention(ext, args)
