@@ -96,7 +96,7 @@ int to_int(int64_t v, const char* name) {
 
 void raise_status(const torch::Tensor& status, const char* op) {
   const int code = status.item<int>();
-  const char* text = code == CAB_PAGED_BAD_PAGE      ? "a needed page table entry lies outside the pool"
+  const char* text = code == CAB_PAGED_BAD_PAGE      ? "a needed page table entry lies outside the pool, or names a page that counts as free"
                      : code == CAB_PAGED_BAD_INDEX   ? "a listed page or sequence is out of range or listed twice, or q_start descends, does not begin "
                                                        "at 0 or passes the tokens"
                      : code == CAB_PAGED_NO_ROOM     ? "not enough free pages, or a sequence longer than its table row"

@@ -237,10 +237,21 @@ __global__ void __launch_bounds__(kPlan) mla_pages_plan_fork_kernel(Pool q, cons
     const int len = q.length[src[i]];
     if (len < 0 || len > most) atomicMax(&bad, (int)CAB_PAGED_BAD_INDEX);
     s.n_a[i] = min(max(len, 0), (int)min(most, (long long)0x7fffffff));
-    if (len > 0 && len % q.page_size) {
-      const int page = q.table[(long long)src[i] * q.max_pages + s.n_a[i] / q.page_size - (s.n_a[i] == most ? 1 : 0)];
-      if ((unsigned)page >= (unsigned)q.num_pages) atomicMax(&bad, (int)CAB_PAGED_BAD_PAGE);
+  }
+  __syncthreads();
+  // Every entry that a child takes over, a warp per parent; one that follows itself in the list is looked at once. A page that
+  // counts as free could be taken as a child's own below.
+  for (int i = threadIdx.x >> 5; i < n && !bad; i += kPlan / 32) {
+    if (i > 0 && src[i] == src[i - 1]) continue;
+    const int need = pages_for(s.n_a[i], q.page_size);
+    const int* row = q.table + (long long)src[i] * q.max_pages;
+    bool lost = false;
+#pragma unroll 4
+    for (int k = threadIdx.x & 31; k < need; k += 32) {
+      const int page = row[k];
+      lost |= (unsigned)page >= (unsigned)q.num_pages || q.refcount[page] <= 0;
     }
+    if (lost) atomicMax(&bad, (int)CAB_PAGED_BAD_PAGE);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n && !bad; i += kPlan) {
@@ -288,7 +299,7 @@ __global__ void __launch_bounds__(kPlan) mla_pages_plan_fork_kernel(Pool q, cons
 template <typename Unit>
 __global__ void __launch_bounds__(kCopy) mla_pages_fork_kernel(Pool q, const int* src, const int* dst, int n, Scratch s,
                                                                uint8_t* pages, long long layer_stride, int layers,
-                                                               long long page_bytes, int* status) {
+                                                               long long page_bytes) {
   cab::after_predecessor();
   if (!s.head[1]) return;
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
@@ -298,8 +309,7 @@ __global__ void __launch_bounds__(kCopy) mla_pages_fork_kernel(Pool q, const int
     for (int k = threadIdx.x; k < full; k += kCopy) {
       const int page = from[k];
       to[k] = page;
-      if ((unsigned)page < (unsigned)q.num_pages) atomicAdd(q.refcount + page, 1);
-      else raise(status, CAB_PAGED_BAD_PAGE);
+      if ((unsigned)page < (unsigned)q.num_pages) atomicAdd(q.refcount + page, 1);   // (the plan found it so)
     }
   }
   copy_pages<Unit>(pages, layer_stride, layers, page_bytes, s.head[0], s.list_b, s.list_a);
@@ -506,7 +516,7 @@ extern "C" int mla_pages_fork_launcher(void* pages, long long layer_stride, int 
   const unsigned grid = grid_of(n, layers, page_bytes, unit, n);
 #define CAB_LAUNCH(U)                                                                                                  \
   return cab::launch_behind(&mla_pages_fork_kernel<U>, dim3(grid), dim3(kCopy), 0, stream, q, src, dst, n, s,             \
-                            static_cast<uint8_t*>(pages), layer_stride, layers, page_bytes, status)
+                            static_cast<uint8_t*>(pages), layer_stride, layers, page_bytes)
   CAB_BY_UNIT(unit, CAB_LAUNCH);
 #undef CAB_LAUNCH
 }

@@ -383,7 +383,8 @@ enum cab_dtype { CAB_BF16 = 0, CAB_F16 = 1, CAB_F32 = 2 };
 /* Codes that the launchers below leave in *status (device int, may be NULL; it is  */
 /* cleared first). 211 .. 219: a bounded wait gave up. */
 enum cab_paged_status {
-  CAB_PAGED_BAD_PAGE = 401,      /* a table entry that is needed lies outside [0, num_pages), or the table row is too short */
+  CAB_PAGED_BAD_PAGE = 401,      /* a table entry that is needed lies outside [0, num_pages), or the table row is too short; */
+                                 /* fork, free, compact: or names a page that counts as free. fork: nothing was changed     */
   CAB_PAGED_BAD_INDEX = 402,     /* a page or sequence number of a list lies outside its range, or stands there twice; */
                                  /* append, attention: q_start does not begin at 0, descends or ends beyond T, nothing  */
                                  /* was written (attention with config 256: all tokens see nothing)                    */

@@ -305,3 +305,30 @@ def test_lists_inside_the_pool_are_refused_and_one_buffer_is_not(ext, cuda_devic
     lists[:2] = ints([2, 7], cuda_device)
     ext.mla_pages_extend(table, length, refcount, lists[:1], lists[1:2], 4, True)
     assert table[2].tolist() == [0, 1, -1, -1] and length.tolist() == [0, 0, 7, 0] and refcount[:3].tolist() == [1, 1, 0]
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 4])
+def test_fork_with_a_bad_entry_changes_nothing(ext, cuda_device, at):
+    """Any needed entry of the parent (full pages 0 to 3, the partly filled fifth): outside the pool, or a page that counts as
+    free and could be the child's fresh one. Sound pairs of the same call are not carried out either."""
+    s = State(cuda_device, 6, 6, 14, 4)
+    ext.mla_pages_extend(s.table, s.length, s.refcount, ints([0, 1], s.dev), ints([18, 9], s.dev), 4, True)
+    s.reset()
+    for bad in (-1, 14, 2 ** 31 - 1, 8):              # eight pages are in use, 8 is the lowest free one
+        table = s.table.clone()
+        table[0, at] = bad
+        keep = table.clone()
+        with pytest.raises(RuntimeError, match="page table"):
+            ext.mla_pages_fork(s.pages, table, s.length, s.refcount, ints([1, 0, 0, 1], s.dev), ints([2, 3, 4, 5], s.dev), True)
+        assert torch.equal(table, keep)
+        s.check()                                     # lengths, counts and pages as they were
+    broken = s.table.clone()
+    broken[1, 2] = 13
+    broken[0, 5] = 99                                 # behind the parent's last page: not needed
+    ext.mla_pages_fork(s.pages, broken, s.length, s.refcount, ints([0, 0], s.dev), ints([2, 3], s.dev), True)
+    s.table.copy_(broken)
+    s.want.table = broken.tolist()
+    for row in (2, 3):
+        s.want.table[row] = [-1] * 6
+    s.want.fork([0, 0], [2, 3])
+    s.check()
