@@ -22,7 +22,7 @@ constexpr int kScan = 4;                       // counts per thread and step of 
 
 // Scratch, in ints: [16] what was decided, then three arrays of num_pages and three of n + 1.
 struct Scratch {
-  int* head;                                   // [0] pages to copy, [1] the call is carried out, [2] pages in use
+  int* head;                                   // [0] pages to copy, [1] the call is carried out
   int *list_a, *list_b, *map;                  // num_pages each
   int *n_a, *n_b, *n_c;                        // n + 1 each
 };
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256) mla_pages_free_kernel(Pool q, const int* 
 }
 
 // ------------------------------------------------------------------------------------------------ compact
-// list_b -> list_a: the moves; map[p] for p >= U: where page p went, -1 if it was free.
+// list_b -> list_a: the moves; map[p]: where page p went, p itself if it stayed, -1 if it was free.
 __global__ void __launch_bounds__(kPlan) mla_pages_plan_compact_kernel(int* refcount, int num_pages, Scratch s, int* status) {
   cab::after_predecessor();
   if (threadIdx.x == 0 && status) *status = 0;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kPlan) mla_pages_plan_compact_kernel(int* refc
 #pragma unroll
     for (int k = 0; k < kScan; ++k) {
       const int p = p0 + k;
-      if (p >= used && p < num_pages) s.map[p] = move[k] ? at : -1;
+      if (p < num_pages) s.map[p] = move[k] ? at : p < used && !hole[k] ? p : -1;
       if (move[k]) s.list_b[at++] = p;
     }
   }
@@ -390,24 +390,22 @@ __global__ void __launch_bounds__(kPlan) mla_pages_plan_compact_kernel(int* refc
     refcount[s.list_a[k]] = refcount[s.list_b[k]];
     refcount[s.list_b[k]] = 0;
   }
-  if (threadIdx.x == 0) { s.head[0] = high; s.head[2] = used; }
+  if (threadIdx.x == 0) s.head[0] = high;
 }
 
 template <typename Unit>
 __global__ void __launch_bounds__(kCopy) mla_pages_compact_kernel(Pool q, Scratch s, uint8_t* pages, long long layer_stride,
                                                                   int layers, long long page_bytes, int* status) {
   cab::after_predecessor();
-  const int used = s.head[2];
   for (int seq = blockIdx.x; seq < q.slots; seq += gridDim.x) {
     const int need = min(pages_for(max(q.length[seq], 0), q.page_size), q.max_pages);
     int* row = q.table + (long long)seq * q.max_pages;
     for (int k = threadIdx.x; k < need; k += kCopy) {
       const int page = row[k];
       if ((unsigned)page >= (unsigned)q.num_pages) { raise(status, CAB_PAGED_BAD_PAGE); continue; }
-      if (page < used) continue;
       const int to = s.map[page];
-      if (to >= 0) row[k] = to;
-      else raise(status, CAB_PAGED_BAD_PAGE);
+      if (to < 0) raise(status, CAB_PAGED_BAD_PAGE);
+      else if (to != page) row[k] = to;
     }
   }
   copy_pages<Unit>(pages, layer_stride, layers, page_bytes, s.head[0], s.list_b, s.list_a);

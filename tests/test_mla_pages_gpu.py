@@ -332,3 +332,17 @@ def test_fork_with_a_bad_entry_changes_nothing(ext, cuda_device, at):
         s.want.table[row] = [-1] * 6
     s.want.fork([0, 0], [2, 3])
     s.check()
+
+
+def test_compact_reports_an_entry_at_a_free_page(ext, cuda_device):
+    """A row that names a free page, which the compaction fills with another sequence's data, whether the page lies among
+    those that stay or above them."""
+    s = State(cuda_device, 5, 4, 12, 4)
+    ext.mla_pages_extend(s.table, s.length, s.refcount, ints([0, 1, 2], s.dev), ints([8, 8, 8], s.dev), 4, True)
+    ext.mla_pages_free(s.table, s.length, s.refcount, ints([1], s.dev), 4, True)
+    assert s.refcount.tolist()[:6] == [1, 1, 0, 0, 1, 1]
+    for bad in (3, 11):
+        table, length, count = s.table.clone(), s.length.clone(), s.refcount.clone()
+        table[0, 1] = bad
+        with pytest.raises(RuntimeError, match="page table"):
+            ext.mla_pages_compact(s.pages.clone(), table, length, count, True)
