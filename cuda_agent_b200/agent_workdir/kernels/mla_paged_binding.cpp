@@ -56,37 +56,58 @@ void check_rows_apart(const torch::Tensor& t, const char* name) {
   TORCH_CHECK(t.numel() == 0 || outer || inner, name, ": rows of the output overlap");
 }
 
-// From the first byte of a view to behind its last: two tensors may share a program's one buffer, but not its bytes.
-std::pair<const char*, const char*> span_of(const torch::Tensor& t) {
+// The bytes of a view: base + any sum of k * stride, k < n, over its dimensions (the last one: the bytes of a row).
+struct Dim { int64_t n, stride; };
+using Dims = std::vector<Dim>;
+int64_t extent(const Dims& dims) {
   int64_t last = 0;
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-  const char* p = static_cast<const char*>(t.data_ptr());
-  return {p, p + (last + 1) * t.element_size()};
+  for (const Dim& d : dims) last += (d.n - 1) * d.stride;
+  return last + 1;
 }
+// Whether two sets of bytes, b's base `shift` behind a's, may have one in common; false is certain. Beside the ranges as a whole
+// it knows views that lie in one another's gaps: for a period w, strides that are multiples of w drop out.
+bool may_share(const Dims& a, const Dims& b, int64_t shift) {
+  if (shift >= extent(a) || -shift >= extent(b)) return false;
+  for (const Dims* from : {&a, &b})
+    for (const Dim& by : *from) {
+      const int64_t w = by.stride;
+      if (w <= 1 || by.n <= 1) continue;
+      Dims x, y;
+      for (const Dim& d : a) if (d.n > 1 && d.stride % w) x.push_back(d);
+      for (const Dim& d : b) if (d.n > 1 && d.stride % w) y.push_back(d);
+      const int64_t ex = extent(x), ey = extent(y), s = ((shift % w) + w) % w;
+      if (ex > w || ey > w) continue;
+      if (s >= ex && s + ey <= w) return false;                // each has its own part of the period
+      // both within one period, wherever it is taken to begin: alike only where they are alike in it
+      if (s + ey <= w && !may_share(x, y, s)) return false;
+      if (ex <= s && !may_share(x, y, s - w)) return false;
+    }
+  return true;
+}
+Dims bytes_of(const torch::Tensor& t) {
+  Dims dims;
+  for (int64_t d = 0; d < t.dim(); ++d) dims.push_back({t.size(d), t.stride(d) * (int64_t)t.element_size()});
+  dims.push_back({(int64_t)t.element_size(), 1});
+  return dims;
+}
+// Two tensors may share a program's one buffer, but not its bytes.
 bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   if (!a.numel() || !b.numel()) return false;
-  const auto x = span_of(a), y = span_of(b);
-  return x.first < y.second && y.first < x.second;
+  auto end_of = [](const torch::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
+  if (pa >= end_of(b) || pb >= end_of(a)) return false;        // the common case
+  return may_share(bytes_of(a), bytes_of(b), pb - pa);
 }
 
 // An output is its input itself, or lies elsewhere.
 void check_apart(const torch::Tensor& out, const torch::Tensor& in, const char* what) {
-  if (!overlap(out, in)) return;
-  if (out.data_ptr() == in.data_ptr() && out.sizes() == in.sizes() && out.strides() == in.strides()) return;
-  // two column ranges of the same rows
-  bool same = out.dim() == in.dim();
-  for (int64_t d = 0; same && d + 1 < out.dim(); ++d) same = out.size(d) <= 1 || in.size(d) <= 1 || out.stride(d) == in.stride(d);
-  if (same && out.dim() >= 2) {
-    int64_t pitch = 0;
-    for (int64_t d = 0; d + 1 < out.dim(); ++d)
-      if (out.size(d) > 1 && in.size(d) > 1) pitch = pitch ? std::min(pitch, out.stride(d)) : out.stride(d);
-    const int64_t shift = (static_cast<const char*>(out.data_ptr()) - static_cast<const char*>(in.data_ptr())) / out.element_size();
-    if (pitch > 0) {
-      const int64_t s = ((shift % pitch) + pitch) % pitch;
-      if (s >= in.size(-1) && pitch - s >= out.size(-1)) return;
-    }
-  }
-  TORCH_CHECK(false, what, " overlap without being the same view");
+  bool same = out.data_ptr() == in.data_ptr() && out.sizes() == in.sizes();
+  for (int64_t d = 0; same && d < out.dim(); ++d) same = out.size(d) <= 1 || out.stride(d) == in.stride(d);
+  TORCH_CHECK(same || !overlap(out, in), what, " overlap without being the same view");
 }
 
 int to_int(int64_t v, const char* name) {

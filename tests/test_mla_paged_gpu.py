@@ -3,6 +3,7 @@
 Every result is compared with a statement in 64 bits (tests/paged_reference.py, where the tolerances are derived).
 """
 import math
+import random
 
 import pytest
 import torch
@@ -560,3 +561,46 @@ def test_attention_with_wrong_starts_returns_no_old_memory(ext, cuda_device, kin
     ext.mla_paged_attention_forward(q, cache, table, wrong, kv, SCALE, out=out, lse=lse)
     assert (out == 7).all() and (lse == 7).all()
     check_attention(ext, args)
+
+
+def test_rope_between_views_of_one_buffer(ext, cuda_device):
+    """Inputs and outputs anywhere in one buffer, with any strides: what shares bytes without being the same view is refused,
+    what is accepted is right. Which bytes a view has is counted element by element."""
+    rng, accepted, refused = random.Random(7), 0, 0
+    freq = torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    base = torch.randn(1000, generator=g, device=cuda_device)
+    places = [((2, 3, 8), (100, 30, 1), 0, (100, 30, 1), 40), ((2, 3, 8), (100, 30, 1), 0, (100, 30, 1), 8),
+              ((3, 4, 8), (64, 16, 1), 8, (64, 16, 1), 0), ((1, 3, 8), (100, 16, 1), 0, (48, 16, 1), 0),
+              ((2, 1, 8), (16, 50, 1), 4, (16, 8, 1), 4)]
+    for _ in range(1500):
+        shape = (rng.randint(1, 4), rng.randint(1, 4), 8)
+        strides = [(rng.choice([8, 16, 24, 30, 48, 64, 100, 120]), rng.choice([8, 9, 16, 24, 30, 40]), 1) for _ in range(2)]
+        if rng.random() < 0.7:
+            strides[1] = strides[0]
+        places.append((shape, strides[0], rng.randint(0, 200), strides[1], rng.randint(0, 200)))
+    for shape, sx, ox, so, oo in places:
+        def elements(strides, offset):
+            return [offset + i * strides[0] + j * strides[1] + c for i in range(shape[0]) for j in range(shape[1]) for c in range(8)]
+        a, b = elements(sx, ox), elements(so, oo)
+        same = a == b
+        if len(set(b)) < len(b):
+            continue                                  # an output whose own rows overlap: another refusal
+        store = base.clone()
+        x, out = torch.as_strided(store, shape, sx, ox), torch.as_strided(store, shape, so, oo)
+        pos = torch.arange(shape[0], dtype=torch.int32, device=cuda_device) + 5
+        want, tol = ref.rotate(x.clone(), pos, freq)
+        try:
+            ext.mla_rope_forward(x, pos, freq, out=out)
+        except RuntimeError as e:
+            assert "overlap" in str(e) and not same, (shape, sx, ox, so, oo)
+            refused += 1
+            assert torch.equal(store, base)
+            continue
+        assert same or not set(a) & set(b), (shape, sx, ox, so, oo)
+        assert ((out.double() - want).abs() <= tol).all(), (shape, sx, ox, so, oo)
+        rest = torch.ones(1000, dtype=torch.bool, device=cuda_device)
+        rest[torch.tensor(b, device=cuda_device)] = False
+        assert torch.equal(store[rest], base[rest])
+        accepted += 1
+    assert accepted > 100 and refused > 100
