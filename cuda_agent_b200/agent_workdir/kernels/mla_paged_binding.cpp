@@ -179,6 +179,7 @@ torch::Tensor mla_rope_forward(torch::Tensor x, torch::Tensor positions, torch::
     check_same_device(x, out, "x", "out");
     check_rows_apart(out, "out");
     check_apart(out, x, "x and out");
+    for (const torch::Tensor* t : {&positions, &freq}) TORCH_CHECK(!overlap(out, *t), "out must not overlap positions or freq");
   }
   check_status(mla_rope_launcher(out.data_ptr(), x.data_ptr(), ptr<const int>(positions), ptr<const double>(freq), to_int(T, "T"),
                                  to_int(H, "H"), to_int(R, "R"), stride_of(x, 0), stride_of(x, 1), stride_of(out, 0),
@@ -215,9 +216,14 @@ torch::Tensor mla_rope_append_forward(torch::Tensor q_pe, torch::Tensor c_kv, to
     check_same_device(cache, out, "cache", "q_out");
     check_rows_apart(out, "q_out");
     check_apart(out, q_pe, "q_pe and q_out");
+    // a CTA may have written its rows before another one has read these
+    for (const torch::Tensor* t : {&c_kv, &k_pe, &freq, &page_table, &q_start, &kv_len})
+      TORCH_CHECK(!overlap(out, *t), "q_out must not overlap an input but q_pe");
   }
   for (const torch::Tensor* t : {&q_pe, &c_kv, &k_pe, &out})
     TORCH_CHECK(!overlap(*t, cache), "the new rows and q_out must not overlap the cache");
+  for (const torch::Tensor* t : {&freq, &page_table, &q_start, &kv_len})
+    TORCH_CHECK(!overlap(*t, cache), "freq and the batch's tables must not overlap the cache");
   torch::Tensor status;
   if (check) status = torch::empty({1}, q_start.options());
   check_status(mla_rope_append_launcher(out.data_ptr(), q_pe.data_ptr(), c_kv.data_ptr(), k_pe.data_ptr(), &batch,
@@ -371,6 +377,8 @@ void mla_pages_fork(torch::Tensor pages, torch::Tensor page_table, torch::Tensor
   const PoolArgs q = pool_of(page_table, length, refcount);
   TORCH_CHECK(q.num_pages == p.num_pages, "refcount must have an entry for each page");
   check_same_device(pages, length, "pages", "length");
+  for (const torch::Tensor* t : {&page_table, &length, &refcount})
+    TORCH_CHECK(!overlap(*t, pages), "pages must not overlap page_table, length or refcount");
   const int n = list_of(src, "src", {&page_table, &length, &refcount, &pages});
   TORCH_CHECK(list_of(dst, "dst", {&page_table, &length, &refcount, &pages}) == n, "src and dst must be equally long");
   c10::cuda::CUDAGuard guard(length.device());
@@ -403,6 +411,8 @@ void mla_pages_compact(torch::Tensor pages, torch::Tensor page_table, torch::Ten
   const PoolArgs q = pool_of(page_table, length, refcount);
   TORCH_CHECK(q.num_pages == p.num_pages, "refcount must have an entry for each page");
   check_same_device(pages, length, "pages", "length");
+  for (const torch::Tensor* t : {&page_table, &length, &refcount})
+    TORCH_CHECK(!overlap(*t, pages), "pages must not overlap page_table, length or refcount");
   c10::cuda::CUDAGuard guard(length.device());
   const auto scratch = scratch_for(q.num_pages, 0);
   const auto status = status_if(check, length);

@@ -604,3 +604,45 @@ def test_rope_between_views_of_one_buffer(ext, cuda_device):
         assert torch.equal(store[rest], base[rest])
         accepted += 1
     assert accepted > 100 and refused > 100
+
+
+def test_outputs_over_other_inputs_are_refused(ext, cuda_device):
+    """Rotation and append: an output over anything that another block still reads. Columns of one joint projection, and one
+    buffer for everything, are fine where no byte is shared."""
+    T, H, bf = 6, 3, torch.bfloat16
+    _, cache, table, start, kv = make_batch([(4, 40), (2, 20)], 1, 16, bf, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    freq = 10000.0 ** (-torch.arange(32, dtype=torch.float64, device=cuda_device) / 32)
+    joint = torch.randn(T, H * 576 + 576, generator=g, device=cuda_device).to(bf)          # queries, latent row, k_pe
+    q, c_kv, k_pe = joint[:, :H * 576].view(T, H, 576), joint[:, H * 576:H * 576 + 512], joint[:, H * 576 + 512:]
+    first, before = cache.clone(), joint.clone()
+    call = lambda out, cache=cache, freq=freq, table=table, start=start, kv=kv, q_pe=q[..., 512:]: ext.mla_rope_append_forward(
+        q_pe, c_kv, k_pe, cache, table, start, kv, freq, out, check=True)
+    flat = joint.view(-1)
+    ints64 = torch.zeros(4096, dtype=torch.float64, device=cuda_device)
+    ints64[:32] = freq
+    as_rows = lambda t: t.view(bf)[:T * H * 64].view(T, H, 64)
+    tables = torch.zeros(4096, dtype=torch.int32, device=cuda_device)
+    for i, t in enumerate((table, start, kv)):
+        tables[i * 64:i * 64 + t.numel()] = t.reshape(-1)
+    inside = [tables[i * 64:i * 64 + t.numel()].view(t.shape) for i, t in enumerate((table, start, kv))]
+    for bad in (lambda: call(k_pe[:, None].expand(T, 1, 64), q_pe=q[:, :1, 512:]), lambda: call(c_kv[:, None, 448:], q_pe=q[:, :1, 512:]),
+                lambda: call(flat[H * 576 - 64:][:T * H * 64].view(T, H, 64)),
+                lambda: call(as_rows(ints64), freq=ints64[:32]), lambda: call(as_rows(tables), table=inside[0]),
+                lambda: call(as_rows(tables), start=inside[1]), lambda: call(as_rows(tables), kv=inside[2]),
+                lambda: call(None, freq=cache.view(-1)[:128].view(torch.float64)),
+                lambda: call(None, kv=cache.view(-1)[:4].view(torch.int32))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            bad()
+    assert torch.equal(cache, first) and torch.equal(joint, before)
+    # in place in the joint projection
+    want = ext.mla_rope_append_forward(q[..., 512:].clone(), c_kv.clone(), k_pe.clone(), first, table, start, kv, freq)
+    call(q[..., 512:])
+    assert torch.equal(q[..., 512:], want) and torch.equal(cache, first) and torch.equal(c_kv, before[:, H * 576:H * 576 + 512])
+    x = torch.randn(4, 2, 8, generator=g, device=cuda_device)
+    pos = torch.arange(64, dtype=torch.int32, device=cuda_device)
+    f = torch.ones(64, dtype=torch.float64, device=cuda_device)
+    for bad in (lambda: ext.mla_rope_forward(x, pos[:4], f[:4], out=pos.view(torch.float32).view(4, 2, 8)),
+                lambda: ext.mla_rope_forward(x, pos[:4], f[:4], out=f.view(torch.float32)[4:68].view(4, 2, 8))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            bad()

@@ -346,3 +346,27 @@ def test_compact_reports_an_entry_at_a_free_page(ext, cuda_device):
         table[0, 1] = bad
         with pytest.raises(RuntimeError, match="page table"):
             ext.mla_pages_compact(s.pages.clone(), table, length, count, True)
+
+
+def test_tables_inside_the_pages_are_refused(ext, cuda_device):
+    pages = torch.zeros(2, 12, 4, 8, dtype=torch.int32, device=cuda_device)
+    s = State(cuda_device, 4, 4, 12, 4)
+    one, two = ints([0], s.dev), ints([1], s.dev)
+    table, length, refcount = pages[0, 0, :2].view(4, 4), pages[1, 11, 3, 4:], pages.view(-1)[100:112]
+    for t, n, r in ((table, s.length, s.refcount), (s.table, length, s.refcount), (s.table, s.length, refcount)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ext.mla_pages_fork(pages, t, n, r, one, two)
+        with pytest.raises(RuntimeError, match="overlap"):
+            ext.mla_pages_compact(pages, t, n, r)
+    assert not pages.any()
+    # the tables in gaps between the layers are elsewhere
+    store = torch.zeros(2, 12 * 4 * 8 + 64, dtype=torch.int32, device=cuda_device)
+    pages = store[:, :12 * 4 * 8].view(2, 12, 4, 8)
+    s.refcount = store[0, 12 * 4 * 8:][:12]
+    s.pages = pages
+    s.reset()
+    s.want.extend([0], [6])
+    ext.mla_pages_extend(s.table, s.length, s.refcount, one, ints([6], s.dev), 4, True)
+    s.want.fork([0], [1])
+    ext.mla_pages_fork(pages, s.table, s.length, s.refcount, one, two, True)
+    s.check()
