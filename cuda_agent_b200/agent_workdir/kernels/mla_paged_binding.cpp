@@ -90,17 +90,21 @@ Dims bytes_of(const torch::Tensor& t) {
   dims.push_back({(int64_t)t.element_size(), 1});
   return dims;
 }
-// Two tensors may share a program's one buffer, but not its bytes.
-bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
-  if (!a.numel() || !b.numel()) return false;
-  auto end_of = [](const torch::Tensor& t) {
+// Two tensors may share a program's one buffer, but not its bytes. (The ends are kept: a call compares a tensor with many.)
+struct Place {
+  const torch::Tensor& t;
+  const char *begin, *end;
+  Place(const torch::Tensor& x) : t(x), begin(static_cast<const char*>(x.data_ptr())), end(begin) {
+    if (!x.numel()) return;
     int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
-  };
-  const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
-  if (pa >= end_of(b) || pb >= end_of(a)) return false;        // the common case
-  return may_share(bytes_of(a), bytes_of(b), pb - pa);
+    const auto n = x.sizes(), stride = x.strides();
+    for (size_t d = 0; d < n.size(); ++d) last += (n[d] - 1) * stride[d];
+    end = begin + (last + 1) * (int64_t)x.element_size();
+  }
+};
+bool overlap(const Place& a, const Place& b) {
+  if (a.begin >= b.end || b.begin >= a.end) return false;      // the common case, and that of tensors without elements
+  return may_share(bytes_of(a.t), bytes_of(b.t), b.begin - a.begin);
 }
 
 // An output is its input itself, or lies elsewhere.
@@ -216,14 +220,15 @@ torch::Tensor mla_rope_append_forward(torch::Tensor q_pe, torch::Tensor c_kv, to
     check_same_device(cache, out, "cache", "q_out");
     check_rows_apart(out, "q_out");
     check_apart(out, q_pe, "q_pe and q_out");
-    // a CTA may have written its rows before another one has read these
-    for (const torch::Tensor* t : {&c_kv, &k_pe, &freq, &page_table, &q_start, &kv_len})
-      TORCH_CHECK(!overlap(out, *t), "q_out must not overlap an input but q_pe");
   }
-  for (const torch::Tensor* t : {&q_pe, &c_kv, &k_pe, &out})
-    TORCH_CHECK(!overlap(*t, cache), "the new rows and q_out must not overlap the cache");
-  for (const torch::Tensor* t : {&freq, &page_table, &q_start, &kv_len})
-    TORCH_CHECK(!overlap(*t, cache), "freq and the batch's tables must not overlap the cache");
+  const Place to(out), rows(cache);
+  TORCH_CHECK(!overlap(q_pe, rows) && !overlap(to, rows), "the new rows and q_out must not overlap the cache");
+  for (const torch::Tensor* t : {&c_kv, &k_pe, &freq, &page_table, &q_start, &kv_len}) {
+    const Place in(*t);
+    TORCH_CHECK(!overlap(in, rows), "the new rows, freq and the batch's tables must not overlap the cache");
+    // a CTA may have written its rows before another one has read these
+    TORCH_CHECK(!overlap(to, in), "q_out must not overlap an input but q_pe");
+  }
   torch::Tensor status;
   if (check) status = torch::empty({1}, q_start.options());
   check_status(mla_rope_append_launcher(out.data_ptr(), q_pe.data_ptr(), c_kv.data_ptr(), k_pe.data_ptr(), &batch,

@@ -261,11 +261,6 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   const int tokens = min(p.r.tokens, end - t0);
   const bool first = blockIdx.x == 0 && blockIdx.y == 0;
   if (tokens <= 0 && !first) return;           // the first one stays, to say whether the starts are sound
-  // Wrong starts would put tokens on rows that are there already. Every CTA looks at all of them, so all agree to write nothing
-  // (no difference up to 4096 sequences, their loads hide behind those of the rows; 16384 of one token with 128 heads 129 -> 169 us).
-  bool wrong = false, lost = false;
-#pragma unroll 4
-  for (int b = threadIdx.x; b < p.batch; b += kThreads) wrong |= cab::wrong_start(p.q_start, b, p.batch, p.r.T);
   // what does not depend on the tables is asked for before they are read
   const int h0 = blockIdx.y * p.r.heads, h1 = min(p.r.H, h0 + p.r.heads);
   RowWalk<T, N, kInterleaved> w(static_cast<T*>(p.r.out) + t0 * p.r.ot + h0 * p.r.oh,
@@ -279,6 +274,12 @@ __global__ void __launch_bounds__(kThreads, 4) mla_rope_append_kernel(const Appe
   const bool copies = blockIdx.y == 0;
   if (copies && threadIdx.x < tokens * (kLatent / C))
     latent = *reinterpret_cast<const Vec<T, C>*>(c + threadIdx.x / (kLatent / C) * p.ct + threadIdx.x % (kLatent / C) * C);
+  // Wrong starts would put tokens on rows that are there already. Every CTA looks at all of them, so all agree to write nothing
+  // (no difference up to 4096 sequences, their loads hide behind those of the rows; 16384 of one token with 128 heads 129 -> 169 us).
+  bool wrong = false, lost = false;
+#pragma unroll 4
+  for (int b = kThreads - 1 - threadIdx.x; b < p.batch; b += kThreads)             // the last warps first: the first one has the search below
+    wrong |= cab::wrong_start(p.q_start, b, p.batch, p.r.T);
   if (threadIdx.x < tokens) {
     const int t = t0 + threadIdx.x;
     int lo = 0, hi = p.batch;                  // last b with q_start[b] <= t
