@@ -6,7 +6,8 @@ device. Its methods are the extension's ``mla_pages_*``, ``mla_rope_append_forwa
 and ``mla_sparse_decode_forward``; nothing is computed in torch but the batch's own small tables. A program serves with it as
 
     cache = PagedLatentCache(layers, pages, 64, slots=256, max_rows=32768)
-    freq, mscale = rope_frequencies(64)
+    freq, mscale = rope_frequencies(64, scaling="yarn", factor=16.0, mscale=1.0, mscale_all_dim=1.0)
+    scale = head_dim ** -0.5 * rope_score_factor(16.0, 1.0)
     cache.extend(seqs, new_length)                       # pages for the new tokens of every sequence
     batch = cache.batch(seqs, q_start)                   # once per step, for all layers
     for layer in range(layers):
@@ -29,22 +30,32 @@ ROW = 576
 
 
 def rope_frequencies(rot: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
-                     original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda"):
-    """(freq, mscale): radians per position of the rot / 2 pairs (64-bit), and the factor on the rotated columns.
+                     original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda",
+                     mscale: float = 1.0, mscale_all_dim: float = 0.0):
+    """(freq, factor on the rotated columns): radians per position of the rot / 2 pairs (64-bit), and what ``append`` takes as
+    ``mscale``.
 
     ``scaling`` stretches a model's positions from ``original_length`` to ``factor`` times it:
       none    base^(-2i / rot)
       linear  every frequency divided by the factor
       ntk     the base raised to base * factor^(rot / (rot - 2)): fast pairs stay, the slowest is divided by the factor
       yarn    pairs that turn more than beta_fast times within original_length stay, those that turn less than beta_slow
-              times are divided by the factor, a ramp over the pair's number in between; mscale = 0.1 ln(factor) + 1
+              times are divided by the factor, a ramp over the pair's number in between. The factor on the rotated
+              columns is m(mscale) / m(mscale_all_dim), m(c) = 0.1 c ln(factor) + 1
+
+    YaRN means m as a temperature of the whole score, m^2 times it. On the rotated columns alone, as without
+    ``mscale_all_dim``, that is so only for a head all of whose columns are rotated. Of the rows of this cache 64 of 576 are: a
+    checkpoint says by its two coefficients (mostly equal, so that the factor is 1) what the rotated columns get, and the whole
+    score takes ``rope_score_factor(factor, mscale_all_dim)``, which belongs into the softmax scale.
     """
     if rot <= 0 or rot % 2:
         raise ValueError("rot must be a positive even number")
     if base <= 1.0 or factor < 1.0 or original_length < 1:
         raise ValueError("base must be above 1, factor and original_length at least 1")
+    if mscale < 0 or mscale_all_dim < 0:
+        raise ValueError("mscale and mscale_all_dim must not be negative")
     i = torch.arange(rot // 2, dtype=torch.float64)
-    mscale = 1.0
+    on_rotated = 1.0
     if scaling == "ntk":
         if rot == 2:
             raise ValueError("ntk scaling needs more than one pair")
@@ -59,10 +70,21 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: str = "none", fac
         high = min(max(math.ceil(pair_of(beta_slow)), 0), rot - 1)
         ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq / factor * ramp + freq * (1 - ramp)
-        mscale = 0.1 * math.log(factor) + 1.0
+        on_rotated = _yarn_m(factor, mscale) / _yarn_m(factor, mscale_all_dim)
     elif scaling not in ("none", "ntk"):
         raise ValueError(f"unknown scaling {scaling!r}: none, linear, ntk or yarn")
-    return freq.to(device), mscale
+    return freq.to(device), on_rotated
+
+
+def _yarn_m(factor: float, coefficient: float) -> float:
+    return 0.1 * coefficient * math.log(factor) + 1.0
+
+
+def rope_score_factor(factor: float, mscale_all_dim: float) -> float:
+    """What yarn scaling by ``factor`` multiplies the softmax scale by, for a checkpoint with the coefficient ``mscale_all_dim``."""
+    if factor < 1.0 or mscale_all_dim < 0:
+        raise ValueError("factor must be at least 1, mscale_all_dim must not be negative")
+    return _yarn_m(factor, mscale_all_dim) ** 2
 
 
 @dataclass

@@ -190,3 +190,33 @@ def test_cache_class_refuses(built_libs):
     assert c.page_table.shape == (3, 5) and (c.page_table == -1).all() and c.pages_free() == 5
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         c.extend([0], [4])
+
+
+def test_yarn_temperature_of_the_whole_score():
+    """A checkpoint's two coefficients (a, b): the rotated columns' part of a score is multiplied by m(a)^2 in all, the latent
+    part by m(b)^2; with equal ones that is one temperature of the whole score. In 64 bits, on rows of 512 + 64 columns."""
+    from cuda_agent_b200.paged import rope_frequencies, rope_score_factor
+    g = torch.Generator().manual_seed(0)
+    q, k = torch.randn(576, generator=g, dtype=torch.float64), torch.randn(576, generator=g, dtype=torch.float64)
+    plain, _ = rope_frequencies(64, scaling="yarn", factor=40.0, device="cpu")
+
+    def rot(x, position, freq, factor):
+        a, b = x[0::2], x[1::2]
+        c, s = (position * freq).cos(), (position * freq).sin()
+        return factor * torch.stack((a * c - b * s, b * c + a * s), -1).flatten()
+
+    for a, b in ((1.0, 1.0), (0.707, 0.707), (1.0, 0.0), (0.5, 0.8), (0.0, 0.0)):
+        freq, mscale = rope_frequencies(64, scaling="yarn", factor=40.0, device="cpu", mscale=a, mscale_all_dim=b)
+        assert torch.equal(freq, plain)
+        score = lambda ms: (q[:512] @ k[:512], rot(q[512:], 5000, freq, ms) @ rot(k[512:], 77, freq, ms))
+        latent, turned = (v * rope_score_factor(40.0, b) for v in score(mscale))
+        m_a, m_b = (0.1 * c * math.log(40.0) + 1 for c in (a, b))
+        want = score(1.0)
+        assert abs(latent - m_b ** 2 * want[0]) <= 1e-12 * abs(want[0]) and abs(turned - m_a ** 2 * want[1]) <= 1e-12 * abs(want[1])
+        if a == b:
+            assert abs(mscale - 1) < 1e-15
+    assert rope_score_factor(1.0, 1.0) == 1.0
+    for bad in (lambda: rope_score_factor(0.5, 1.0), lambda: rope_score_factor(2.0, -1.0),
+                lambda: rope_frequencies(64, scaling="yarn", factor=2.0, device="cpu", mscale=-1.0)):
+        with pytest.raises(ValueError):
+            bad()
