@@ -139,7 +139,24 @@ class PagedLatentCache:
     # ------------------------------------------------------------------------------------------ steps
     def batch(self, seqs, q_start) -> PagedBatch:
         """The batch of sequences ``seqs``, whose new tokens are [q_start[i], q_start[i + 1]) of the step's and whose lengths
-        (the new tokens among them) are the present ones."""
+        (the new tokens among them) are the present ones. A sequence stands in a batch once: two would write the same rows.
+        Of a list that is checked here. A tensor is not read by the host: a sequence that is out of range, or stands before
+        already, gets no pages and length 0, so ``append`` writes nothing for it and reports it, and attention sees nothing."""
+        slots = self.length.numel()
+        if torch.is_tensor(seqs):
+            seqs = seqs.to(self.length.device, torch.int64)
+            n, inside = seqs.numel(), (seqs >= 0) & (seqs < slots)
+            at, order = torch.where(inside, seqs, slots), torch.arange(seqs.numel(), device=seqs.device)
+            first = torch.full((slots + 1,), n, device=seqs.device).scatter_reduce_(0, at, order, "amin")
+            fine = inside & (first[at] == order)
+            at = at.clamp_max(slots - 1)
+            return PagedBatch(torch.where(fine[:, None], self.page_table[at], -1), self._list(q_start),
+                              torch.where(fine, self.length[at], 0))
+        seqs = list(seqs)
+        if not all(0 <= s < slots for s in seqs):
+            raise ValueError(f"sequences must lie in [0, {slots})")
+        if len(set(seqs)) < len(seqs):
+            raise ValueError("a sequence is listed twice")
         seqs = self._list(seqs).long()
         return PagedBatch(self.page_table[seqs], self._list(q_start), self.length[seqs])
 

@@ -220,3 +220,23 @@ def test_yarn_temperature_of_the_whole_score():
                 lambda: rope_frequencies(64, scaling="yarn", factor=2.0, device="cpu", mscale=-1.0)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_batch_of_sequences_that_are_not_there_or_twice(built_libs):
+    """A list raises; a tensor, which the host does not read, gives such places no pages and length 0."""
+    from cuda_agent_b200.paged import PagedLatentCache
+    c = PagedLatentCache(1, 8, 16, 4, 64, device="cpu")
+    c.page_table[:] = torch.arange(16, dtype=torch.int32).view(4, 4)
+    c.length[:] = torch.tensor([5, 6, 7, 8], dtype=torch.int32)
+    for bad in ([4], [0, -1], [1, 2, 1], [2 ** 40]):
+        with pytest.raises(ValueError):
+            c.batch(bad, [0] * (len(bad) + 1))
+    for seqs, fine in (([2, 0], [1, 1]), ([3, 4, 0], [1, 0, 1]), ([-1, 3], [0, 1]), ([1, 2, 1, 1, 0], [1, 1, 0, 0, 1]),
+                       ([9, 2 ** 40, -2 ** 40, 3, 0], [0, 0, 0, 1, 1]), ([2 ** 32 + 1, 1], [0, 1]), ([], [])):
+        b = c.batch(torch.tensor(seqs, dtype=torch.int64), list(range(len(seqs) + 1)))
+        assert b.page_table.dtype == b.kv_len.dtype == b.q_start.dtype == torch.int32
+        assert b.page_table.tolist() == [c.page_table[s].tolist() if f else [-1] * 4 for s, f in zip(seqs, fine)]
+        assert b.kv_len.tolist() == [5 + s if f else 0 for s, f in zip(seqs, fine)]
+        if all(fine):
+            same = c.batch(seqs, list(range(len(seqs) + 1)))
+            assert torch.equal(same.page_table, b.page_table) and torch.equal(same.kv_len, b.kv_len)

@@ -156,3 +156,32 @@ def test_task_loops(cuda_device, built_libs, capsys, monkeypatch, config):
     if config == "0":
         assert profiling.main(args + ["--iters", "3", "--no-compile"]) == 0
         assert "CUDA Extension:" in capsys.readouterr().out
+
+
+def test_batch_from_numbers_on_the_gpu(cuda_device):
+    """A place of the batch that names no sequence, or one that stands before it: reported by the append, nothing written for
+    it, nothing seen by its tokens; also in a captured step."""
+    p = Program(cuda_device, torch.bfloat16, 16, 64)
+    p.step({0: 60, 1: 130, 2: 7})
+    p.cache.extend([0, 1, 2], [61, 131, 8])
+    seqs = torch.tensor([0, 24, 1, 0, -3, 2], dtype=torch.int32, device=cuda_device)
+    fine = [0, 2, 5]
+    joint, q_pe, q = p.rand(6, 576), p.rand(6, 16, 64), p.rand(6, 16, 576)
+    start = torch.arange(7, dtype=torch.int32, device=cuda_device)
+
+    before = p.cache.rows.clone()
+    batch = p.cache.batch(seqs, start)
+    with pytest.raises(RuntimeError, match="page table"):
+        p.cache.append(0, batch, q_pe, joint[:, :512], joint[:, 512:], p.freq, q[..., 512:], check=True)
+    changed = (p.cache.rows != before).any(-1).nonzero().tolist()
+    assert sorted(changed) == sorted([0, int(p.cache.page_table[s, n // 64]), n % 64] for s, n in ((0, 60), (1, 130), (2, 7)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch = p.cache.batch(seqs, start)
+        p.cache.append(0, batch, q_pe, joint[:, :512], joint[:, 512:], p.freq, q[..., 512:])
+        out, lse = p.cache.attend(0, batch, q, SCALE)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, want_lse, tol, tol_lse = ref.attention(q, p.cache.rows[0], batch.page_table, start, batch.kv_len, SCALE)
+    assert ((out.double() - want).abs() <= tol).all() and torch.isinf(lse[[1, 3, 4]]).all() and (out[[1, 3, 4]] == 0).all()
+    assert ((lse.double() - want_lse)[fine].abs() <= tol_lse[fine]).all() and torch.isfinite(lse[fine]).all()
