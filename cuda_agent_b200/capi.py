@@ -294,12 +294,19 @@ def _dtype_code(t) -> int:
     return {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[t.dtype]
 
 
+def _view(t) -> int:
+    """The first element of a tensor whose strides go along with it."""
+    if not t.is_cuda:
+        raise ValueError("the C ABI takes device pointers; got a CPU tensor")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError("the last dimension must be contiguous")
+    return t.data_ptr()
+
+
 def mla_paged_batch(cache, page_table, q_start, kv_len) -> MlaPagedBatch:
     """cache [pages, page_size, 576] (rows and pages may be strided), page_table [batch, max_pages], q_start [batch + 1],
     kv_len [batch]; the tensors have to outlive the calls that take the result."""
-    if not cache.is_cuda:
-        raise ValueError("the C ABI takes device pointers; got a CPU tensor")
-    return MlaPagedBatch(cache.data_ptr(), cache.stride(0), cache.stride(1), cache.shape[0], cache.shape[1], _p(page_table),
+    return MlaPagedBatch(_view(cache), cache.stride(0), cache.stride(1), cache.shape[0], cache.shape[1], _p(page_table),
                          _p(q_start), _p(kv_len), page_table.shape[0], page_table.shape[1], _dtype_code(cache))
 
 
@@ -308,7 +315,7 @@ def mla_rope(out, x, positions, freq, interleaved: bool = False, mscale: float =
     """Rotary positions on x [T, H, R] (any strides but the last); out may be x."""
     T, H, R = x.shape
     _check("mla_rope_launcher",
-           lib().mla_rope_launcher(out.data_ptr(), x.data_ptr(), _p(positions), _p(freq), T, H, R, x.stride(0), x.stride(1),
+           lib().mla_rope_launcher(_view(out), _view(x), _p(positions), _p(freq), T, H, R, x.stride(0), x.stride(1),
                                    out.stride(0), out.stride(1), _dtype_code(x), int(interleaved), int(inverse), mscale,
                                    config, _stream()))
 
@@ -317,10 +324,9 @@ def mla_rope_append(q_out, q_pe, c_kv, k_pe, batch: MlaPagedBatch, freq, interle
                     status=None, config: int = 0) -> None:
     T, H, _ = q_pe.shape
     _check("mla_rope_append_launcher",
-           lib().mla_rope_append_launcher(q_out.data_ptr(), q_pe.data_ptr(), c_kv.data_ptr(), k_pe.data_ptr(),
-                                          ctypes.byref(batch), _p(freq), T, H, q_out.stride(0), q_out.stride(1),
-                                          q_pe.stride(0), q_pe.stride(1), c_kv.stride(0), k_pe.stride(0), int(interleaved),
-                                          mscale, _opt(status), config, _stream()))
+           lib().mla_rope_append_launcher(_view(q_out), _view(q_pe), _view(c_kv), _view(k_pe), ctypes.byref(batch), _p(freq),
+                                          T, H, q_out.stride(0), q_out.stride(1), q_pe.stride(0), q_pe.stride(1), c_kv.stride(0),
+                                          k_pe.stride(0), int(interleaved), mscale, _opt(status), config, _stream()))
 
 
 def mla_paged_workspace_bytes(T: int, H: int) -> int:

@@ -240,3 +240,42 @@ def test_batch_of_sequences_that_are_not_there_or_twice(built_libs):
         if all(fine):
             same = c.batch(seqs, list(range(len(seqs) + 1)))
             assert torch.equal(same.page_table, b.page_table) and torch.equal(same.kv_len, b.kv_len)
+
+
+class OnTheGpu:
+    """What the wrappers ask of a tensor, said of one that is on a GPU; its address is never used."""
+
+    def __init__(self, t, cuda=True):
+        self.t, self.is_cuda, self.shape, self.dtype = t, cuda, t.shape, t.dtype
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def test_c_wrappers_pass_on_device_pointers_only(capi, monkeypatch):
+    """A host address, or columns that are not next to one another, never reach a launcher."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append(name) or 0
+    monkeypatch.setattr(capi, "lib", lambda: Lib())
+    monkeypatch.setattr(capi, "_stream", lambda: 0)
+    bf, i32 = torch.bfloat16, torch.int32
+    gpu = lambda *s, dtype=bf: OnTheGpu(torch.zeros(*s, dtype=dtype))
+    freq, table, start, kv = gpu(32, dtype=torch.float64), gpu(2, 4, dtype=i32), gpu(3, dtype=i32), gpu(2, dtype=i32)
+    rope = dict(out=gpu(3, 2, 64), x=gpu(3, 2, 64), positions=gpu(3, dtype=i32), freq=freq)
+    append = dict(q_out=gpu(3, 2, 64), q_pe=gpu(3, 2, 64), c_kv=gpu(3, 512), k_pe=gpu(3, 64), freq=freq)
+    cache = dict(cache=gpu(4, 16, 576), page_table=table, q_start=start, kv_len=kv)
+    batch = capi.mla_paged_batch(**cache)
+    capi.mla_rope(**rope)
+    capi.mla_rope_append(batch=batch, **append)
+    assert calls == ["mla_rope_launcher", "mla_rope_append_launcher"]
+    apart = lambda t: OnTheGpu(torch.zeros(*t.shape, 2, dtype=t.dtype)[..., 0])
+    for f, args in ((capi.mla_rope, rope), (capi.mla_rope_append, {**append, "batch": batch}), (capi.mla_paged_batch, cache)):
+        for name, t in args.items():
+            if isinstance(t, OnTheGpu):
+                for bad in (OnTheGpu(t.t, cuda=False), apart(t)):
+                    with pytest.raises(ValueError):
+                        f(**{**args, name: bad})
+    assert len(calls) == 2
