@@ -165,9 +165,9 @@ def build_extension(verbose: bool = False) -> Path:
              + ["-L" + str(LIB_DIR), "-lcuda_agent_b200", "-Wl,-rpath,$ORIGIN/../lib",
                 "-L" + torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
                 "-ltorch_python",
-                # the C++ runtime torch itself runs on: a compiler that would link a second copy statically gives a
-                # module whose streams crash when an error message holds a number
-                "-nostdlib++", "-l:libstdc++.so.6"])
+                # the C++ runtime torch itself runs on, before the one the compiler adds: a compiler whose own is static would
+                # give the module a second copy, whose streams crash when an error message holds a number
+                "-l:libstdc++.so.6"])
     return EXT_SO
 
 
