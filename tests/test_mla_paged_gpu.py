@@ -646,3 +646,21 @@ def test_outputs_over_other_inputs_are_refused(ext, cuda_device):
                 lambda: ext.mla_rope_forward(x, pos[:4], f[:4], out=f.view(torch.float32)[4:68].view(4, 2, 8))):
         with pytest.raises(RuntimeError, match="overlap"):
             bad()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_forward_and_inverse_are_adjoint(ext, cuda_device, dtype, interleaved):
+    """<dy, R x> = <R' dy, x> between the two directions of the kernel, on 64 columns of wider heads. Either side is off by at most
+    its results' tolerance (derived in paged_reference) times the other factor, summed."""
+    g = torch.Generator(device=cuda_device).manual_seed(11)
+    x, dy = (torch.randn(37, 6, 192, generator=g, device=cuda_device).to(dtype)[..., o:o + 64] for o in (128, 64))
+    pos = torch.randint(0, 1 << 20, (37,), generator=g, device=cuda_device, dtype=torch.int32)
+    freq = 10000.0 ** (-torch.arange(32, dtype=torch.float64, device=cuda_device) / 32)
+    y = ext.mla_rope_forward(x, pos, freq, interleaved, 1.5)
+    dx = ext.mla_rope_forward(dy, pos, freq, interleaved, 1.5, True)
+    _, tol_y = ref.rotate(x, pos, freq, interleaved, 1.5)
+    _, tol_dx = ref.rotate(dy, pos, freq, interleaved, 1.5, True)
+    left, right = (dy.double() * y.double()).sum(2), (dx.double() * x.double()).sum(2)
+    assert ((left - right).abs() <= (dy.double().abs() * tol_y + x.double().abs() * tol_dx).sum(2)).all()
+    assert (left.abs() > 1).any()                     # not all lost in the tolerance
