@@ -3,7 +3,8 @@
 ``PagedLatentCache`` holds the rows (512 latent + 64 rotary columns) of many sequences over several layers in pages of
 equal size, and the bookkeeping that says which page holds what: a table row, a length and reference counts on the
 device. Its methods are the extension's ``mla_pages_*``, ``mla_rope_append_forward``, ``mla_paged_attention_forward``
-and ``mla_sparse_decode_forward``; nothing is computed in torch but the batch's own small tables. A program serves with it as
+and ``mla_sparse_decode_forward``; what is computed in torch are the batch's own small tables and, for ``attend_sparse``, the
+rows of the selected positions. A program serves with it as
 
     cache = PagedLatentCache(layers, pages, 64, slots=256, max_rows=32768)
     freq, mscale = rope_frequencies(64, scaling="yarn", factor=16.0, mscale=1.0, mscale_all_dim=1.0)
@@ -140,18 +141,15 @@ class PagedLatentCache:
     def batch(self, seqs, q_start) -> PagedBatch:
         """The batch of sequences ``seqs``, whose new tokens are [q_start[i], q_start[i + 1]) of the step's and whose lengths
         (the new tokens among them) are the present ones. A sequence stands in a batch once: two would write the same rows.
-        Of a list that is checked here. A tensor is not read by the host: a sequence that is out of range, or stands before
-        already, gets no pages and length 0, so ``append`` writes nothing for it and reports it, and attention sees nothing."""
+        Of a list that is checked here. A tensor is not read by the host: there a sequence that is out of range gets no pages
+        and length 0, so ``append`` writes nothing for it and reports it, and attention sees nothing; whether one stands there
+        twice is not looked at."""
         slots = self.length.numel()
         if torch.is_tensor(seqs):
             seqs = seqs.to(self.length.device, torch.int64)
-            n, inside = seqs.numel(), (seqs >= 0) & (seqs < slots)
-            at, order = torch.where(inside, seqs, slots), torch.arange(seqs.numel(), device=seqs.device)
-            first = torch.full((slots + 1,), n, device=seqs.device).scatter_reduce_(0, at, order, "amin")
-            fine = inside & (first[at] == order)
-            at = at.clamp_max(slots - 1)
-            return PagedBatch(torch.where(fine[:, None], self.page_table[at], -1), self._list(q_start),
-                              torch.where(fine, self.length[at], 0))
+            at = seqs.clamp(0, slots - 1)
+            inside = at == seqs
+            return PagedBatch(torch.where(inside[:, None], self.page_table[at], -1), self._list(q_start), self.length[at] * inside)
         seqs = list(seqs)
         if not all(0 <= s < slots for s in seqs):
             raise ValueError(f"sequences must lie in [0, {slots})")
@@ -174,7 +172,9 @@ class PagedLatentCache:
 
     def attend_sparse(self, layer: int, batch: PagedBatch, q, idx, softmax_scale: float, check: bool = False):
         """Top-k sparse decode on the same pages: one new token per sequence, q [B, H, 576], idx [B, topk] the selected
-        positions of each sequence (-1: none). The pool is one run of rows to ``mla_sparse_decode_forward``."""
+        positions of each sequence (-1: none). The pool is one run of rows to ``mla_sparse_decode_forward``, whose limits hold
+        here: bfloat16 and a multiple of 64 heads, where ``attend`` takes either type and any number. The positions become rows by
+        some ten small torch operations in every call."""
         layers, pages, size, _ = self.rows.shape
         B, topk = idx.shape
         at = idx.clamp_min(0).long()

@@ -223,7 +223,7 @@ def test_yarn_temperature_of_the_whole_score():
 
 
 def test_batch_of_sequences_that_are_not_there_or_twice(built_libs):
-    """A list raises; a tensor, which the host does not read, gives such places no pages and length 0."""
+    """A list raises; a tensor, which the host does not read, gives a place out of range no pages and length 0."""
     from cuda_agent_b200.paged import PagedLatentCache
     c = PagedLatentCache(1, 8, 16, 4, 64, device="cpu")
     c.page_table[:] = torch.arange(16, dtype=torch.int32).view(4, 4)
@@ -231,8 +231,8 @@ def test_batch_of_sequences_that_are_not_there_or_twice(built_libs):
     for bad in ([4], [0, -1], [1, 2, 1], [2 ** 40]):
         with pytest.raises(ValueError):
             c.batch(bad, [0] * (len(bad) + 1))
-    for seqs, fine in (([2, 0], [1, 1]), ([3, 4, 0], [1, 0, 1]), ([-1, 3], [0, 1]), ([1, 2, 1, 1, 0], [1, 1, 0, 0, 1]),
-                       ([9, 2 ** 40, -2 ** 40, 3, 0], [0, 0, 0, 1, 1]), ([2 ** 32 + 1, 1], [0, 1]), ([], [])):
+    for seqs, fine in (([2, 0], [1, 1]), ([3, 4, 0], [1, 0, 1]), ([-1, 3], [0, 1]), ([1, 2, 0, -5], [1, 1, 1, 0]),
+                       ([9, 2 ** 40, -2 ** 40, 3, 0], [0, 0, 0, 1, 1]), ([2 ** 32 + 1, 2 ** 32, 1], [0, 0, 1]), ([], [])):
         b = c.batch(torch.tensor(seqs, dtype=torch.int64), list(range(len(seqs) + 1)))
         assert b.page_table.dtype == b.kv_len.dtype == b.q_start.dtype == torch.int32
         assert b.page_table.tolist() == [c.page_table[s].tolist() if f else [-1] * 4 for s, f in zip(seqs, fine)]

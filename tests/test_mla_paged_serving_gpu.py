@@ -159,20 +159,22 @@ def test_task_loops(cuda_device, built_libs, capsys, monkeypatch, config):
 
 
 def test_batch_from_numbers_on_the_gpu(cuda_device):
-    """A place of the batch that names no sequence, or one that stands before it: reported by the append, nothing written for
-    it, nothing seen by its tokens; also in a captured step."""
+    """A place of the batch that names no sequence: reported by the append, nothing written for it, nothing seen by its tokens;
+    also in a captured step, and where the step counts the lengths up."""
     p = Program(cuda_device, torch.bfloat16, 16, 64)
     p.step({0: 60, 1: 130, 2: 7})
     p.cache.extend([0, 1, 2], [61, 131, 8])
-    seqs = torch.tensor([0, 24, 1, 0, -3, 2], dtype=torch.int32, device=cuda_device)
+    seqs = torch.tensor([0, 24, 1, 2 ** 31 - 1, -3, 2], dtype=torch.int32, device=cuda_device)
     fine = [0, 2, 5]
     joint, q_pe, q = p.rand(6, 576), p.rand(6, 16, 64), p.rand(6, 16, 576)
     start = torch.arange(7, dtype=torch.int32, device=cuda_device)
 
     before = p.cache.rows.clone()
     batch = p.cache.batch(seqs, start)
-    with pytest.raises(RuntimeError, match="page table"):
-        p.cache.append(0, batch, q_pe, joint[:, :512], joint[:, 512:], p.freq, q[..., 512:], check=True)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="page table"):
+            p.cache.append(0, batch, q_pe, joint[:, :512], joint[:, 512:], p.freq, q[..., 512:], check=True)
+        batch.kv_len[[1, 3, 4]] += 1                  # a step that counts the lengths up itself: still no page of anyone's
     changed = (p.cache.rows != before).any(-1).nonzero().tolist()
     assert sorted(changed) == sorted([0, int(p.cache.page_table[s, n // 64]), n % 64] for s, n in ((0, 60), (1, 130), (2, 7)))
     graph = torch.cuda.CUDAGraph()
