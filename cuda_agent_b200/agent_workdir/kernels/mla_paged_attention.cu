@@ -39,8 +39,8 @@
 // that cuts a tile; each CTA finds its run itself from q_start and kv_len. Tiles cut by a boundary leave
 // unnormalised fp32 sums, and mla_paged_merge_kernel joins them in a fixed order.
 // Every wait is bounded.
-// Measured, 128 heads, bf16, pages of 64: 1024 tokens after 7168 rows 1.78 ms (1235 TFLOP/s; 1.93 ms at the power limit,
-// 1.6 GHz); 64 sequences of 8192 rows and less, one token each, 119 to 129 us from one B200 to another (3 TB/s of the
+// Measured, 128 heads, bf16, pages of 64: 1024 tokens after 7168 rows 1.70 ms after a rest (1289 TFLOP/s), 1.93 ms in a long
+// run at the power limit (1.6 GHz); 64 sequences of 8192 rows and less, one token each, 117 and 130 us (3 TB/s of the
 // cache: a step waits for its rows, the merge is 13 us of it). 32 sequences of 4096 rows and less, 5 tokens with 24
 // heads, pages of 16: 49 us. One token with 16 heads and 1000 rows: 15 to 17 us, set-up and latency.
 #include <cuda_fp16.h>

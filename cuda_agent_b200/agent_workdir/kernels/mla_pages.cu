@@ -5,12 +5,13 @@
 // and keeps the used part of a pool dense.
 //
 // The decisions of a call (which pages, is there room, is the list sound) are made by one CTA that scans the
-// counts, 4096 at a time, and stops when it has found enough; nothing is changed before they are all made. The
+// counts, 4096 at a time, and stops when it has found enough. extend and fork change nothing before they are all made, or
+// nothing at all; copy leaves out the pairs it refuses, free and compact the table entries that they find wrong on their way. The
 // bulk (page data, table rows) is done by the whole device in a second launch, which reads what was decided from
 // scratch memory, so the host never waits. Page data is bound by memory: 16 bytes per access, 64 per thread in
 // flight.
 // Measured: the compaction of a pool of 2048 pages of 64 rows x 8 layers, half of them in use, 95 us for the pages that move (582 MB,
-// 6.1 TB/s) and 4.7 us to decide; 4 forks of a 1500-row sequence 4.9 us to decide and 2.8 us to carry out; 200 sequences
+// 6.1 TB/s) and 5.2 us to decide; 4 forks of a 1500-row sequence 5.5 us to decide and 2.8 us to carry out; 200 sequences
 // of 8192 rows and less given back in 3.4 us.
 #include "cab_common.cuh"
 

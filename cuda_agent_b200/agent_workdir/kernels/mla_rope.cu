@@ -10,8 +10,8 @@
 // for before the sines and cosines are made.
 // Measured: 64 of 576 bf16 columns of 4096 tokens x 128 heads, in halves, 24.9 us (5.4 TB/s of the 134 MB read and
 // written; a library copy of the same strided view takes 24.7 us); 64 of 128 fp32 columns of 2047 tokens x 16 heads, inverse,
-// 3.8 us; the append of 4096 tokens with 128 heads 31.2 us (144 MB, 4.6 TB/s: the heads' 128-byte pieces of q and the cache
-// rows at once), of 32 tokens 5.9 us. (Per call, calls one behind the other.)
+// 3.9 us; the append of 4096 tokens with 128 heads 31.8 us (144 MB, 4.5 TB/s: neither DRAM, 42 %, nor issue slots, 51 %, are
+// full; its CTAs wait for starts and table entries before they write), of 32 tokens 6.0 us. (Per call, calls one behind the other.)
 #include <cuda_fp16.h>
 
 #include <type_traits>

@@ -421,7 +421,8 @@ int mla_rope_launcher(void* out, const void* x, const int* positions, const doub
 /* The new rows of a batch: rotates q_pe [T, H, 64] into q_out (strides as above) and k_pe [T, 64] as */
 /* mla_rope does (freq [32]), and writes c_kv [T, 512] | rotated k_pe into the page rows of the tokens' */
 /* positions. Tokens at and after q_start[batch] are left alone. A row whose page is invalid is not written */
-/* (status CAB_PAGED_BAD_PAGE). H == 0: only the cache is written. */
+/* (status CAB_PAGED_BAD_PAGE). H == 0: only the cache is written. q_out may be q_pe; it shares no byte with */
+/* another argument, nor the cache with any. No two tokens have the same row: a sequence stands in a batch once. */
 int mla_rope_append_launcher(void* q_out, const void* q_pe, const void* c_kv, const void* k_pe,
                              const cab_mla_paged_batch* batch, const double* freq, int T, int H,
                              long long q_out_stride_t, long long q_out_stride_h, long long q_stride_t,
@@ -449,7 +450,7 @@ int mla_paged_attention_launcher(void* out, float* lse, const void* q, const cab
 /* s has length[s] rows, in the first ceil(length / page_size) entries of page_table[s, max_pages]; the */
 /* entries after them are -1. Free pages are taken lowest number first, in the order of the list and of the */
 /* positions. extend and fork change everything or nothing. The lists are read again after the pool changed: */
-/* they must lie outside it. scratch: mla_pages_scratch_bytes(num_pages, n) bytes, 16-byte aligned, contents */
+/* they must lie outside it, and the three tables outside the pages. scratch: mla_pages_scratch_bytes(num_pages, n) bytes, 16-byte aligned, contents */
 /* irrelevant. */
 size_t mla_pages_scratch_bytes(int num_pages, int n);
 /* pages[:, dst[i]] = pages[:, src[i]]. src[i] < 0 or dst[i] < 0 skips the pair. A number beyond the pool, a */
@@ -472,7 +473,8 @@ int mla_pages_fork_launcher(void* pages, long long layer_stride, int layers, lon
 int mla_pages_free_launcher(int* page_table, int* length, int* refcount, int slots, int max_pages, int num_pages,
                             int page_size, const int* seqs, int n, int* status, int config, cab_stream_t stream);
 /* With U pages in use: those numbered U and above move, in ascending order, to the free ones below U; tables */
-/* and reference counts follow. */
+/* and reference counts follow. A table entry outside the pool or at a free page stays as it is and raises */
+/* CAB_PAGED_BAD_PAGE; the rest is carried out. */
 int mla_pages_compact_launcher(void* pages, long long layer_stride, int layers, long long page_bytes, int* page_table,
                                const int* length, int* refcount, int slots, int max_pages, int num_pages, int page_size,
                                void* scratch, int* status, int config, cab_stream_t stream);
