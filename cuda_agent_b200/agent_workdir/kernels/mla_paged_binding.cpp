@@ -103,7 +103,8 @@ struct Place {
   }
 };
 bool overlap(const Place& a, const Place& b) {
-  if (a.begin >= b.end || b.begin >= a.end) return false;      // the common case, and that of tensors without elements
+  if (a.begin == a.end || b.begin == b.end) return false;      // no elements
+  if (a.begin >= b.end || b.begin >= a.end) return false;      // the common case
   return may_share(bytes_of(a.t), bytes_of(b.t), b.begin - a.begin);
 }
 

@@ -370,3 +370,15 @@ def test_tables_inside_the_pages_are_refused(ext, cuda_device):
     s.want.fork([0], [1])
     ext.mla_pages_fork(pages, s.table, s.length, s.refcount, one, two, True)
     s.check()
+
+
+def test_empty_lists_anywhere(ext, cuda_device):
+    """A list without elements shares nothing, wherever it points."""
+    s = State(cuda_device, 6, 6, 14, 4, dtype=torch.int32)
+    none = (s.length[2:2], s.table[1, 3:3], s.refcount[5:5], s.pages.view(-1)[40:40])
+    for a in none:
+        ext.mla_pages_extend(s.table, s.length, s.refcount, a, a, 4, True)
+        ext.mla_pages_fork(s.pages, s.table, s.length, s.refcount, a, a, True)
+        ext.mla_pages_free(s.table, s.length, s.refcount, a, 4, True)
+        ext.mla_pages_copy(s.pages, a, a, True)
+    s.check()
