@@ -68,6 +68,7 @@ constexpr int kQBox = 16;                      // rows of the small box for Q
 constexpr uint32_t kColO = 0, kColS = 256, kColQ = 320, kTmemCols = 512;
 static_assert(kColQ + kTTiles * 32 == kTmemCols, "tensor memory");
 constexpr int kMaxBatch = 16384;
+constexpr float kLog2e = 1.4426950408889634f;
 enum { kWaitN = 211, kWaitFree, kWaitV, kWaitS, kWaitP, kWaitPv, kWaitQ, kWaitRead, kWaitPeer };
 
 // A sequence as this call sees it: tokens [tok, tok + n), `len` cache rows, the first token at position pos.
@@ -1239,7 +1240,7 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
       (batch->batch > 0 && (!batch->page_table || !batch->kv_len)))
     return CAB_ERR_BAD_ARGUMENT;
   if (batch->num_pages <= 0 || batch->page_size <= 0 || batch->max_pages <= 0 || window < 0 || !(softmax_scale > 0.f) ||
-      !(softmax_scale < 3.0e38f) || (batch->dtype != CAB_BF16 && batch->dtype != CAB_F16))
+      !(softmax_scale * kLog2e < 3.4e38f) || (batch->dtype != CAB_BF16 && batch->dtype != CAB_F16))
     return CAB_ERR_BAD_ARGUMENT;
   if (batch->page_stride % 8 || batch->token_stride % 8 || batch->token_stride < kD || batch->page_stride < kD)
     return CAB_ERR_BAD_ARGUMENT;
@@ -1267,7 +1268,7 @@ extern "C" int mla_paged_attention_launcher(void* out, float* lse, const void* q
   p.causal = causal != 0;
   p.window = window < (long long)batch->max_pages * batch->page_size ? window : 0;   // wider than any history: none
   p.rows_cap = rows_cap_of(T, H);
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = softmax_scale * kLog2e;
   const int sms = cab::sm_count();
   if (sms < 2) return CAB_ERR_LAUNCH;
   p.pairs = sms / 2 < kPairs ? sms / 2 : kPairs;

@@ -279,3 +279,13 @@ def test_c_wrappers_pass_on_device_pointers_only(capi, monkeypatch):
                     with pytest.raises(ValueError):
                         f(**{**args, name: bad})
     assert len(calls) == 2
+
+
+def test_attention_refuses_a_scale_beyond_float(capi):
+    """The scale is taken in powers of two, which may pass the largest float where the scale itself does not."""
+    p, need = 0x10000, capi.mla_paged_workspace_bytes(8, 16)
+
+    def call(scale):                                 # rows not aligned: what comes after the look at the scale
+        return capi.lib().mla_paged_attention_launcher(p, p, p, batch(capi, rows=p + 8), 8, 16, scale, 1, 0, p, need, None, 0, None)
+
+    assert [call(scale) for scale in (2.4e38, 2.9e38, 3.4e38)] == [BAD] * 3 and call(2.3e38) == MISALIGNED
