@@ -450,8 +450,8 @@ int mla_paged_attention_launcher(void* out, float* lse, const void* q, const cab
 /* s has length[s] rows, in the first ceil(length / page_size) entries of page_table[s, max_pages]; the */
 /* entries after them are -1. Free pages are taken lowest number first, in the order of the list and of the */
 /* positions. extend and fork change everything or nothing. The lists are read again after the pool changed: */
-/* they must lie outside it, and the three tables outside the pages. scratch: mla_pages_scratch_bytes(num_pages, n) bytes, 16-byte aligned, contents */
-/* irrelevant. */
+/* they must lie outside it, and the three tables outside the pages. scratch: */
+/* mla_pages_scratch_bytes(num_pages, n) bytes, 16-byte aligned, contents irrelevant. */
 size_t mla_pages_scratch_bytes(int num_pages, int n);
 /* pages[:, dst[i]] = pages[:, src[i]]. src[i] < 0 or dst[i] < 0 skips the pair. A number beyond the pool, a */
 /* dst that stands there twice and a dst that is another pair's src skip every pair concerned and raise */
